@@ -279,6 +279,198 @@ int kmb_gemm_bf16(const KmbGemm *args);
  * the last check (synchronous calls check it themselves). */
 int kmb_gemm_check_error(void);
 
+/* ------------------------------------------------------------------ */
+/* Element types of the operators below                                */
+/* ------------------------------------------------------------------ */
+#define KMB_F32  0
+#define KMB_BF16 1   /* rounded to nearest even on output */
+
+/* ------------------------------------------------------------------ */
+/* Layer norm                                                          */
+/* ------------------------------------------------------------------ */
+/*
+ * Forward, for each of `rows` rows of D values:
+ *   mean = sum x / D,  rstd = 1 / sqrt(sum (x - mean)^2 / D + eps)
+ *   y = (x - mean) rstd weight + bias
+ * x and y are [rows, D] with ld_x / ld_y >= D elements between rows, of
+ * types x_type and y_type (an fp32 residual stream normalised into bf16
+ * GEMM operands is x_type KMB_F32, y_type KMB_BF16).  weight and bias are
+ * fp32 [D]; NULL stands for ones / zeros.  mean and rstd are optional fp32
+ * [rows] outputs.
+ *
+ * Backward: reads x, weight, dy (y_type, ld_dy) and either the forward's
+ * mean and rstd or, when both are NULL, computes them again from x and
+ * eps.  With xhat = (x - mean) rstd and g = dy weight it writes
+ *   dx = rstd (g - avg(g) - xhat avg(g xhat)) [+ dres]    (averages over D)
+ *   dweight = sum over rows of dy xhat,   dbias = sum over rows of dy
+ * dx is of x_type (ld_dx).  dres (optional, x_type, ld_dres) is the
+ * gradient that reaches x by another way, the residual path of a pre-norm
+ * block.  dweight / dbias are optional fp32 [D], overwritten, or added to
+ * when accumulate is 1; their sums run in a fixed order (the same bits
+ * every run).
+ *
+ * y may be the very tensor x, and dx the very tensor x, dy or dres (same
+ * pointer, type and row stride); any other overlap of an output with
+ * another tensor is not allowed.  rows = 0 is allowed.  All tensors are
+ * device memory of the current device, aligned to their element.
+ *
+ * workspace: device memory of kmb_layernorm_workspace_bytes(args) bytes,
+ * 16-byte aligned, used by the backward when dweight or dbias is asked
+ * for.  With NULL the call takes pooled scratch and synchronises the
+ * stream before it returns; that form, and any call while kmb_set_sync is
+ * on, is refused during stream capture.  A workspace carries nothing from
+ * one call to the next: calls that follow one another on one stream may
+ * share it, calls that can overlap may not.
+ */
+typedef struct {
+    const void *x;
+    const float *weight;
+    const float *bias;
+    void *y;
+    float *mean;
+    float *rstd;
+    const void *dy;
+    const void *dres;
+    void *dx;
+    float *dweight;
+    float *dbias;
+    void *workspace;
+    size_t workspace_bytes;
+    long rows;
+    long D;
+    long ld_x;
+    long ld_y;
+    long ld_dy;
+    long ld_dres;
+    long ld_dx;
+    float eps;
+    int x_type;
+    int y_type;
+    int accumulate;
+} KmbLayerNorm;
+
+int kmb_layernorm_fwd(const KmbLayerNorm *args);
+int kmb_layernorm_bwd(const KmbLayerNorm *args);
+/* Workspace of kmb_layernorm_bwd for args->rows and args->D (0 when the
+ * sizes are invalid). */
+size_t kmb_layernorm_workspace_bytes(const KmbLayerNorm *args);
+
+/* ------------------------------------------------------------------ */
+/* Gated linear recurrence                                             */
+/* ------------------------------------------------------------------ */
+/*
+ * One state per channel d, for every sequence:
+ *   r_t = sigmoid(gate_r_t),  i_t = sigmoid(gate_i_t)
+ *   a_t = exp(-scale softplus(decay_d) r_t)                     (0 < a <= 1)
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) i_t x_t,   h_{-1} = h0
+ *   y_t = h_t
+ * The gates are pre-activations, as the GEMM of the block's projections
+ * leaves them.  x, gate_r, gate_i, y and their gradients are of one type
+ * (KMB_F32 or KMB_BF16); decay, h0, h_last, ckpt, dh_last, dh0 and ddecay
+ * are fp32, and so is every state and sum.
+ *
+ * Sequences, without offsets: `batch` sequences of L rows.  Each tensor is
+ * a KmbRows: row t of sequence b begins at data + b batch_stride + t
+ * row_stride (elements; channels are contiguous, both strides >= D, so
+ * batch-major and time-major layouts, slices and the three parts of one
+ * fused projection all work).
+ * With offsets (device int64 [batch + 1], not decreasing, 0 <= offset <=
+ * L): sequence b has the packed rows offsets[b] .. offsets[b + 1] - 1 of
+ * tensors with L rows; batch_stride is not read.  Sequences may be empty.
+ * Rows outside every sequence are neither read nor written.
+ *
+ * h0 (may be NULL: zeros), h_last, dh_last (may be NULL: zeros) and dh0
+ * are [batch, D]; the outputs among them are optional.  h_last of an empty
+ * sequence is its h0, dh0 its dh_last.  h_last may be h0 itself, dh0 may be
+ * dh_last.
+ *
+ * ckpt (optional output of the forward, kmb_glr_ckpt_elems() floats): the
+ * state before each KMB_GLR_CHUNK-th row.  The backward reads the ckpt of
+ * the same arguments, or with NULL runs the states again into its
+ * workspace.
+ *
+ * Backward: reads dy and dh_last, writes dx, dgate_r, dgate_i, and
+ * optionally dh0 and ddecay [D] (summed over all rows in a fixed order;
+ * overwritten, or added to when accumulate is 1).
+ *
+ * An output may be the very tensor of an input of the same call (same
+ * pointer and strides); any other overlap is not allowed.  batch = 0 and
+ * L = 0 are allowed.  Device memory of the current device only, every
+ * tensor aligned to its element.
+ *
+ * workspace: kmb_glr_workspace_bytes(args, bwd) bytes of device memory,
+ * 16-byte aligned; the rules of KmbLayerNorm's workspace hold.
+ */
+#define KMB_GLR_CHUNK 64
+
+typedef struct {
+    void *data;
+    long row_stride;
+    long batch_stride;
+} KmbRows;
+
+typedef struct {
+    KmbRows x;
+    KmbRows gate_r;
+    KmbRows gate_i;
+    KmbRows y;
+    KmbRows dy;
+    KmbRows dx;
+    KmbRows dgate_r;
+    KmbRows dgate_i;
+    const float *decay;
+    const float *h0;
+    float *h_last;
+    float *ckpt;
+    const float *dh_last;
+    float *dh0;
+    float *ddecay;
+    const long *offsets;
+    void *workspace;
+    size_t workspace_bytes;
+    long batch;
+    long L;
+    long D;
+    float scale;     /* > 0 */
+    int type;
+    int accumulate;
+    int pad_;
+} KmbGLR;
+
+/* Sizes read batch, L, D and whether offsets is NULL (workspace: also
+ * whether ckpt and ddecay are); 0 when the sizes are invalid. */
+long kmb_glr_ckpt_elems(const KmbGLR *args);
+size_t kmb_glr_workspace_bytes(const KmbGLR *args, int bwd);
+int kmb_glr_fwd(const KmbGLR *args);
+int kmb_glr_bwd(const KmbGLR *args);
+
+/*
+ * One token for each row of a serving batch.  Row k of x, gate_r, gate_i
+ * and y (row_stride; batch_stride is not read) belongs to the state
+ * slots[k] of state [n_states, D] (fp32, ld_state elements between states;
+ * slots NULL: state k), which is advanced by one step in place and written
+ * to y.  A row whose slot is negative or >= n_states (padding) is left out:
+ * nothing of it is read or written.  Of several rows that name one slot
+ * the first is taken and the others are left out.
+ */
+typedef struct {
+    KmbRows x;
+    KmbRows gate_r;
+    KmbRows gate_i;
+    KmbRows y;
+    const float *decay;
+    float *state;
+    const long *slots;
+    long rows;
+    long n_states;
+    long D;
+    long ld_state;
+    float scale;
+    int type;
+} KmbGLRStep;
+
+int kmb_glr_step(const KmbGLRStep *args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -75,6 +75,40 @@ int kmb_is_device_ptr(const void *p) {
     return at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged;
 }
 
+int kmb_check_device_ptrs(const char *who, const void *const *ptrs, int n) {
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        (void)cudaGetLastError();
+        dev = -1;
+    }
+    for (int i = 0; i < n; ++i) {
+        struct cudaPointerAttributes at;
+        if (!ptrs[i]) continue;
+        if (cudaPointerGetAttributes(&at, ptrs[i]) != cudaSuccess) {
+            (void)cudaGetLastError();
+            at.type = cudaMemoryTypeUnregistered;
+        }
+        if (at.type == cudaMemoryTypeManaged) continue;
+        if (at.type != cudaMemoryTypeDevice)
+            return kmb_fail(KMB_EINVAL, "%s: every tensor must be device memory", who);
+        if (at.device != dev)
+            return kmb_fail(KMB_EINVAL, "%s: a tensor of device %d, while device %d is current", who,
+                            at.device, dev);
+    }
+    return KMB_OK;
+}
+
+int kmb_check_capture(const char *who, cudaStream_t s, int needs_pool) {
+    enum cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (!needs_pool && !kmb_sync_enabled()) return KMB_OK;
+    const cudaError_t e = cudaStreamIsCapturing(s, &st);
+    if (e != cudaSuccess) return kmb_cuda_fail(e, who);
+    if (st != cudaStreamCaptureStatusNone)
+        return kmb_fail(KMB_EINVAL, "%s: stream capture needs kmb_set_sync(0) and the caller's workspace",
+                        who);
+    return KMB_OK;
+}
+
 /* ------------------------------------------------------------------ */
 /* device pool                                                         */
 /* ------------------------------------------------------------------ */

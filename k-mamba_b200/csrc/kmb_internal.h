@@ -100,6 +100,20 @@ int kmb_scan2d_check_error(void);
 /* tcgen05 bf16 GEMM (csrc/cuda/gemm_tc.cu); operands already validated. */
 int kmb_launch_gemm_bf16(const KmbGemm *g, cudaStream_t s);
 
+/* Layer norm (csrc/cuda/layernorm.cu); arguments already validated, the
+ * workspace in place.  The backward's partial sums take
+ * kmb_layernorm_parts(rows, D) rows of 2 D floats. */
+int kmb_launch_layernorm_fwd(const KmbLayerNorm *a, cudaStream_t s);
+int kmb_launch_layernorm_bwd(const KmbLayerNorm *a, cudaStream_t s);
+long kmb_layernorm_parts(long rows, long D);
+
+/* Gated linear recurrence (csrc/cuda/glr.cu); arguments already validated,
+ * the workspace in place. */
+int kmb_launch_glr_fwd(const KmbGLR *a, cudaStream_t s);
+int kmb_launch_glr_bwd(const KmbGLR *a, cudaStream_t s);
+int kmb_launch_glr_step(const KmbGLRStep *a, cudaStream_t s);
+size_t kmb_glr_scratch_bytes(const KmbGLR *a, int bwd);
+
 /* Mamba-ND block pieces (csrc/cuda/ndblock.cu). */
 int kmb_nd_to_bf16(const float *src, long lds, void *dst, long ldd, long rows, long cols,
                    cudaStream_t s);
@@ -185,6 +199,12 @@ cudaStream_t kmb_stream(void);
 int kmb_sync_enabled(void);
 /* 1 when p is device-accessible memory (device or managed). */
 int kmb_is_device_ptr(const void *p);
+/* KMB_EINVAL unless every non-NULL pointer is device memory of the current
+ * device (or managed memory). */
+int kmb_check_device_ptrs(const char *who, const void *const *ptrs, int n);
+/* KMB_EINVAL when `s` is being captured and the call would have to
+ * synchronise: synchronous mode, or pooled scratch (needs_pool). */
+int kmb_check_capture(const char *who, cudaStream_t s, int needs_pool);
 
 /*
  * Staging of caller buffers.  kmb_stage_in/out return a device pointer:

@@ -24,6 +24,11 @@ KMB_ETIMEOUT = -4
 KMB_EUNSUPPORTED = -5
 
 KMB_SCAN1D_CHUNK = 8
+KMB_GLR_CHUNK = 64
+
+# element types of KmbLayerNorm, KmbGLR and KmbGLRStep
+KMB_F32 = 0
+KMB_BF16 = 1
 
 fp = C.c_void_p  # float* / long* passed as raw addresses
 lg = C.c_long
@@ -104,6 +109,34 @@ class KmbConvND(C.Structure):
     _fields_ = [(n, fp) for n in ("input", "kernel", "bias", "output", "dy", "dinput",
                                   "dkernel", "dbias")] + [
         ("dims", lg * 8), ("ndims", lg), ("batch", lg), ("D", lg), ("K", lg)]
+
+
+class KmbLayerNorm(C.Structure):
+    _fields_ = [(n, fp) for n in ("x", "weight", "bias", "y", "mean", "rstd", "dy", "dres", "dx",
+                                  "dweight", "dbias", "workspace")] + [
+        ("workspace_bytes", C.c_size_t)] + [
+        (n, lg) for n in ("rows", "D", "ld_x", "ld_y", "ld_dy", "ld_dres", "ld_dx")] + [
+        ("eps", C.c_float), ("x_type", C.c_int), ("y_type", C.c_int), ("accumulate", C.c_int)]
+
+
+class KmbRows(C.Structure):
+    _fields_ = [("data", fp), ("row_stride", lg), ("batch_stride", lg)]
+
+
+class KmbGLR(C.Structure):
+    _fields_ = [(n, KmbRows) for n in ("x", "gate_r", "gate_i", "y", "dy", "dx", "dgate_r",
+                                       "dgate_i")] + [
+        (n, fp) for n in ("decay", "h0", "h_last", "ckpt", "dh_last", "dh0", "ddecay", "offsets",
+                          "workspace")] + [
+        ("workspace_bytes", C.c_size_t), ("batch", lg), ("L", lg), ("D", lg),
+        ("scale", C.c_float), ("type", C.c_int), ("accumulate", C.c_int), ("pad_", C.c_int)]
+
+
+class KmbGLRStep(C.Structure):
+    _fields_ = [(n, KmbRows) for n in ("x", "gate_r", "gate_i", "y")] + [
+        (n, fp) for n in ("decay", "state", "slots")] + [
+        (n, lg) for n in ("rows", "n_states", "D", "ld_state")] + [
+        ("scale", C.c_float), ("type", C.c_int)]
 
 
 VISIT_FN = C.CFUNCTYPE(C.c_int, C.POINTER(lg), lg, lg, lg, C.c_void_p)
@@ -292,6 +325,16 @@ PROTOTYPES = {
     # tensor-core GEMM
     "kmb_gemm_bf16": (C.c_int, [C.POINTER(KmbGemm)]),
     "kmb_gemm_check_error": (C.c_int, []),
+    # layer norm
+    "kmb_layernorm_fwd": (C.c_int, [C.POINTER(KmbLayerNorm)]),
+    "kmb_layernorm_bwd": (C.c_int, [C.POINTER(KmbLayerNorm)]),
+    "kmb_layernorm_workspace_bytes": (C.c_size_t, [C.POINTER(KmbLayerNorm)]),
+    # gated linear recurrence
+    "kmb_glr_ckpt_elems": (lg, [C.POINTER(KmbGLR)]),
+    "kmb_glr_workspace_bytes": (C.c_size_t, [C.POINTER(KmbGLR), C.c_int]),
+    "kmb_glr_fwd": (C.c_int, [C.POINTER(KmbGLR)]),
+    "kmb_glr_bwd": (C.c_int, [C.POINTER(KmbGLR)]),
+    "kmb_glr_step": (C.c_int, [C.POINTER(KmbGLRStep)]),
     # 1D scan
     "kmb_scan1d_ckpt_elems": (lg, [lg, lg, lg, lg]),
     # segments and steps per segment the 1D entry points split L into
