@@ -443,6 +443,9 @@ long kmb_glr_ckpt_elems(const KmbGLR *args);
 size_t kmb_glr_workspace_bytes(const KmbGLR *args, int bwd);
 int kmb_glr_fwd(const KmbGLR *args);
 int kmb_glr_bwd(const KmbGLR *args);
+/* KMB_ETIMEOUT when a bounded wait between the tiles of a sequence gave up
+ * since the last check (synchronous calls check it themselves). */
+int kmb_glr_check_error(void);
 
 /*
  * One token for each row of a serving batch.  Row k of x, gate_r, gate_i

@@ -100,7 +100,8 @@ static int run(const KmbGLR *a, int bwd) {
     if (need && !d.workspace) d.workspace = kmb_scratch(&st, need);
     rc = st.status;
     if (!rc) rc = bwd ? kmb_launch_glr_bwd(&d, st.s) : kmb_launch_glr_fwd(&d, st.s);
-    return kmb_stage_finish(&st, rc);
+    rc = kmb_stage_finish(&st, rc);
+    return !rc && need && kmb_sync_enabled() ? kmb_glr_check_error() : rc;
 }
 
 int kmb_glr_fwd(const KmbGLR *a) { return run(a, 0); }

@@ -334,6 +334,7 @@ PROTOTYPES = {
     "kmb_glr_workspace_bytes": (C.c_size_t, [C.POINTER(KmbGLR), C.c_int]),
     "kmb_glr_fwd": (C.c_int, [C.POINTER(KmbGLR)]),
     "kmb_glr_bwd": (C.c_int, [C.POINTER(KmbGLR)]),
+    "kmb_glr_check_error": (C.c_int, []),
     "kmb_glr_step": (C.c_int, [C.POINTER(KmbGLRStep)]),
     # 1D scan
     "kmb_scan1d_ckpt_elems": (lg, [lg, lg, lg, lg]),

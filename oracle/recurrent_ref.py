@@ -122,7 +122,9 @@ def glr_bwd(x, gr, gi, decay, scale, h0, dy, dh_last):
         eG = ec + 2 * U * (np.abs(G) + np.abs(c))
         share, mem = q["kappa"][t] * b, u * a * hp[t]
         udu = G * (share - mem)
-        e = q["e_u"][t] + q["e_b"][t]
+        # a relative error e of u is (1 - u) e of u a = u e^-u, and at most
+        # (1 + 2 u) e of kappa = u / (e^2u - 1)
+        e = (1 + 2 * u) * q["e_u"][t] + q["e_b"][t]
         e_udu = eG * np.abs(share - mem) + np.abs(G) * (e * (np.abs(share) + np.abs(mem)) + u * a * ep[t])
         out["udu"][t], err["udu"][t] = udu, e_udu
         out["dx"][t] = G * q["root"][t] * q["i"][t]
