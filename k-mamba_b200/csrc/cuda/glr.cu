@@ -13,7 +13,7 @@
  * kappa b, so nothing divides by a vanishing root: kappa -> 1/2 at u = 0.)
  *
  * Both directions are one pass over the data.  A CTA takes a tile of rows x
- * 64 channels: a warp owns a run of consecutive rows, a lane two channels.
+ * 128 channels: a warp owns a run of consecutive rows, a lane four channels.
  * A run is first reduced to its affine map h -> A h + H, the maps of a
  * tile's warps are joined through shared memory, and the maps of the tiles
  * of one channel group through global memory: a tile publishes its map,
@@ -32,68 +32,95 @@
 namespace {
 
 constexpr int kChunk = KMB_GLR_CHUNK;
-constexpr int kC = 64;      /* channels of a tile: two a lane */
-constexpr int kWindow = 16; /* tiles before its own that a tile looks at */
+constexpr int kV = 4;       /* channels of a lane */
+constexpr int kC = 32 * kV; /* channels of a tile */
+constexpr int kWindow = 12; /* tiles before its own that a tile looks at */
 constexpr unsigned kUnset = 0xffffffffu; /* workspace word not written yet */
 
 /* set when a wait for another tile's state gave up (kmb_glr_check_error) */
 __device__ int g_glr_error;
 
 /* ------------------------------------------------------------------ */
-/* two channels of one row                                              */
+/* four channels of one row, as two FFMA2 pairs                          */
 /* ------------------------------------------------------------------ */
 
-__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return kmb_f2(a.x - b.x, a.y - b.y); }
-__device__ __forceinline__ float2 neg2(float2 a) { return kmb_f2(-a.x, -a.y); }
+struct F4 {
+    float2 l, h;
+};
+__device__ __forceinline__ F4 f4s(float v) { return {kmb_f2s(v), kmb_f2s(v)}; }
+__device__ __forceinline__ F4 f4(float4 v) { return {kmb_f2(v.x, v.y), kmb_f2(v.z, v.w)}; }
+__device__ __forceinline__ float4 v4(F4 a) { return make_float4(a.l.x, a.l.y, a.h.x, a.h.y); }
+__device__ __forceinline__ F4 operator+(F4 a, F4 b) { return {kmb_add2(a.l, b.l), kmb_add2(a.h, b.h)}; }
+__device__ __forceinline__ F4 operator*(F4 a, F4 b) { return {kmb_mul2(a.l, b.l), kmb_mul2(a.h, b.h)}; }
+__device__ __forceinline__ F4 fma4(F4 a, F4 b, F4 c) {
+    return {kmb_fma2(a.l, b.l, c.l), kmb_fma2(a.h, b.h, c.h)};
+}
+template <typename Fn>
+__device__ __forceinline__ F4 each(Fn f) { /* f(channel) */
+    return {kmb_f2(f(0), f(1)), kmb_f2(f(2), f(3))};
+}
+__device__ __forceinline__ float get(const F4 &a, int k) {
+    return k == 0 ? a.l.x : k == 1 ? a.l.y : k == 2 ? a.h.x : a.h.y;
+}
 
-/* VEC: channels 2 lane, 2 lane + 1 in one access; else lane and lane + 32,
- * for odd widths, strides and addresses (every access still covers a
- * contiguous piece of the row). */
+/* VEC: channels 4 lane .. 4 lane + 3 in one access; else lane + 32 k, for
+ * odd widths, strides and addresses (every access still covers a contiguous
+ * piece of the row).  m: bit k set where channel k exists. */
 template <typename T>
 struct Raw;
 template <>
 struct Raw<float> {
-    typedef float2 type;
-    static __device__ __forceinline__ float2 f(float2 v) { return v; }
+    typedef float4 type;
+    static __device__ __forceinline__ F4 f(float4 v) { return f4(v); }
     template <bool VEC>
-    static __device__ __forceinline__ float2 load(const float *p, bool ok0, bool ok1) {
-        if (VEC) return ok0 ? __ldcs(reinterpret_cast<const float2 *>(p)) : kmb_f2s(0.f);
-        return kmb_f2(ok0 ? __ldcs(p) : 0.f, ok1 ? __ldcs(p + 32) : 0.f);
+    static __device__ __forceinline__ float4 load(const float *p, unsigned m) {
+        if (VEC) return m ? __ldcs(reinterpret_cast<const float4 *>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        return make_float4(m & 1 ? __ldcs(p) : 0.f, m & 2 ? __ldcs(p + 32) : 0.f,
+                           m & 4 ? __ldcs(p + 64) : 0.f, m & 8 ? __ldcs(p + 96) : 0.f);
     }
     template <bool VEC>
-    static __device__ __forceinline__ void store(float *p, float2 v, bool ok0, bool ok1) {
+    static __device__ __forceinline__ void store(float *p, F4 v, unsigned m) {
         if (VEC) {
-            if (ok0) __stcs(reinterpret_cast<float2 *>(p), v);
+            if (m) __stcs(reinterpret_cast<float4 *>(p), v4(v));
             return;
         }
-        if (ok0) __stcs(p, v.x);
-        if (ok1) __stcs(p + 32, v.y);
+        if (m & 1) __stcs(p, v.l.x);
+        if (m & 2) __stcs(p + 32, v.l.y);
+        if (m & 4) __stcs(p + 64, v.h.x);
+        if (m & 8) __stcs(p + 96, v.h.y);
     }
 };
 template <>
 struct Raw<__nv_bfloat16> {
-    typedef unsigned type; /* the first channel in the low half */
-    static __device__ __forceinline__ float2 f(unsigned v) {
-        return kmb_f2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    typedef uint2 type; /* the even channels in the low halves */
+    static __device__ __forceinline__ F4 f(uint2 v) {
+        return {kmb_f2(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u)),
+                kmb_f2(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u))};
     }
-    template <bool VEC>
-    static __device__ __forceinline__ unsigned load(const __nv_bfloat16 *p, bool ok0, bool ok1) {
-        if (VEC) return ok0 ? __ldcs(reinterpret_cast<const unsigned *>(p)) : 0u;
-        const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
-        const unsigned a = ok0 ? __ldcs(q) : 0u, b = ok1 ? __ldcs(q + 32) : 0u;
-        return a | b << 16;
-    }
-    template <bool VEC>
-    static __device__ __forceinline__ void store(__nv_bfloat16 *p, float2 v, bool ok0, bool ok1) {
+    static __device__ __forceinline__ unsigned pack(float2 v) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
-        const unsigned u = *reinterpret_cast<const unsigned *>(&h);
+        return *reinterpret_cast<const unsigned *>(&h);
+    }
+    template <bool VEC>
+    static __device__ __forceinline__ uint2 load(const __nv_bfloat16 *p, unsigned m) {
+        if (VEC) return m ? __ldcs(reinterpret_cast<const uint2 *>(p)) : make_uint2(0u, 0u);
+        const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
+        const unsigned a = m & 1 ? __ldcs(q) : 0u, b = m & 2 ? __ldcs(q + 32) : 0u;
+        const unsigned c = m & 4 ? __ldcs(q + 64) : 0u, d = m & 8 ? __ldcs(q + 96) : 0u;
+        return make_uint2(a | b << 16, c | d << 16);
+    }
+    template <bool VEC>
+    static __device__ __forceinline__ void store(__nv_bfloat16 *p, F4 v, unsigned m) {
+        const uint2 u = make_uint2(pack(v.l), pack(v.h));
         if (VEC) {
-            if (ok0) __stcs(reinterpret_cast<unsigned *>(p), u);
+            if (m) __stcs(reinterpret_cast<uint2 *>(p), u);
             return;
         }
         unsigned short *q = reinterpret_cast<unsigned short *>(p);
-        if (ok0) __stcs(q, (unsigned short)u);
-        if (ok1) __stcs(q + 32, (unsigned short)(u >> 16));
+        if (m & 1) __stcs(q, (unsigned short)u.x);
+        if (m & 2) __stcs(q + 32, (unsigned short)(u.x >> 16));
+        if (m & 4) __stcs(q + 64, (unsigned short)u.y);
+        if (m & 8) __stcs(q + 96, (unsigned short)(u.y >> 16));
     }
 };
 
@@ -123,132 +150,158 @@ __device__ __forceinline__ float sqrt_mufu(float v) {
  * Polynomials of the exponent u on [0, kWeak], fitted for minimax relative
  * error with the constant term held (iteratively reweighted least squares
  * on Chebyshev nodes); in fp32 Horner form each is within 7e-8:
- *   (1 - e^-u) / u                    2.9e-9 in real arithmetic
+ *   (e^-u - 1) / u                    2.9e-9 in real arithmetic
  *   sqrt((1 - e^-2u) / (2 u))         4.8e-9
  *   kappa = u / (e^2u - 1)            3.4e-9
  * A channel whose rate is at most kWeak needs no exponential of u, no
- * square root and no cancelling 1 - a^2, and its recurrence runs on w = 1 -
- * a as h + (b - w h): a memory of 1 / w steps multiplies the error of the
- * decay, and a itself, next to 1, cannot hold w to more than 2^-25 / w.
+ * square root and no cancelling 1 - a^2, and its recurrence runs on a - 1
+ * as h + (b + (a - 1) h): a memory of 1 / (1 - a) steps multiplies the error
+ * of the decay, and a itself, next to 1, cannot hold it to more than
+ * 2^-25 / (1 - a).
  */
 constexpr float kWeak = 0.25f;
 
-__device__ __forceinline__ float2 poly4(float2 u, float c0, float c1, float c2, float c3, float c4) {
-    float2 p = kmb_fma2(kmb_f2s(c4), u, kmb_f2s(c3));
-    p = kmb_fma2(p, u, kmb_f2s(c2));
-    p = kmb_fma2(p, u, kmb_f2s(c1));
-    return kmb_fma2(p, u, kmb_f2s(c0));
+__device__ __forceinline__ F4 poly4(F4 u, float c0, float c1, float c2, float c3, float c4) {
+    F4 p = fma4(f4s(c4), u, f4s(c3));
+    p = fma4(p, u, f4s(c2));
+    p = fma4(p, u, f4s(c1));
+    return fma4(p, u, f4s(c0));
 }
-__device__ __forceinline__ float2 poly_w(float2 u) {
-    return poly4(u, 1.f, -0.49999964237213135f, 0.1666528880596161f, -0.04150013253092766f,
-                 0.007530174218118191f);
+__device__ __forceinline__ F4 poly_expm1(F4 u) {
+    return poly4(u, -1.f, 0.49999964237213135f, -0.1666528880596161f, 0.04150013253092766f,
+                 -0.007530174218118191f);
 }
-__device__ __forceinline__ float2 poly_root(float2 u) {
+__device__ __forceinline__ F4 poly_root(F4 u) {
     return poly4(u, 1.f, -0.49999940395355225f, 0.20831027626991272f, -0.06222091242671013f,
                  0.01236682292073965f);
 }
-__device__ __forceinline__ float2 poly_kappa(float2 u) {
+__device__ __forceinline__ F4 poly_kappa(F4 u) {
     return poly4(u, 0.5f, -0.5000002980232239f, 0.1666753739118576f, -8.377274934900925e-05f,
                  -0.010830916464328766f);
 }
 
 /* Per channel: rate, and sqrt(2 rate) for root = sqrt(2 u) sqrt((1 - e^-2u) / 2u). */
 struct Rates {
-    float2 rate, sroot;
+    F4 rate, sroot;
 };
 
-/* Of one row: c is 1 - a (WEAK) or a, q = sqrt(r) = (1 + e^-gate_r)^-1/2, i,
+/* Of one row: c is a - 1 (WEAK) or a, q = sqrt(r) = (1 + e^-gate_r)^-1/2, i,
  * and si = root i. */
 struct Terms {
-    float2 c, q, i, si;
+    F4 c, q, i, si;
 };
 
 template <bool WEAK>
-__device__ __forceinline__ Terms terms(float2 gr, float2 gi, const Rates &k) {
+__device__ __forceinline__ Terms terms(F4 gr, F4 gi, const Rates &k) {
     Terms t;
-    const float2 nl = kmb_f2s(-KMB_LOG2E), one = kmb_f2s(1.f);
-    const float2 er = kmb_add2(kmb_ex2_2(kmb_mul2(gr, nl)), one);
-    const float2 ei = kmb_add2(kmb_ex2_2(kmb_mul2(gi, nl)), one);
-    t.q = kmb_f2(rsqrt_mufu(er.x), rsqrt_mufu(er.y));
-    t.i = kmb_f2(rcp_mufu(ei.x), rcp_mufu(ei.y));
-    const float2 u = kmb_mul2(k.rate, kmb_mul2(t.q, t.q));
-    const float2 w = kmb_mul2(u, poly_w(u));
-    float2 root = kmb_mul2(kmb_mul2(k.sroot, t.q), poly_root(u));
+    const F4 nl = f4s(-KMB_LOG2E), one = f4s(1.f);
+    gr = gr * nl;
+    gi = gi * nl;
+    const F4 er = each([&](int n) { return kmb_ex2(get(gr, n)); }) + one;
+    const F4 ei = each([&](int n) { return kmb_ex2(get(gi, n)); }) + one;
+    t.q = each([&](int n) { return rsqrt_mufu(get(er, n)); });
+    t.i = each([&](int n) { return rcp_mufu(get(ei, n)); });
+    const F4 u = k.rate * (t.q * t.q);
+    const F4 m = u * poly_expm1(u);
+    F4 root = k.sroot * t.q * poly_root(u);
     if (WEAK) {
-        t.c = w;
+        t.c = m;
     } else {
-        const float2 e = kmb_ex2_2(kmb_mul2(u, nl));
-        t.c = kmb_f2(u.x <= kWeak ? 1.f - w.x : e.x, u.y <= kWeak ? 1.f - w.y : e.y);
-        root = kmb_f2(u.x <= kWeak ? root.x : sqrt_mufu(fmaf(-e.x, e.x, 1.f)),
-                      u.y <= kWeak ? root.y : sqrt_mufu(fmaf(-e.y, e.y, 1.f)));
+        const F4 un = u * nl;
+        const F4 e = each([&](int n) { return kmb_ex2(get(un, n)); });
+        t.c = each([&](int n) { return get(u, n) <= kWeak ? 1.f + get(m, n) : get(e, n); });
+        root = each([&](int n) {
+            return get(u, n) <= kWeak ? get(root, n) : sqrt_mufu(fmaf(-get(e, n), get(e, n), 1.f));
+        });
     }
-    t.si = kmb_mul2(root, t.i);
+    t.si = root * t.i;
     return t;
 }
 
 /* a h + b */
 template <bool WEAK>
-__device__ __forceinline__ float2 advance(float2 c, float2 h, float2 b) {
-    return WEAK ? kmb_add2(h, kmb_fma2(neg2(c), h, b)) : kmb_fma2(c, h, b);
+__device__ __forceinline__ F4 advance(F4 c, F4 h, F4 b) {
+    return WEAK ? h + fma4(c, h, b) : fma4(c, h, b);
 }
 /* a A */
 template <bool WEAK>
-__device__ __forceinline__ float2 shrink(float2 c, float2 A) {
-    return WEAK ? kmb_fma2(neg2(c), A, A) : kmb_mul2(c, A);
+__device__ __forceinline__ F4 shrink(F4 c, F4 A) {
+    return WEAK ? fma4(c, A, A) : c * A;
 }
 
 /* ------------------------------------------------------------------ */
-/* affine maps; A = -1 marks a constant one (a sequence began inside)    */
+/* affine maps h -> A h + H; A = -1 marks a constant one                 */
 /* ------------------------------------------------------------------ */
 
-__device__ __forceinline__ float apply(float A, float H, float h) { return A < 0.f ? H : fmaf(A, h, H); }
+struct Map {
+    F4 A, H;
+};
+
+/* MARKED: constant maps occur (a sequence began inside, a final state) */
+template <bool MARKED>
+__device__ __forceinline__ F4 apply(const Map &m, F4 h) {
+    const F4 r = fma4(m.A, h, m.H);
+    if (!MARKED) return r;
+    return each([&](int n) { return get(m.A, n) < 0.f ? get(m.H, n) : get(r, n); });
+}
 
 /* the map of `first` then `then` */
-__device__ __forceinline__ float2 join(float2 first, float2 then) {
-    if (then.x < 0.f) return then;
-    return kmb_f2(first.x < 0.f ? -1.f : first.x * then.x, fmaf(then.x, first.y, then.y));
+template <bool MARKED>
+__device__ __forceinline__ Map join(const Map &first, const Map &then) {
+    Map r;
+    r.H = apply<MARKED>(then, first.H);
+    r.A = first.A * then.A;
+    if (MARKED)
+        r.A = each([&](int n) { return get(first.A, n) < 0.f || get(then.A, n) < 0.f ? -1.f : get(r.A, n); });
+    return r;
 }
 
+/* What tiles show one another: [place in the chain][chain][lane] of four
+ * channels.  Every word is written once, and was kUnset (the workspace is
+ * filled at the start of the call): a word that is not kUnset is the value
+ * itself, so no fence orders flags against data. */
+struct Shown {
+    float4 *A, *H, *end; /* map, final state */
+    long step;           /* entries between places of a chain */
+};
+
+__device__ __forceinline__ bool peek(const float4 *p, F4 &v) {
+    unsigned a, b, c, d;
+    asm volatile("ld.relaxed.gpu.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+                 : "l"(p)
+                 : "memory");
+    v = {kmb_f2(__uint_as_float(a), __uint_as_float(b)), kmb_f2(__uint_as_float(c), __uint_as_float(d))};
+    return a != kUnset && b != kUnset && c != kUnset && d != kUnset;
+}
 __device__ __forceinline__ float not_unset(float v) {
     return __float_as_uint(v) == kUnset ? __uint_as_float(0x7fffffffu) : v;
 }
-
-__device__ __forceinline__ unsigned peek(const float *p) {
-    unsigned v;
-    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ void show(float *p, float v) {
-    asm volatile("st.relaxed.gpu.global.f32 [%0], %1;" ::"l"(p), "f"(not_unset(v)) : "memory");
+__device__ __forceinline__ void show(float4 *p, F4 v) {
+    asm volatile("st.relaxed.gpu.global.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(not_unset(v.l.x)),
+                 "f"(not_unset(v.l.y)), "f"(not_unset(v.h.x)), "f"(not_unset(v.h.y))
+                 : "memory");
 }
 
-/* What tiles show one another: [position in the chain][chain][channel].
- * Every word is written once, and was kUnset (the workspace is filled at
- * the start of the call): a word that is not kUnset is the value itself, so
- * no fence orders flags against data. */
-struct Shown {
-    float *A, *H, *end; /* map, final state */
-    long step;          /* words between positions of a chain */
-};
-
-/* The map of a position, or as a constant one its final state: waits for
+/* The map of a place, or as a constant one its final state: waits for
  * whichever comes first (last: for the final state).  Bounded by about 2^31
  * cycles; then the error word is set and later waits return at once. */
-__device__ __forceinline__ float2 look(const Shown &s, long pos, int ch, bool last) {
-    const long o = pos * s.step + ch;
+__device__ __forceinline__ Map look(const Shown &s, long o, bool last) {
     const long long t0 = clock64();
+    Map m;
     for (int n = 0;; ++n) {
-        const unsigned e = peek(s.end + o);
-        if (e != kUnset) return kmb_f2(-1.f, __uint_as_float(e));
-        if (!last) {
-            const unsigned a = peek(s.A + o), h = peek(s.H + o);
-            if (a != kUnset && h != kUnset) return kmb_f2(__uint_as_float(a), __uint_as_float(h));
+        if (peek(s.end + o, m.H)) {
+            m.A = f4s(-1.f);
+            return m;
         }
+        if (!last && peek(s.A + o, m.A) && peek(s.H + o, m.H)) return m;
         if ((n & 63) == 63) {
-            if (*reinterpret_cast<volatile int *>(&g_glr_error)) return kmb_f2(-1.f, 0.f);
-            if (clock64() - t0 > (1ll << 31)) {
-                atomicExch(&g_glr_error, 1);
-                return kmb_f2(-1.f, 0.f);
+            const bool late = clock64() - t0 > (1ll << 31);
+            if (late) atomicExch(&g_glr_error, 1);
+            if (late || *reinterpret_cast<volatile int *>(&g_glr_error)) {
+                m.A = f4s(-1.f);
+                m.H = f4s(0.f);
+                return m;
             }
         }
     }
@@ -265,7 +318,7 @@ struct Dev {
     int states_only;            /* forward: checkpoints alone are wanted */
     const float *ckpt_in;
     float *ckpt_out;
-    float *part;                /* [tiles * batch][groups * 64] sums of u dL/du */
+    float *part;                /* [tiles * batch][groups * kC] sums of u dL/du */
     unsigned *ticket;
     Shown shown;
 };
@@ -274,19 +327,21 @@ struct Place {
     long pos, chain, b, ch0; /* place in the chain, chain, sequence (0 when packed), first channel */
 };
 
-/* Tiles are taken in the order of their positions: a tile waits only for
- * tiles that another CTA has taken before. */
+/* Tiles are taken in the order of their places: a tile waits only for tiles
+ * that another CTA has taken before. */
 __device__ __forceinline__ Place place(const Dev &p, unsigned *slot) {
     if (p.tiles > 1) {
         if (threadIdx.x == 0) *slot = atomicAdd(p.ticket, 1u) + 1u; /* the fill makes it -1 */
         __syncthreads();
     }
-    const long id = p.tiles > 1 ? (long)*slot : (long)blockIdx.x;
+    const unsigned id = p.tiles > 1 ? *slot : blockIdx.x;
     Place t;
-    t.pos = id / p.chains;
-    t.chain = id - t.pos * p.chains;
-    t.b = t.chain / p.groups;
-    t.ch0 = (t.chain - t.b * p.groups) * kC;
+    const unsigned pos = id / (unsigned)p.chains, chain = id - pos * (unsigned)p.chains;
+    const unsigned b = chain / (unsigned)p.groups;
+    t.pos = pos;
+    t.chain = chain;
+    t.b = b;
+    t.ch0 = (long)(chain - b * (unsigned)p.groups) * kC;
     return t;
 }
 
@@ -334,7 +389,8 @@ __device__ void map_rows(RowMap<ROWS> &m, const KmbGLR &a, long row0) {
             const long from = lo > row0 ? lo : row0, to = hi < end ? hi : end;
             for (long r = from; r < to; ++r) {
                 m.seq[r - row0] = (int)(s + lane);
-                m.edge[r - row0] = (unsigned char)((r == (lo < 0 ? 0 : lo) ? 1 : 0) | (r == (hi > a.L ? a.L : hi) - 1 ? 2 : 0));
+                m.edge[r - row0] = (unsigned char)((r == (lo < 0 ? 0 : lo) ? 1 : 0) |
+                                                   (r == (hi > a.L ? a.L : hi) - 1 ? 2 : 0));
             }
             if (__any_sync(~0u, s + lane < a.batch && lo >= end)) break;
         }
@@ -364,92 +420,107 @@ __device__ void empty_sequences(const KmbGLR &a, const float *from, float *to, l
     }
 }
 
-template <typename T>
-__device__ __forceinline__ T *row_ptr(const KmbRows &r, long b, long t, long d) {
-    return (T *)r.data + b * r.batch_stride + t * r.row_stride + d;
-}
-
-/* The lane's channels: the first, whether each exists. */
+/* The lane's channels: the first, and which exist. */
 template <bool VEC>
 struct Lane {
     long d;
-    int off; /* within the group */
-    bool ok0, ok1;
-    static constexpr int kNext = VEC ? 1 : 32; /* to the second channel */
+    unsigned m;
+    int lane;
+    static constexpr int kNext = VEC ? 1 : 32; /* to the next channel */
     __device__ __forceinline__ Lane(long ch0, long D) {
-        const int lane = threadIdx.x % 32;
-        off = VEC ? 2 * lane : lane;
-        d = ch0 + off;
-        ok0 = d < D;
-        ok1 = d + kNext < D;
+        lane = threadIdx.x % 32;
+        d = ch0 + (VEC ? kV * lane : lane);
+        m = 0;
+#pragma unroll
+        for (int k = 0; k < kV; ++k) m |= d + k * kNext < D ? 1u << k : 0u;
     }
-    /* a [.., D] fp32 vector of the channels */
-    __device__ __forceinline__ float2 get(const float *p) const {
-        return kmb_f2(p && ok0 ? p[d] : 0.f, p && ok1 ? p[d + kNext] : 0.f);
+    /* a [.., D] fp32 vector at the channels, 0 where NULL */
+    __device__ __forceinline__ F4 at(const float *p) const {
+        return each([&](int k) { return p && (m >> k & 1) ? p[d + k * kNext] : 0.f; });
     }
-    __device__ __forceinline__ void put(float *p, float2 v) const {
-        if (p && ok0) p[d] = v.x;
-        if (p && ok1) p[d + kNext] = v.y;
+    __device__ __forceinline__ void put(float *p, F4 v) const {
+#pragma unroll
+        for (int k = 0; k < kV; ++k)
+            if (p && (m >> k & 1)) p[d + k * kNext] = get(v, k);
     }
 };
 
-__device__ __forceinline__ Rates rates(float2 decay, float scale) {
-    Rates k;
-    k.rate = kmb_f2(scale * softplus(decay.x), scale * softplus(decay.y));
-    k.sroot = kmb_f2(sqrtf(2.f * k.rate.x), sqrtf(2.f * k.rate.y));
-    return k;
+/* A tensor's rows of the run: pointer to the lane's channels of row j. */
+template <typename T, bool VEC>
+struct Run {
+    T *p;
+    long step;
+    __device__ __forceinline__ Run(const KmbRows &r, long b, long row, const Lane<VEC> &ln) {
+        p = (T *)r.data + b * r.batch_stride + row * r.row_stride + ln.d;
+        step = r.row_stride;
+    }
+    __device__ __forceinline__ T *operator[](int j) const { return p + j * step; }
+};
+
+/* The channels' rates, one thread a channel, and whether one of them is
+ * above kWeak.  Ends with a barrier. */
+template <bool VEC>
+__device__ __forceinline__ bool make_rates(const KmbGLR &a, long ch0, float *rate, float *sroot) {
+    bool strong = false;
+    for (int c = threadIdx.x; c < kC; c += blockDim.x) {
+        const int k = VEC ? c : (c % 32) * kV + c / 32; /* its place in the lanes' order */
+        float r = 0.f;
+        if (ch0 + c < a.D) {
+            r = a.scale * softplus(a.decay[ch0 + c]);
+            strong |= !(r <= kWeak);
+        }
+        rate[k] = r;
+        sroot[k] = sqrtf(2.f * r);
+    }
+    return __syncthreads_or(strong);
 }
 
+/* Maps of the warps of a tile. */
+template <int W>
+struct Maps {
+    float4 A[W][32], H[W][32];
+    __device__ __forceinline__ void put(int w, int lane, F4 a, F4 h) {
+        A[w][lane] = v4(a);
+        H[w][lane] = v4(h);
+    }
+    __device__ __forceinline__ Map at(int w, int lane) const { return {f4(A[w][lane]), f4(H[w][lane])}; }
+};
+
 /* Joins the tile with the ones before it in its chain and returns the state
- * that enters it.  sagg: the warps' maps; `run` the number of warps, in the
- * order that the recurrence runs; first: the state that enters the chain. */
-template <bool VEC>
-__device__ __forceinline__ float2 enter_tile(const Dev &p, const Place &at, const Lane<VEC> &ln,
-                                             const float2 (*sagg)[kC], float2 (*smap)[kC], int warps,
-                                             bool reverse, const float *first) {
-    const int warp = threadIdx.x / 32;
-    const float2 init = ln.get(first);
-    if (p.tiles == 1) return init;
+ * that enters it.  agg: the warps' maps, joined from the last when reverse;
+ * first: the state that enters the chain. */
+template <bool VEC, bool MARKED, bool REVERSE, int W>
+__device__ __forceinline__ F4 enter_tile(const Dev &p, const Place &at, const Lane<VEC> &ln,
+                                         const Maps<W> &agg, Maps<kWindow> &seen, const float *first) {
+    const int warp = threadIdx.x / 32, warps = blockDim.x / 32;
+    F4 h = ln.at(first);
+    if (p.tiles == 1) return h;
     Shown s = p.shown;
-    s.A += at.chain * kC;
-    s.H += at.chain * kC;
-    s.end += at.chain * kC;
-    float2 m0 = kmb_f2(1.f, 0.f), m1 = m0;
-    const long o = at.pos * s.step + ln.off;
-    if (warp == 0) {
-        for (int k = 0; k < warps; ++k) {
-            const int w = reverse ? warps - 1 - k : k;
-            m0 = join(m0, sagg[w][ln.off]);
-            m1 = join(m1, sagg[w][ln.off + Lane<VEC>::kNext]);
-        }
-        if (at.pos > 0 && at.pos + 1 < p.tiles) {
-            show(s.A + o, m0.x);
-            show(s.H + o, m0.y);
-            show(s.A + o + Lane<VEC>::kNext, m1.x);
-            show(s.H + o + Lane<VEC>::kNext, m1.y);
+    const long o = at.pos * s.step + at.chain * 32 + ln.lane;
+    Map m = {f4s(1.f), f4s(0.f)};
+    if (warp == 0 && at.pos + 1 < p.tiles) {
+        for (int k = 0; k < warps; ++k) m = join<MARKED>(m, agg.at(REVERSE ? warps - 1 - k : k, ln.lane));
+        if (at.pos > 0) {
+            show(s.A + o, m.A);
+            show(s.H + o, m.H);
         }
     }
-    float2 h = init;
     if (at.pos > 0) {
         const int n = at.pos < kWindow ? (int)at.pos : kWindow;
         for (int k = warp; k < n; k += warps) {
-            const bool last = k == kWindow - 1;
-            smap[k][ln.off] = look(s, at.pos - 1 - k, ln.off, last);
-            smap[k][ln.off + Lane<VEC>::kNext] = look(s, at.pos - 1 - k, ln.off + Lane<VEC>::kNext, last);
+            const Map v = look(s, o - (k + 1) * s.step, k == kWindow - 1);
+            seen.put(k, ln.lane, v.A, v.H);
         }
         __syncthreads();
-        /* from the nearest final state (or the chain's beginning) on */
-        int k0 = 0, k1 = 0;
-        while (k0 < n && !(smap[k0][ln.off].x < 0.f)) ++k0;
-        while (k1 < n && !(smap[k1][ln.off + Lane<VEC>::kNext].x < 0.f)) ++k1;
-        for (int k = k0 < n ? k0 : n - 1; k >= 0; --k) h.x = apply(smap[k][ln.off].x, smap[k][ln.off].y, h.x);
-        for (int k = k1 < n ? k1 : n - 1; k >= 0; --k)
-            h.y = apply(smap[k][ln.off + Lane<VEC>::kNext].x, smap[k][ln.off + Lane<VEC>::kNext].y, h.y);
+        /* from the nearest final states on */
+        int k = 0;
+        for (; k < n - 1; ++k) {
+            const float4 A = seen.A[k][ln.lane];
+            if (A.x < 0.f && A.y < 0.f && A.z < 0.f && A.w < 0.f) break;
+        }
+        for (; k >= 0; --k) h = apply<true>(seen.at(k, ln.lane), h);
     }
-    if (warp == 0 && at.pos + 1 < p.tiles) {
-        show(s.end + o, apply(m0.x, m0.y, h.x));
-        show(s.end + o + Lane<VEC>::kNext, apply(m1.x, m1.y, h.y));
-    }
+    if (warp == 0 && at.pos + 1 < p.tiles) show(s.end + o, apply<MARKED>(m, h));
     return h;
 }
 
@@ -457,76 +528,76 @@ __device__ __forceinline__ float2 enter_tile(const Dev &p, const Place &at, cons
 /* forward                                                              */
 /* ------------------------------------------------------------------ */
 
-constexpr int kFR = 8;           /* rows of a warp */
-constexpr int kFW = 16;          /* warps of a full CTA */
-constexpr int kFT = kFR * kFW;   /* rows of a tile */
+constexpr int kFR = 8;         /* rows of a warp */
+constexpr int kFW = 8;         /* warps of a full CTA */
+constexpr int kFT = kFR * kFW; /* rows of a tile */
+static_assert(kFT % kChunk == 0 || kChunk % kFT == 0, "checkpoints lie at the beginning of a run");
 
-template <typename T, bool VEC, bool PACKED>
+template <bool PACKED>
 struct FwdShared {
-    float2 agg[kFW][kC];
-    float2 map[kWindow][kC];
+    Maps<kFW> agg;
+    Maps<kWindow> seen;
+    float4 rate[32], sroot[32];
     unsigned slot;
     RowMap<PACKED ? kFT : 1> rows;
 };
 
 template <typename T, bool VEC, bool PACKED, bool WEAK>
 __device__ __forceinline__ void fwd_tile(const Dev &p, const Place &at, const Lane<VEC> &ln,
-                                         const Rates &rt, FwdShared<T, VEC, PACKED> &sh,
-                                         const typename Raw<T>::type (&x)[kFR],
+                                         FwdShared<PACKED> &sh, const typename Raw<T>::type (&x)[kFR],
                                          const typename Raw<T>::type (&gr)[kFR],
                                          const typename Raw<T>::type (&gi)[kFR], long row0, int live) {
-    const int warp = threadIdx.x / 32, warps = blockDim.x / 32;
-    float2 c[kFR], b[kFR];
-    float2 A = kmb_f2s(1.f), H = kmb_f2s(0.f);
+    const int warp = threadIdx.x / 32;
+    F4 c[kFR], b[kFR];
+    {
+        const Rates rt = {f4(sh.rate[ln.lane]), f4(sh.sroot[ln.lane])};
 #pragma unroll
-    for (int j = 0; j < kFR; ++j) {
-        const Terms t = terms<WEAK>(Raw<T>::f(gr[j]), Raw<T>::f(gi[j]), rt);
-        c[j] = t.c;
-        b[j] = kmb_mul2(t.si, Raw<T>::f(x[j]));
+        for (int j = 0; j < kFR; ++j) {
+            const Terms t = terms<WEAK>(Raw<T>::f(gr[j]), Raw<T>::f(gi[j]), rt);
+            c[j] = t.c;
+            b[j] = t.si * Raw<T>::f(x[j]);
+        }
     }
+    const auto in = [&](int j) { return PACKED ? sh.rows.seq[warp * kFR + j] >= 0 : j < live; };
+    const auto begins = [&](int j) { return PACKED && (sh.rows.edge[warp * kFR + j] & 1); };
+    const auto h0 = [&](int j) { return ln.at(p.a.h0 ? p.a.h0 + sh.rows.seq[warp * kFR + j] * p.a.D : nullptr); };
+    F4 A = f4s(1.f), H = f4s(0.f);
     bool fresh = false; /* a sequence begins in this run */
 #pragma unroll
     for (int j = 0; j < kFR; ++j) {
-        const int lr = warp * kFR + j;
-        if (PACKED ? sh.rows.seq[lr] >= 0 : j < live) {
-            if (PACKED && (sh.rows.edge[lr] & 1)) {
-                H = ln.get(p.a.h0 ? p.a.h0 + sh.rows.seq[lr] * p.a.D : nullptr);
+        if (in(j)) {
+            if (begins(j)) {
+                H = h0(j);
                 fresh = true;
             }
             H = advance<WEAK>(c[j], H, b[j]);
             A = shrink<WEAK>(c[j], A);
         }
     }
-    if (fresh) A = kmb_f2s(-1.f);
-    sh.agg[warp][ln.off] = kmb_f2(A.x, H.x);
-    sh.agg[warp][ln.off + Lane<VEC>::kNext] = kmb_f2(A.y, H.y);
+    sh.agg.put(warp, ln.lane, fresh ? f4s(-1.f) : A, H);
     __syncthreads();
     const float *first = !PACKED && p.a.h0 ? p.a.h0 + at.b * p.a.D : nullptr;
-    float2 h = enter_tile<VEC>(p, at, ln, sh.agg, sh.map, warps, false, first);
-    for (int w = 0; w < warp; ++w) {
-        const float2 m0 = sh.agg[w][ln.off], m1 = sh.agg[w][ln.off + Lane<VEC>::kNext];
-        h = kmb_f2(apply(m0.x, m0.y, h.x), apply(m1.x, m1.y, h.y));
-    }
+    F4 h = enter_tile<VEC, PACKED, false>(p, at, ln, sh.agg, sh.seen, first);
+    for (int w = 0; w < warp; ++w) h = apply<PACKED>(sh.agg.at(w, ln.lane), h);
     if (p.ckpt_out && row0 % kChunk == 0 && row0 < p.a.L)
         ln.put(p.ckpt_out + (at.b * p.chunks + row0 / kChunk) * p.a.D, h);
+    const Run<T, VEC> y(p.a.y, at.b, row0, ln);
 #pragma unroll
     for (int j = 0; j < kFR; ++j) {
-        const int lr = warp * kFR + j;
-        if (PACKED ? sh.rows.seq[lr] >= 0 : j < live) {
-            if (PACKED && (sh.rows.edge[lr] & 1))
-                h = ln.get(p.a.h0 ? p.a.h0 + sh.rows.seq[lr] * p.a.D : nullptr);
+        if (in(j)) {
+            if (begins(j)) h = h0(j);
             h = advance<WEAK>(c[j], h, b[j]);
-            if (!p.states_only)
-                Raw<T>::template store<VEC>(row_ptr<T>(p.a.y, at.b, row0 + j, ln.d), h, ln.ok0, ln.ok1);
-            if (PACKED && (sh.rows.edge[lr] & 2) && p.a.h_last) ln.put(p.a.h_last + sh.rows.seq[lr] * p.a.D, h);
+            if (!p.states_only) Raw<T>::template store<VEC>(y[j], h, ln.m);
+            if (PACKED && (sh.rows.edge[warp * kFR + j] & 2) && p.a.h_last)
+                ln.put(p.a.h_last + sh.rows.seq[warp * kFR + j] * p.a.D, h);
         }
     }
     if (!PACKED && p.a.h_last && live > 0 && row0 + live == p.a.L) ln.put(p.a.h_last + at.b * p.a.D, h);
 }
 
 template <typename T, bool VEC, bool PACKED>
-__global__ void __launch_bounds__(kFW * 32, 2) k_glr_fwd(const Dev p) {
-    __shared__ FwdShared<T, VEC, PACKED> sh;
+__global__ void __launch_bounds__(kFW * 32, 2) k_glr_fwd(const __grid_constant__ Dev p) {
+    __shared__ FwdShared<PACKED> sh;
     typedef typename Raw<T>::type raw;
     const int warp = threadIdx.x / 32;
     const Place at = place(p, &sh.slot);
@@ -536,21 +607,21 @@ __global__ void __launch_bounds__(kFW * 32, 2) k_glr_fwd(const Dev p) {
     const int live = left < 0 ? 0 : left < kFR ? (int)left : kFR;
     if (PACKED) map_rows(sh.rows, p.a, tile0);
     raw x[kFR], gr[kFR], gi[kFR];
+    {
+        const Run<const T, VEC> pr(p.a.gate_r, at.b, row0, ln), pi(p.a.gate_i, at.b, row0, ln),
+            px(p.a.x, at.b, row0, ln);
 #pragma unroll
-    for (int j = 0; j < kFR; ++j) {
-        const bool in = PACKED ? sh.rows.seq[warp * kFR + j] >= 0 : j < live;
-        const bool k0 = in && ln.ok0, k1 = in && ln.ok1;
-        gr[j] = Raw<T>::template load<VEC>(row_ptr<const T>(p.a.gate_r, at.b, row0 + j, ln.d), k0, k1);
-        gi[j] = Raw<T>::template load<VEC>(row_ptr<const T>(p.a.gate_i, at.b, row0 + j, ln.d), k0, k1);
-        x[j] = Raw<T>::template load<VEC>(row_ptr<const T>(p.a.x, at.b, row0 + j, ln.d), k0, k1);
+        for (int j = 0; j < kFR; ++j) {
+            const unsigned m = (PACKED ? sh.rows.seq[warp * kFR + j] >= 0 : j < live) ? ln.m : 0u;
+            gr[j] = Raw<T>::template load<VEC>(pr[j], m);
+            gi[j] = Raw<T>::template load<VEC>(pi[j], m);
+            x[j] = Raw<T>::template load<VEC>(px[j], m);
+        }
     }
-    const Rates rt = rates(ln.get(p.a.decay), p.a.scale);
-    /* channels that do not exist have decay 0: their rate must not decide */
-    const bool strong = (ln.ok0 && !(rt.rate.x <= kWeak)) || (ln.ok1 && !(rt.rate.y <= kWeak));
-    if (__syncthreads_or(strong))
-        fwd_tile<T, VEC, PACKED, false>(p, at, ln, rt, sh, x, gr, gi, row0, live);
+    if (make_rates<VEC>(p.a, at.ch0, (float *)sh.rate, (float *)sh.sroot))
+        fwd_tile<T, VEC, PACKED, false>(p, at, ln, sh, x, gr, gi, row0, live);
     else
-        fwd_tile<T, VEC, PACKED, true>(p, at, ln, rt, sh, x, gr, gi, row0, live);
+        fwd_tile<T, VEC, PACKED, true>(p, at, ln, sh, x, gr, gi, row0, live);
     if (PACKED && at.pos == 0) empty_sequences(p.a, p.a.h0, p.a.h_last, at.ch0);
 }
 
@@ -558,14 +629,14 @@ __global__ void __launch_bounds__(kFW * 32, 2) k_glr_fwd(const Dev p) {
 /* backward                                                             */
 /* ------------------------------------------------------------------ */
 
-constexpr int kBR = 8, kBW = 8, kBT = kBR * kBW;
+constexpr int kBR = 4, kBW = 16, kBT = kBR * kBW;
 static_assert(kBT == kChunk, "a backward tile begins at a checkpoint");
 
-template <typename T, bool VEC, bool PACKED>
+template <bool PACKED>
 struct BwdShared {
-    float2 fagg[kBW][kC]; /* maps of the states */
-    float2 agg[kBW][kC];  /* maps of the adjoint */
-    float2 map[kWindow][kC];
+    Maps<kBW> states, agg; /* the warps' maps of the states and of the adjoint */
+    Maps<kWindow> seen;
+    float4 rate[32], sroot[32];
     unsigned slot;
     RowMap<PACKED ? kBT : 1> rows;
 };
@@ -573,124 +644,112 @@ struct BwdShared {
 /* The adjoint that reaches row t - 1 from row t is C_t = a_t (dy_t + C_{t+1}). */
 template <typename T, bool VEC, bool PACKED, bool WEAK>
 __device__ __forceinline__ void bwd_tile(const Dev &p, const Place &at, const Lane<VEC> &ln,
-                                         const Rates &rt, BwdShared<T, VEC, PACKED> &sh,
-                                         const typename Raw<T>::type (&x)[kBR],
+                                         BwdShared<PACKED> &sh, const typename Raw<T>::type (&x)[kBR],
                                          const typename Raw<T>::type (&gr)[kBR],
                                          const typename Raw<T>::type (&gi)[kBR],
                                          const typename Raw<T>::type (&dy)[kBR], long tile, long row0,
                                          int live) {
     const int warp = threadIdx.x / 32, warps = blockDim.x / 32;
-    const float2 zero = kmb_f2s(0.f), one = kmb_f2s(1.f);
-    float2 c[kBR], q[kBR], in[kBR], si[kBR];
+    const F4 zero = f4s(0.f), one = f4s(1.f), minus = f4s(-1.f);
+    Terms t[kBR];
+    {
+        const Rates rt = {f4(sh.rate[ln.lane]), f4(sh.sroot[ln.lane])};
 #pragma unroll
-    for (int j = 0; j < kBR; ++j) {
-        const Terms t = terms<WEAK>(Raw<T>::f(gr[j]), Raw<T>::f(gi[j]), rt);
-        c[j] = t.c;
-        q[j] = t.q;
-        in[j] = t.i;
-        si[j] = t.si;
+        for (int j = 0; j < kBR; ++j) t[j] = terms<WEAK>(Raw<T>::f(gr[j]), Raw<T>::f(gi[j]), rt);
     }
-    float2 A = one, H = zero, K = zero;
-    bool fresh = false, ends = false;
+    const auto in = [&](int j) { return PACKED ? sh.rows.seq[warp * kBR + j] >= 0 : j < live; };
+    const auto begins = [&](int j) { return PACKED && (sh.rows.edge[warp * kBR + j] & 1); };
+    const auto ends = [&](int j) { return PACKED && (sh.rows.edge[warp * kBR + j] & 2); };
+    const auto of = [&](const float *v, int j) { return ln.at(v ? v + sh.rows.seq[warp * kBR + j] * p.a.D : nullptr); };
+    F4 A = one, H = zero, K = zero;
+    bool fresh = false, closed = false;
 #pragma unroll
     for (int j = 0; j < kBR; ++j) {
-        const int lr = warp * kBR + j;
-        if (PACKED ? sh.rows.seq[lr] >= 0 : j < live) {
-            if (PACKED && (sh.rows.edge[lr] & 1)) {
-                H = ln.get(p.a.h0 ? p.a.h0 + sh.rows.seq[lr] * p.a.D : nullptr);
+        if (in(j)) {
+            if (begins(j)) {
+                H = of(p.a.h0, j);
                 fresh = true;
             }
-            H = advance<WEAK>(c[j], H, kmb_mul2(si[j], Raw<T>::f(x[j])));
-            A = shrink<WEAK>(c[j], A);
+            H = advance<WEAK>(t[j].c, H, t[j].si * Raw<T>::f(x[j]));
+            A = shrink<WEAK>(t[j].c, A);
         }
     }
-    sh.fagg[warp][ln.off] = kmb_f2(fresh ? -1.f : A.x, H.x);
-    sh.fagg[warp][ln.off + Lane<VEC>::kNext] = kmb_f2(fresh ? -1.f : A.y, H.y);
+    sh.states.put(warp, ln.lane, fresh ? minus : A, H);
 #pragma unroll
     for (int j = kBR - 1; j >= 0; --j) {
-        const int lr = warp * kBR + j;
-        if (PACKED ? sh.rows.seq[lr] >= 0 : j < live) {
-            if (PACKED && (sh.rows.edge[lr] & 2)) {
-                K = ln.get(p.a.dh_last ? p.a.dh_last + sh.rows.seq[lr] * p.a.D : nullptr);
-                ends = true;
+        if (in(j)) {
+            if (ends(j)) {
+                K = of(p.a.dh_last, j);
+                closed = true;
             }
-            K = shrink<WEAK>(c[j], kmb_add2(K, Raw<T>::f(dy[j])));
+            K = shrink<WEAK>(t[j].c, K + Raw<T>::f(dy[j]));
         }
     }
-    sh.agg[warp][ln.off] = kmb_f2(ends ? -1.f : A.x, K.x);
-    sh.agg[warp][ln.off + Lane<VEC>::kNext] = kmb_f2(ends ? -1.f : A.y, K.y);
+    sh.agg.put(warp, ln.lane, closed ? minus : A, K);
     __syncthreads();
 
-    /* the states before each row */
-    float2 h = tile < p.chunks ? ln.get(p.ckpt_in + (at.b * p.chunks + tile) * p.a.D) : zero;
-    for (int w = 0; w < warp; ++w) {
-        const float2 m0 = sh.fagg[w][ln.off], m1 = sh.fagg[w][ln.off + Lane<VEC>::kNext];
-        h = kmb_f2(apply(m0.x, m0.y, h.x), apply(m1.x, m1.y, h.y));
-    }
-    float2 hp[kBR];
-#pragma unroll
-    for (int j = 0; j < kBR; ++j) {
-        const int lr = warp * kBR + j;
-        if (PACKED && sh.rows.seq[lr] >= 0 && (sh.rows.edge[lr] & 1))
-            h = ln.get(p.a.h0 ? p.a.h0 + sh.rows.seq[lr] * p.a.D : nullptr);
-        hp[j] = h;
-        h = advance<WEAK>(c[j], h, kmb_mul2(si[j], Raw<T>::f(x[j])));
-    }
-
     const float *last = !PACKED && p.a.dh_last ? p.a.dh_last + at.b * p.a.D : nullptr;
-    float2 C = enter_tile<VEC>(p, at, ln, sh.agg, sh.map, warps, true, last);
-    for (int w = warps - 1; w > warp; --w) {
-        const float2 m0 = sh.agg[w][ln.off], m1 = sh.agg[w][ln.off + Lane<VEC>::kNext];
-        C = kmb_f2(apply(m0.x, m0.y, C.x), apply(m1.x, m1.y, C.y));
+    F4 C = enter_tile<VEC, PACKED, true>(p, at, ln, sh.agg, sh.seen, last);
+    for (int w = warps - 1; w > warp; --w) C = apply<PACKED>(sh.agg.at(w, ln.lane), C);
+
+    /* the states before each row */
+    F4 hp[kBR];
+    {
+        F4 h = tile < p.chunks ? ln.at(p.ckpt_in + (at.b * p.chunks + tile) * p.a.D) : zero;
+        for (int w = 0; w < warp; ++w) h = apply<PACKED>(sh.states.at(w, ln.lane), h);
+#pragma unroll
+        for (int j = 0; j < kBR; ++j) {
+            if (begins(j)) h = of(p.a.h0, j);
+            hp[j] = h;
+            h = advance<WEAK>(t[j].c, h, t[j].si * Raw<T>::f(x[j]));
+        }
     }
-    float2 sum = zero;
+    F4 sum = zero;
+    const F4 rate = f4(sh.rate[ln.lane]);
+    const Run<T, VEC> dx(p.a.dx, at.b, row0, ln), dgr(p.a.dgate_r, at.b, row0, ln), dgi(p.a.dgate_i, at.b, row0, ln);
 #pragma unroll
     for (int j = kBR - 1; j >= 0; --j) {
-        const int lr = warp * kBR + j;
-        if (PACKED ? sh.rows.seq[lr] >= 0 : j < live) {
-            if (PACKED && (sh.rows.edge[lr] & 2))
-                C = ln.get(p.a.dh_last ? p.a.dh_last + sh.rows.seq[lr] * p.a.D : nullptr);
-            const float2 G = kmb_add2(C, Raw<T>::f(dy[j]));
-            const float2 r = kmb_mul2(q[j], q[j]), u = kmb_mul2(rt.rate, r);
-            const float2 b = kmb_mul2(si[j], Raw<T>::f(x[j]));
-            float2 kappa = poly_kappa(u), ua;
+        if (in(j)) {
+            if (ends(j)) C = of(p.a.dh_last, j);
+            const F4 c = t[j].c, G = C + Raw<T>::f(dy[j]);
+            const F4 r = t[j].q * t[j].q, u = rate * r, b = t[j].si * Raw<T>::f(x[j]);
+            F4 kappa = poly_kappa(u), ua; /* ua: -u a */
             if (WEAK) {
-                ua = kmb_fma2(neg2(c[j]), u, u);
+                ua = fma4(c, u, u) * minus;
             } else {
                 /* e^-u is 0 long before u is 100 */
-                ua = kmb_f2(u.x > 100.f ? 0.f : u.x * c[j].x, u.y > 100.f ? 0.f : u.y * c[j].y);
-                kappa = kmb_f2(u.x <= kWeak ? kappa.x : ua.x * c[j].x * rcp_mufu(fmaf(-c[j].x, c[j].x, 1.f)),
-                               u.y <= kWeak ? kappa.y : ua.y * c[j].y * rcp_mufu(fmaf(-c[j].y, c[j].y, 1.f)));
+                ua = each([&](int n) { return get(u, n) > 100.f ? 0.f : -get(u, n) * get(c, n); });
+                kappa = each([&](int n) {
+                    const float a = get(c, n);
+                    return get(u, n) <= kWeak ? get(kappa, n) : -get(ua, n) * a * rcp_mufu(fmaf(-a, a, 1.f));
+                });
             }
-            const float2 udu = kmb_mul2(G, kmb_fma2(neg2(ua), hp[j], kmb_mul2(kappa, b)));
-            sum = kmb_add2(sum, udu);
-            Raw<T>::template store<VEC>(row_ptr<T>(p.a.dx, at.b, row0 + j, ln.d), kmb_mul2(G, si[j]), ln.ok0,
-                                        ln.ok1);
-            Raw<T>::template store<VEC>(row_ptr<T>(p.a.dgate_r, at.b, row0 + j, ln.d),
-                                        kmb_mul2(udu, sub2(one, r)), ln.ok0, ln.ok1);
-            Raw<T>::template store<VEC>(row_ptr<T>(p.a.dgate_i, at.b, row0 + j, ln.d),
-                                        kmb_mul2(kmb_mul2(G, b), sub2(one, in[j])), ln.ok0, ln.ok1);
-            C = shrink<WEAK>(c[j], G);
-            if (PACKED && (sh.rows.edge[lr] & 1) && p.a.dh0) ln.put(p.a.dh0 + sh.rows.seq[lr] * p.a.D, C);
+            const F4 udu = G * fma4(ua, hp[j], kappa * b);
+            sum = sum + udu;
+            Raw<T>::template store<VEC>(dx[j], G * t[j].si, ln.m);
+            Raw<T>::template store<VEC>(dgr[j], udu * fma4(r, minus, one), ln.m);
+            Raw<T>::template store<VEC>(dgi[j], G * b * fma4(t[j].i, minus, one), ln.m);
+            C = shrink<WEAK>(c, G);
+            if (begins(j) && p.a.dh0) ln.put(p.a.dh0 + sh.rows.seq[warp * kBR + j] * p.a.D, C);
         }
     }
     if (!PACKED && tile == 0 && warp == 0 && p.a.dh0) ln.put(p.a.dh0 + at.b * p.a.D, C);
     if (p.part) {
-        __syncthreads(); /* every warp is done with the maps */
-        sh.fagg[warp][ln.off].x = sum.x;
-        sh.fagg[warp][ln.off + Lane<VEC>::kNext].x = sum.y;
+        __syncthreads(); /* every warp is done with the states' maps */
+        sh.states.H[warp][ln.lane] = v4(sum);
         __syncthreads();
-        for (int ch = threadIdx.x; ch < kC; ch += blockDim.x) {
+        for (int k = threadIdx.x; k < kC; k += blockDim.x) {
             float v = 0.f;
-            for (int w = 0; w < warps; ++w) v += sh.fagg[w][ch].x;
-            p.part[at.pos * p.chains * kC + at.chain * kC + ch] = v;
+            for (int w = 0; w < warps; ++w) v += ((const float *)sh.states.H[w])[k];
+            const int ch = VEC ? k : (k % kV) * 32 + k / kV;
+            p.part[(at.pos * p.chains + at.chain) * kC + ch] = v;
         }
     }
 }
 
 template <typename T, bool VEC, bool PACKED>
-__global__ void __launch_bounds__(kBW * 32, 2) k_glr_bwd(const Dev p) {
-    __shared__ BwdShared<T, VEC, PACKED> sh;
+__global__ void __launch_bounds__(kBW * 32, 1) k_glr_bwd(const __grid_constant__ Dev p) {
+    __shared__ BwdShared<PACKED> sh;
     typedef typename Raw<T>::type raw;
     const int warp = threadIdx.x / 32;
     const Place at = place(p, &sh.slot);
@@ -700,21 +759,22 @@ __global__ void __launch_bounds__(kBW * 32, 2) k_glr_bwd(const Dev p) {
     const int live = left < 0 ? 0 : left < kBR ? (int)left : kBR;
     if (PACKED) map_rows(sh.rows, p.a, tile0);
     raw x[kBR], gr[kBR], gi[kBR], dy[kBR];
+    {
+        const Run<const T, VEC> pr(p.a.gate_r, at.b, row0, ln), pi(p.a.gate_i, at.b, row0, ln),
+            px(p.a.x, at.b, row0, ln), pd(p.a.dy, at.b, row0, ln);
 #pragma unroll
-    for (int j = 0; j < kBR; ++j) {
-        const bool in = PACKED ? sh.rows.seq[warp * kBR + j] >= 0 : j < live;
-        const bool k0 = in && ln.ok0, k1 = in && ln.ok1;
-        gr[j] = Raw<T>::template load<VEC>(row_ptr<const T>(p.a.gate_r, at.b, row0 + j, ln.d), k0, k1);
-        gi[j] = Raw<T>::template load<VEC>(row_ptr<const T>(p.a.gate_i, at.b, row0 + j, ln.d), k0, k1);
-        x[j] = Raw<T>::template load<VEC>(row_ptr<const T>(p.a.x, at.b, row0 + j, ln.d), k0, k1);
-        dy[j] = Raw<T>::template load<VEC>(row_ptr<const T>(p.a.dy, at.b, row0 + j, ln.d), k0, k1);
+        for (int j = 0; j < kBR; ++j) {
+            const unsigned m = (PACKED ? sh.rows.seq[warp * kBR + j] >= 0 : j < live) ? ln.m : 0u;
+            gr[j] = Raw<T>::template load<VEC>(pr[j], m);
+            gi[j] = Raw<T>::template load<VEC>(pi[j], m);
+            x[j] = Raw<T>::template load<VEC>(px[j], m);
+            dy[j] = Raw<T>::template load<VEC>(pd[j], m);
+        }
     }
-    const Rates rt = rates(ln.get(p.a.decay), p.a.scale);
-    const bool strong = (ln.ok0 && !(rt.rate.x <= kWeak)) || (ln.ok1 && !(rt.rate.y <= kWeak));
-    if (__syncthreads_or(strong))
-        bwd_tile<T, VEC, PACKED, false>(p, at, ln, rt, sh, x, gr, gi, dy, tile, row0, live);
+    if (make_rates<VEC>(p.a, at.ch0, (float *)sh.rate, (float *)sh.sroot))
+        bwd_tile<T, VEC, PACKED, false>(p, at, ln, sh, x, gr, gi, dy, tile, row0, live);
     else
-        bwd_tile<T, VEC, PACKED, true>(p, at, ln, rt, sh, x, gr, gi, dy, tile, row0, live);
+        bwd_tile<T, VEC, PACKED, true>(p, at, ln, sh, x, gr, gi, dy, tile, row0, live);
     if (PACKED && tile == 0) empty_sequences(p.a, p.a.dh_last, p.a.dh0, at.ch0);
 }
 
@@ -765,21 +825,19 @@ __global__ void __launch_bounds__(kStepThreads) k_glr_step(KmbGLRStep a, long ti
     const long d = (blockIdx.x - k * tiles) * kStepThreads + threadIdx.x;
     if (d >= a.D) return;
     const float rate = a.scale * softplus(a.decay[d]);
-    Rates rt;
-    rt.rate = kmb_f2s(rate);
-    rt.sroot = kmb_f2s(sqrtf(2.f * rate));
+    const Rates rt = {f4s(rate), f4s(sqrtf(2.f * rate))};
     const T *px = (const T *)a.x.data + k * a.x.row_stride + d;
     const T *pr = (const T *)a.gate_r.data + k * a.gate_r.row_stride + d;
     const T *pi = (const T *)a.gate_i.data + k * a.gate_i.row_stride + d;
-    const float2 gr = kmb_f2s((float)*pr), gi = kmb_f2s((float)*pi), x = kmb_f2s((float)*px);
+    const F4 gr = f4s((float)*pr), gi = f4s((float)*pi), x = f4s((float)*px);
     float *s = a.state + slot * a.ld_state + d;
     float h = *s;
     if (rate <= kWeak) {
         const Terms t = terms<true>(gr, gi, rt);
-        h = advance<true>(t.c, kmb_f2s(h), kmb_mul2(t.si, x)).x;
+        h = advance<true>(t.c, f4s(h), t.si * x).l.x;
     } else {
         const Terms t = terms<false>(gr, gi, rt);
-        h = advance<false>(t.c, kmb_f2s(h), kmb_mul2(t.si, x)).x;
+        h = advance<false>(t.c, f4s(h), t.si * x).l.x;
     }
     *s = h;
     ((T *)a.y.data)[k * a.y.row_stride + d] = (T)h;
@@ -794,16 +852,16 @@ int done(const char *what) {
     return e == cudaSuccess ? KMB_OK : kmb_cuda_fail(e, what);
 }
 
-/* Whether the tensors allow two channels an access: even width, strides and
- * addresses. */
-bool paired(const KmbGLR *a, const KmbRows *const *rows, int n) {
+/* Whether the tensors allow four channels an access: width, strides and
+ * addresses are multiples of four elements. */
+bool vectors(const KmbGLR *a, const KmbRows *const *rows, int n) {
     const size_t es = a->type == KMB_BF16 ? 2 : 4;
-    if (a->D % 2) return false;
+    if (a->D % kV) return false;
     for (int i = 0; i < n; ++i) {
         const KmbRows *r = rows[i];
         if (!r->data) continue;
-        if (((size_t)r->data / es) % 2 || r->row_stride % 2) return false;
-        if (!a->offsets && a->batch > 1 && r->batch_stride % 2) return false;
+        if (((size_t)r->data / es) % kV || r->row_stride % kV) return false;
+        if (!a->offsets && a->batch > 1 && r->batch_stride % kV) return false;
     }
     return true;
 }
@@ -838,10 +896,10 @@ int begin(Dev &d, const Plan &q, void *ws, cudaStream_t s) {
     const cudaError_t e = cudaMemsetAsync(ws, 0xff, shown_bytes(q), s);
     if (e != cudaSuccess) return kmb_cuda_fail(e, "glr: workspace fill");
     d.ticket = (unsigned *)ws;
-    d.shown.A = (float *)((char *)ws + kHead);
-    d.shown.H = d.shown.A + q.words;
-    d.shown.end = d.shown.H + q.words;
-    d.shown.step = q.chains * kC;
+    d.shown.A = (float4 *)((char *)ws + kHead);
+    d.shown.H = d.shown.A + q.words / kV;
+    d.shown.end = d.shown.H + q.words / kV;
+    d.shown.step = q.chains * 32;
     return KMB_OK;
 }
 
@@ -891,7 +949,7 @@ int run_fwd(const KmbGLR *a, float *ckpt, bool write_y, void *ws, cudaStream_t s
     const int rc = begin(d, q, ws, s);
     if (rc) return rc;
     const KmbRows *rows[] = {&d.a.x, &d.a.gate_r, &d.a.gate_i, &d.a.y};
-    const bool vec = paired(&d.a, rows, 4);
+    const bool vec = vectors(&d.a, rows, 4);
     return a->type == KMB_BF16 ? launch_fwd<__nv_bfloat16>(d, q, vec, s) : launch_fwd<float>(d, q, vec, s);
 }
 
@@ -952,7 +1010,7 @@ extern "C" int kmb_launch_glr_bwd(const KmbGLR *a, cudaStream_t s) {
     }
     if ((rc = begin(d, q, ws, s))) return rc;
     const KmbRows *rows[] = {&d.a.x, &d.a.gate_r, &d.a.gate_i, &d.a.dy, &d.a.dx, &d.a.dgate_r, &d.a.dgate_i};
-    const bool vec = paired(&d.a, rows, 7);
+    const bool vec = vectors(&d.a, rows, 7);
     rc = a->type == KMB_BF16 ? launch_bwd<__nv_bfloat16>(d, q, vec, s) : launch_bwd<float>(d, q, vec, s);
     if (rc || !a->ddecay) return rc;
     k_glr_ddecay<<<(unsigned)((a->D + 31) / 32), dim3(32, 32), 0, s>>>(
