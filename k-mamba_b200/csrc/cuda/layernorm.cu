@@ -7,13 +7,12 @@
  * and bias' gradients are the column sums of dy xhat and dy.
  *
  * Memory bounds both: every tensor is to be read or written once.  A row
- * stays in the registers of a warp (D <= 256) or a CTA from its load to the
- * store, 8 values a thread, so the mean and the centred squares are two
- * passes over registers.  CTAs are resident for the whole call and walk the
- * rows: weight and bias are loaded once, the next row's loads are in flight
- * while a row is reduced, and in the backward every thread keeps the column
- * sums of its own 8 columns, written once at the end as one row of partial
- * sums a CTA, which a second kernel adds in a fixed order.
+ * stays in the registers of a warp (up to 1024 values, 512 in the backward)
+ * or a CTA from its load to the store, so the mean and the centred squares
+ * are two passes over registers.  CTAs are resident for the whole call and
+ * walk the rows.  In the backward every thread keeps the column sums of its
+ * own columns, written once at the end as one row of partial sums a CTA,
+ * which a second kernel adds in a fixed order.
  */
 #include <cuda_bf16.h>
 
@@ -23,13 +22,7 @@
 namespace {
 
 constexpr int kSMs = 148;
-constexpr int kEpt = 8;        /* values of a thread */
-constexpr int kGroup = 256;    /* widest row of a single warp */
-constexpr int kGroups = 8;     /* such rows of a CTA */
-constexpr int kSmall = 256;    /* threads up to which a thread has 80 registers, not 64 */
-constexpr int kMaxD = 1024 * kEpt;
-constexpr int kWideEpt = 32;   /* forward: values of a thread for wider rows */
-constexpr int kWideD = 1024 * kWideEpt;
+constexpr int kWarps = 8;      /* warps of a CTA whose warps have a row each */
 constexpr int kLoop = 512;     /* threads for rows that do not stay in registers */
 
 __device__ __forceinline__ float ld(const float *p) { return *p; }
@@ -115,26 +108,27 @@ struct Reducer {
     int warps; /* of a row */
     int turn;
     __device__ __forceinline__ Reducer(float2 (*s)[32], int w) : slot(s), warps(w), turn(0) {}
-    __device__ __forceinline__ float2 two(float a, float b) {
+    template <bool TWO>
+    __device__ __forceinline__ float2 sum(float a, float b) {
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             a += __shfl_xor_sync(~0u, a, o);
-            b += __shfl_xor_sync(~0u, b, o);
+            if (TWO) b += __shfl_xor_sync(~0u, b, o);
         }
         if (warps == 1) return make_float2(a, b);
-        const int lane = threadIdx.x % 32;
-        if (lane == 0) slot[turn][threadIdx.x / 32] = make_float2(a, b);
+        if (threadIdx.x % 32 == 0) slot[turn][threadIdx.x / 32] = make_float2(a, b);
         __syncthreads();
-        float2 v = lane < warps ? slot[turn][lane] : make_float2(0.f, 0.f);
-        turn ^= 1;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            v.x += __shfl_xor_sync(~0u, v.x, o);
-            v.y += __shfl_xor_sync(~0u, v.y, o);
+        a = b = 0.f;
+        for (int w = 0; w < warps; ++w) {
+            const float2 v = slot[turn][w];
+            a += v.x;
+            if (TWO) b += v.y;
         }
-        return v;
+        turn ^= 1;
+        return make_float2(a, b);
     }
-    __device__ __forceinline__ float one(float a) { return two(a, 0.f).x; }
+    __device__ __forceinline__ float2 two(float a, float b) { return sum<true>(a, b); }
+    __device__ __forceinline__ float one(float a) { return sum<false>(a, 0.f).x; }
 };
 
 /* Sums of rows whose plain fp32 sums overflow are taken again on scaled
@@ -142,107 +136,135 @@ struct Reducer {
  * A row with an infinity or a NaN stays what it is. */
 constexpr float kDown = 0x1p-32f, kUp = 0x1p32f, kSqDown = 0x1p-80f;
 
-/* each(f) calls f(value) for the thread's values of the row */
-template <typename Each>
-__device__ __forceinline__ void row_stats(Each each, Reducer &red, float n, float eps, float &mean,
-                                          float &rstd) {
-    float s = 0.f;
-    each([&](float x) { s += x; });
-    mean = red.one(s) / n;
-    if (!isfinite(mean)) {
-        s = 0.f;
-        each([&](float x) { s = fmaf(x, kDown, s); });
-        mean = red.one(s) / n * kUp;
-    }
-    s = 0.f;
-    each([&](float x) { s = fmaf(x - mean, x - mean, s); });
-    s = red.one(s);
+/* sum(f): the sum of f(pair) over the row's values, pairs of values */
+template <typename Sum>
+__device__ __forceinline__ void row_stats(Sum sum, float n, float eps, float &mean, float &rstd) {
+    mean = sum([](float2 x) { return x; }) / n;
+    if (!isfinite(mean)) mean = sum([](float2 x) { return kmb_mul2(x, kmb_f2s(kDown)); }) / n * kUp;
+    const float2 m = kmb_f2s(-mean);
+    const float s = sum([&](float2 x) {
+        const float2 c = kmb_add2(x, m);
+        return kmb_mul2(c, c);
+    });
     rstd = 1.f / sqrtf(s / n + eps);
     if (!isfinite(s)) {
-        s = 0.f;
-        each([&](float x) { s = fmaf((x - mean) * kSqDown, (x - mean) * kSqDown, s); });
-        rstd = kSqDown / sqrtf(red.one(s) / n + eps * kSqDown * kSqDown);
+        const float t = sum([&](float2 x) {
+            const float2 c = kmb_mul2(kmb_add2(x, m), kmb_f2s(kSqDown));
+            return kmb_mul2(c, c);
+        });
+        rstd = kSqDown / sqrtf(t / n + eps * kSqDown * kSqDown);
     }
 }
 
-/* The thread's columns: vector k begins at col(k); all of a vector's
- * columns exist or none. */
-template <int V>
+/* The thread's columns of a row of `tpr` threads, EPT of them at most:
+ * vector k begins at col(k); all of a vector's columns exist or none.  FULL:
+ * all exist. */
+template <int V, int EPT, bool FULL>
 struct Cols {
+    static constexpr int NV = EPT / V;
     int t, tpr, D;
     __device__ __forceinline__ int col(int k) const { return (t + k * tpr) * V; }
-    __device__ __forceinline__ bool in(int k) const { return col(k) < D; }
+    __device__ __forceinline__ bool in(int k) const { return FULL || col(k) < D; }
+    __device__ __forceinline__ bool has(int e) const { return in(e / V); } /* value e */
+    __device__ __forceinline__ void vector(const float *p, float none, float *out) const {
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) out[e] = p && has(e) ? p[col(e / V) + e % V] : none;
+    }
+    /* values that do not exist are 0 */
+    template <typename T>
+    __device__ __forceinline__ void fetch(const T *p, Vec<T, V> (&raw)[NV]) const {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (in(k)) raw[k].load(p + col(k));
+            else raw[k] = Vec<T, V>{};
+        }
+    }
+    template <typename T>
+    static __device__ __forceinline__ void unpack(const Vec<T, V> (&raw)[NV], float2 (&x)[EPT / 2]) {
+        float f[EPT];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) raw[k].get(f + k * V);
+#pragma unroll
+        for (int e = 0; e < EPT / 2; ++e) x[e] = kmb_f2(f[2 * e], f[2 * e + 1]);
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(T *p, const float2 (&x)[EPT / 2]) const {
+        float f[EPT];
+#pragma unroll
+        for (int e = 0; e < EPT / 2; ++e) {
+            f[2 * e] = x[e].x;
+            f[2 * e + 1] = x[e].y;
+        }
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            if (in(k)) Vec<T, V>::store(p + col(k), f + k * V);
+    }
+    __device__ __forceinline__ void columns(float *p, const float2 (&x)[EPT / 2]) const {
+#pragma unroll
+        for (int e = 0; e < EPT; ++e)
+            if (has(e)) p[col(e / V) + e % V] = e % 2 ? x[e / 2].y : x[e / 2].x;
+    }
+    /* 0 where a value does not exist */
+    __device__ __forceinline__ float2 mask(int pair, float2 v) const {
+        return kmb_f2(has(2 * pair) ? v.x : 0.f, has(2 * pair + 1) ? v.y : 0.f);
+    }
+    template <typename Fn>
+    __device__ __forceinline__ float sum(const float2 (&x)[EPT / 2], Fn f) const {
+        float2 s = kmb_f2s(0.f);
+#pragma unroll
+        for (int e = 0; e < EPT / 2; ++e) s = kmb_add2(s, mask(e, f(x[e])));
+        return s.x + s.y;
+    }
 };
-
-template <int V, int NV>
-__device__ __forceinline__ void load_cols(const Cols<V> &c, const float *p, float none, float *out) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e) out[k * V + e] = p && c.in(k) ? p[c.col(k) + e] : none;
-}
 
 /* ------------------------------------------------------------------ */
 /* forward                                                              */
 /* ------------------------------------------------------------------ */
 
-template <typename TX, typename TY, int V, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT, MAXT == kSmall ? 3 : 1) k_ln_fwd(const __grid_constant__ KmbLayerNorm a, int wpr) {
+/* KEEP: weight and bias stay in registers */
+template <typename TX, typename TY, int V, int EPT, bool FULL, bool KEEP>
+__global__ void __launch_bounds__(KEEP ? 512 : 1024) k_ln_fwd(const __grid_constant__ KmbLayerNorm a, int wpr) {
     __shared__ float2 slot[2][32];
-    constexpr bool kKeep = V * NV <= kEpt; /* weight and bias in registers, next row ahead */
+    typedef Cols<V, EPT, FULL> C;
     const bool single = wpr == 1;
     const int groups = single ? (int)blockDim.x / 32 : 1;
-    const Cols<V> c = {single ? (int)threadIdx.x % 32 : (int)threadIdx.x, wpr * 32, (int)a.D};
+    const C c = {single ? (int)threadIdx.x % 32 : (int)threadIdx.x, wpr * 32, (int)a.D};
     Reducer red(slot, wpr);
-    const long step = (long)gridDim.x * groups;
-    long r = (long)blockIdx.x * groups + (single ? threadIdx.x / 32 : 0);
-    const float n = (float)a.D;
-    float w[kKeep ? V * NV : 1], b[kKeep ? V * NV : 1];
-    if (kKeep) {
-        load_cols<V, kKeep ? NV : 0>(c, a.weight, 1.f, w);
-        load_cols<V, kKeep ? NV : 0>(c, a.bias, 0.f, b);
+    float w[KEEP ? EPT : 2], b[KEEP ? EPT : 2];
+    if (KEEP) {
+        c.vector(a.weight, 1.f, w);
+        c.vector(a.bias, 0.f, b);
     }
-    Vec<TX, V> raw[NV];
-    const auto fetch = [&](long row) {
-        const TX *x = (const TX *)a.x + row * a.ld_x;
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (c.in(k)) raw[k].load(x + c.col(k));
-    };
-    if (r < a.rows) fetch(r);
-    for (; r < a.rows; r += step) {
-        float x[V * NV];
-#pragma unroll
-        for (int k = 0; k < NV; ++k) raw[k].get(x + k * V);
-        if (kKeep && r + step < a.rows) fetch(r + step);
-        float mean, rstd;
-        row_stats(
-            [&](auto f) {
-#pragma unroll
-                for (int k = 0; k < NV; ++k)
-                    if (c.in(k))
-#pragma unroll
-                        for (int e = 0; e < V; ++e) f(x[k * V + e]);
-            },
-            red, n, a.eps, mean, rstd);
-        TY *y = (TY *)a.y + r * a.ld_y;
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (!c.in(k)) continue;
-            float o[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float wv = kKeep ? w[k * V + e] : a.weight ? a.weight[c.col(k) + e] : 1.f;
-                const float bv = kKeep ? b[k * V + e] : a.bias ? a.bias[c.col(k) + e] : 0.f;
-                o[e] = fmaf((x[k * V + e] - mean) * rstd, wv, bv);
-            }
-            Vec<TY, V>::store(y + c.col(k), o);
+    for (long r = (long)blockIdx.x * groups + (single ? threadIdx.x / 32 : 0); r < a.rows;
+         r += (long)gridDim.x * groups) {
+        float2 x[EPT / 2];
+        {
+            Vec<TX, V> raw[C::NV];
+            c.fetch((const TX *)a.x + r * a.ld_x, raw);
+            C::unpack(raw, x);
         }
+        float mean, rstd;
+        row_stats([&](auto f) { return red.one(c.sum(x, f)); }, (float)a.D, a.eps, mean, rstd);
+        const float2 m = kmb_f2s(-mean), s = kmb_f2s(rstd);
+#pragma unroll
+        for (int e = 0; e < EPT / 2; ++e) {
+            float2 wv, bv;
+            if (KEEP) {
+                wv = kmb_f2(w[2 * e], w[2 * e + 1]);
+                bv = kmb_f2(b[2 * e], b[2 * e + 1]);
+            } else {
+                const int i = c.col(2 * e / V) + 2 * e % V;
+                const bool ok = c.has(2 * e);
+                wv = ok && a.weight ? *reinterpret_cast<const float2 *>(a.weight + i) : kmb_f2s(1.f);
+                bv = ok && a.bias ? *reinterpret_cast<const float2 *>(a.bias + i) : kmb_f2s(0.f);
+            }
+            x[e] = kmb_fma2(kmb_mul2(kmb_add2(x[e], m), s), wv, bv);
+        }
+        c.store((TY *)a.y + r * a.ld_y, x);
         if (c.t == 0) {
             if (a.mean) a.mean[r] = mean;
             if (a.rstd) a.rstd[r] = rstd;
         }
-        if (!kKeep && r + step < a.rows) fetch(r + step);
     }
 }
 
@@ -257,9 +279,11 @@ __global__ void __launch_bounds__(kLoop) k_ln_fwd_loop(const __grid_constant__ K
         float mean, rstd;
         row_stats(
             [&](auto f) {
-                for (long j = threadIdx.x; j < a.D; j += kLoop) f(ld(x + j));
+                float s = 0.f;
+                for (long j = threadIdx.x; j < a.D; j += kLoop) s += f(kmb_f2s(ld(x + j))).x;
+                return red.one(s);
             },
-            red, (float)a.D, a.eps, mean, rstd);
+            (float)a.D, a.eps, mean, rstd);
         for (long j = threadIdx.x; j < a.D; j += kLoop)
             st(y + j, fmaf((ld(x + j) - mean) * rstd, a.weight ? a.weight[j] : 1.f, a.bias ? a.bias[j] : 0.f));
         if (threadIdx.x == 0) {
@@ -273,34 +297,30 @@ __global__ void __launch_bounds__(kLoop) k_ln_fwd_loop(const __grid_constant__ K
 /* backward                                                             */
 /* ------------------------------------------------------------------ */
 
-template <typename TX, typename TY, int V, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT, MAXT == kSmall ? 3 : 1) k_ln_bwd(const __grid_constant__ KmbLayerNorm a, int wpr, int sums) {
-    static_assert(V * NV == kEpt, "8 values a thread");
+/* The next row's loads are in flight while a row is reduced. */
+template <typename TX, typename TY, int V, int EPT, bool FULL>
+__global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayerNorm a, int wpr, int sums) {
     __shared__ float2 slot[2][32];
-    __shared__ float fold[kGroups][kGroup];
+    __shared__ float fold[kWarps][32 * EPT];
+    typedef Cols<V, EPT, FULL> C;
     const bool single = wpr == 1;
     const int groups = single ? (int)blockDim.x / 32 : 1, warp = threadIdx.x / 32;
-    const Cols<V> c = {single ? (int)threadIdx.x % 32 : (int)threadIdx.x, wpr * 32, (int)a.D};
+    const C c = {single ? (int)threadIdx.x % 32 : (int)threadIdx.x, wpr * 32, (int)a.D};
     Reducer red(slot, wpr);
     const long step = (long)gridDim.x * groups;
     long r = (long)blockIdx.x * groups + (single ? warp : 0);
-    const float n = (float)a.D, inv = 1.f / n;
-    float w[kEpt], pw[kEpt], pb[kEpt];
-    load_cols<V, NV>(c, a.weight, 1.f, w);
+    const float inv = 1.f / (float)a.D;
+    float w[EPT];
+    c.vector(a.weight, 1.f, w);
+    float2 pw[EPT / 2], pb[EPT / 2];
 #pragma unroll
-    for (int e = 0; e < kEpt; ++e) pw[e] = pb[e] = 0.f;
-    Vec<TX, V> rx[NV];
-    Vec<TY, V> rd[NV];
+    for (int e = 0; e < EPT / 2; ++e) pw[e] = pb[e] = kmb_f2s(0.f);
+    Vec<TX, V> rx[C::NV];
+    Vec<TY, V> rd[C::NV];
     float mean = 0.f, rstd = 0.f;
     const auto fetch = [&](long row) {
-        const TX *x = (const TX *)a.x + row * a.ld_x;
-        const TY *dy = (const TY *)a.dy + row * a.ld_dy;
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (c.in(k)) {
-                rx[k].load(x + c.col(k));
-                rd[k].load(dy + c.col(k));
-            }
+        c.fetch((const TX *)a.x + row * a.ld_x, rx);
+        c.fetch((const TY *)a.dy + row * a.ld_dy, rd);
         if (a.mean) {
             mean = a.mean[row];
             rstd = a.rstd[row];
@@ -308,87 +328,52 @@ __global__ void __launch_bounds__(MAXT, MAXT == kSmall ? 3 : 1) k_ln_bwd(const _
     };
     if (r < a.rows) fetch(r);
     for (; r < a.rows; r += step) {
-        float h[kEpt], d[kEpt];
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            rx[k].get(h + k * V);
-            rd[k].get(d + k * V);
-        }
+        float2 h[EPT / 2], d[EPT / 2];
+        C::unpack(rx, h);
+        C::unpack(rd, d);
         float m = mean, s = rstd;
         if (r + step < a.rows) fetch(r + step);
-        Vec<TX, V> res[NV];
-        if (a.dres) {
-            const TX *p = (const TX *)a.dres + r * a.ld_dres;
+        if (!a.mean) row_stats([&](auto f) { return red.one(c.sum(h, f)); }, (float)a.D, a.eps, m, s);
+        float2 t1 = kmb_f2s(0.f), t2 = t1;
+        const float2 m2 = kmb_f2s(-m), sd = kmb_f2s(s);
 #pragma unroll
-            for (int k = 0; k < NV; ++k)
-                if (c.in(k)) res[k].load(p + c.col(k));
+        for (int e = 0; e < EPT / 2; ++e) { /* d is 0 where a value does not exist */
+            h[e] = kmb_mul2(kmb_add2(h[e], m2), sd);
+            pw[e] = kmb_fma2(d[e], h[e], pw[e]);
+            pb[e] = kmb_add2(pb[e], d[e]);
+            d[e] = kmb_mul2(d[e], kmb_f2(w[2 * e], w[2 * e + 1]));
+            t1 = kmb_add2(t1, d[e]);
+            t2 = kmb_fma2(d[e], h[e], t2);
         }
-        if (!a.mean)
-            row_stats(
-                [&](auto f) {
+        const float2 t = red.two(t1.x + t1.y, t2.x + t2.y);
+        const float2 s1 = kmb_f2s(-t.x * inv), s2 = kmb_f2s(-t.y * inv);
 #pragma unroll
-                    for (int k = 0; k < NV; ++k)
-                        if (c.in(k))
+        for (int e = 0; e < EPT / 2; ++e) d[e] = kmb_mul2(kmb_fma2(h[e], s2, kmb_add2(d[e], s1)), sd);
+        if (a.dres) {
+            Vec<TX, V> raw[C::NV];
+            c.fetch((const TX *)a.dres + r * a.ld_dres, raw);
+            C::unpack(raw, h);
 #pragma unroll
-                            for (int e = 0; e < V; ++e) f(h[k * V + e]);
-                },
-                red, n, a.eps, m, s);
-        float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (c.in(k))
-#pragma unroll
-                for (int e = k * V; e < k * V + V; ++e) {
-                    h[e] = (h[e] - m) * s;
-                    pw[e] = fmaf(d[e], h[e], pw[e]);
-                    pb[e] += d[e];
-                    d[e] *= w[e];
-                    s1 += d[e];
-                    s2 = fmaf(d[e], h[e], s2);
-                }
-        const float2 t = red.two(s1, s2);
-        s1 = t.x * inv;
-        s2 = t.y * inv;
-        TX *dx = (TX *)a.dx + r * a.ld_dx;
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (c.in(k)) {
-                float o[V], q[V];
-                if (a.dres) res[k].get(q);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    o[e] = s * (d[k * V + e] - s1 - h[k * V + e] * s2);
-                    if (a.dres) o[e] += q[e];
-                }
-                Vec<TX, V>::store(dx + c.col(k), o);
-            }
+            for (int e = 0; e < EPT / 2; ++e) d[e] = kmb_add2(d[e], h[e]);
+        }
+        c.store((TX *)a.dx + r * a.ld_dx, d);
     }
     if (!sums) return;
     float *part = (float *)a.workspace + (long)blockIdx.x * 2 * a.D;
-    if (!single) {
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (c.in(k))
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    part[c.col(k) + e] = pw[k * V + e];
-                    part[a.D + c.col(k) + e] = pb[k * V + e];
-                }
-        return;
-    }
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
+        float2 (&v)[EPT / 2] = which ? pb : pw;
+        if (!single) {
+            c.columns(part + which * a.D, v);
+            continue;
+        }
         __syncthreads();
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (c.in(k))
-#pragma unroll
-                for (int e = 0; e < V; ++e) fold[warp][c.col(k) + e] = which ? pb[k * V + e] : pw[k * V + e];
+        c.columns(fold[warp], v);
         __syncthreads();
         for (int j = threadIdx.x; j < a.D; j += blockDim.x) {
-            float v = 0.f;
-            for (int g = 0; g < groups; ++g) v += fold[g][j];
-            part[which * a.D + j] = v;
+            float t = 0.f;
+            for (int g = 0; g < groups; ++g) t += fold[g][j];
+            part[which * a.D + j] = t;
         }
     }
 }
@@ -419,9 +404,11 @@ __global__ void __launch_bounds__(kLoop) k_ln_bwd_loop(const __grid_constant__ K
         } else {
             row_stats(
                 [&](auto f) {
-                    for (long j = threadIdx.x; j < a.D; j += kLoop) f(ld(x + j));
+                    float s = 0.f;
+                    for (long j = threadIdx.x; j < a.D; j += kLoop) s += f(kmb_f2s(ld(x + j))).x;
+                    return red.one(s);
                 },
-                red, (float)a.D, a.eps, mean, rstd);
+                (float)a.D, a.eps, mean, rstd);
         }
         float s1 = 0.f, s2 = 0.f;
         for (long j = threadIdx.x; j < a.D; j += kLoop) {
@@ -475,20 +462,26 @@ __global__ void __launch_bounds__(1024) k_ln_sums(const float *part, long parts,
 /* launches                                                             */
 /* ------------------------------------------------------------------ */
 
-int warps_of(long D, int ept) { return (int)((D + 32 * ept - 1) / (32 * ept)); }
+/* Values of a thread.  More of them mean fewer sums across threads (each
+ * costs a warp 5 shuffles and a barrier), fewer mean more rows in flight. */
+int fwd_ept(long D) { return D <= 256 ? 8 : D <= 512 ? 16 : 32; }
+int bwd_ept(long D) { return D <= 256 ? 8 : 16; }
+constexpr long kFwdKeep = 512 * 32, kFwdWide = 1024 * 32, kBwdMax = 512 * 16;
 
-/* CTAs of the resident kernels: as many as the registers let an SM hold, no
+int warps_of(long D, int ept) { return (int)((D + 32 * ept - 1) / (32 * ept)); }
+int threads_of(int wpr) { return 32 * (wpr == 1 ? kWarps : wpr); }
+
+/* CTAs of a resident kernel of 512 threads an SM (128 registers each), no
  * more than there are rows (or groups of rows) */
-long ctas(long rows, long D, int ept) {
-    const int wpr = warps_of(D, ept), threads = wpr == 1 ? 32 * kGroups : 32 * wpr;
-    const long need = wpr == 1 ? (rows + kGroups - 1) / kGroups : rows;
-    const long most = (long)kSMs * (threads <= kSmall ? 3 * kSmall / threads : 1024 / threads);
+long ctas(long rows, int wpr) {
+    const long need = wpr == 1 ? (rows + kWarps - 1) / kWarps : rows;
+    const int fit = 512 / threads_of(wpr);
+    const long most = (long)kSMs * (fit > 0 ? fit : 1);
     return need < most ? (need > 0 ? need : 1) : most;
 }
 
-bool aligned(const void *p, long ld, int type, int v) {
-    const size_t es = type == KMB_BF16 ? 2 : 4;
-    return !p || ((size_t)p / es % v == 0 && ld % v == 0);
+bool aligned(const void *p, long ld, size_t es, int v) {
+    return !p || ((size_t)p % (es * v) == 0 && ld % v == 0);
 }
 
 int done() {
@@ -496,37 +489,52 @@ int done() {
     return e == cudaSuccess ? KMB_OK : kmb_cuda_fail(e, "layernorm: launch");
 }
 
-template <typename TX, typename TY, int V, int NV>
+template <typename TX, typename TY, int V, int EPT, bool KEEP>
 void run_fwd(const KmbLayerNorm *a, cudaStream_t s) {
-    const int wpr = warps_of(a->D, V * NV), threads = wpr == 1 ? 32 * kGroups : 32 * wpr;
-    const unsigned n = (unsigned)ctas(a->rows, a->D, V * NV);
-    if (V * NV == kEpt && threads <= kSmall)
-        k_ln_fwd<TX, TY, V, NV, V * NV == kEpt ? kSmall : 1024><<<n, threads, 0, s>>>(*a, wpr);
+    const int wpr = warps_of(a->D, EPT), t = threads_of(wpr);
+    const unsigned n = (unsigned)ctas(a->rows, wpr);
+    if (V > 1 && a->D == 32L * wpr * EPT)
+        k_ln_fwd<TX, TY, V, EPT, (V > 1), KEEP><<<n, t, 0, s>>>(*a, wpr);
     else
-        k_ln_fwd<TX, TY, V, NV, 1024><<<n, threads, 0, s>>>(*a, wpr);
+        k_ln_fwd<TX, TY, V, EPT, false, KEEP><<<n, t, 0, s>>>(*a, wpr);
+}
+
+template <typename TX, typename TY, int V>
+bool fwd_v(const KmbLayerNorm *a, cudaStream_t s) {
+    if (a->D > (V > 1 ? kFwdWide : kFwdKeep)) return false;
+    if (a->D > kFwdKeep) run_fwd<TX, TY, V, 32, V == 1>(a, s);
+    else if (fwd_ept(a->D) == 8) run_fwd<TX, TY, V, 8, true>(a, s);
+    else if (fwd_ept(a->D) == 16) run_fwd<TX, TY, V, 16, true>(a, s);
+    else run_fwd<TX, TY, V, 32, true>(a, s);
+    return true;
 }
 
 template <typename TX, typename TY>
 int fwd(const KmbLayerNorm *a, cudaStream_t s) {
     constexpr int V = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;
-    const bool vec = a->D % V == 0 && aligned(a->x, a->ld_x, a->x_type, V) && aligned(a->y, a->ld_y, a->y_type, V);
-    if (a->D <= kMaxD)
-        vec ? run_fwd<TX, TY, V, kEpt / V>(a, s) : run_fwd<TX, TY, 1, kEpt>(a, s);
-    else if (a->D <= kWideD && vec)
-        run_fwd<TX, TY, V, kWideEpt / V>(a, s);
-    else
+    /* the widest rows read weight and bias by pairs */
+    const bool vec = a->D % V == 0 && aligned(a->x, a->ld_x, sizeof(TX), V) &&
+                     aligned(a->y, a->ld_y, sizeof(TY), V) &&
+                     (a->D <= kFwdKeep || (aligned(a->weight, 0, 4, 2) && aligned(a->bias, 0, 4, 2)));
+    if (!(vec ? fwd_v<TX, TY, V>(a, s) : fwd_v<TX, TY, 1>(a, s)))
         k_ln_fwd_loop<TX, TY><<<(unsigned)(a->rows < 4 * kSMs ? a->rows : 4 * kSMs), kLoop, 0, s>>>(*a);
     return done();
 }
 
-template <typename TX, typename TY, int V, int NV>
+template <typename TX, typename TY, int V, int EPT>
 void run_bwd(const KmbLayerNorm *a, int sums, cudaStream_t s) {
-    const int wpr = warps_of(a->D, V * NV), threads = wpr == 1 ? 32 * kGroups : 32 * wpr;
-    const unsigned n = (unsigned)ctas(a->rows, a->D, V * NV);
-    if (threads <= kSmall)
-        k_ln_bwd<TX, TY, V, NV, kSmall><<<n, threads, 0, s>>>(*a, wpr, sums);
+    const int wpr = warps_of(a->D, EPT), t = threads_of(wpr);
+    const unsigned n = (unsigned)ctas(a->rows, wpr);
+    if (V > 1 && a->D == 32L * wpr * EPT)
+        k_ln_bwd<TX, TY, V, EPT, (V > 1)><<<n, t, 0, s>>>(*a, wpr, sums);
     else
-        k_ln_bwd<TX, TY, V, NV, 1024><<<n, threads, 0, s>>>(*a, wpr, sums);
+        k_ln_bwd<TX, TY, V, EPT, false><<<n, t, 0, s>>>(*a, wpr, sums);
+}
+
+template <typename TX, typename TY, int V>
+void bwd_v(const KmbLayerNorm *a, int sums, cudaStream_t s) {
+    if (bwd_ept(a->D) == 8) run_bwd<TX, TY, V, 8>(a, sums, s);
+    else run_bwd<TX, TY, V, 16>(a, sums, s);
 }
 
 constexpr size_t kColsShared = 200 * 1024; /* of the 227 KB an SM can give a CTA */
@@ -536,11 +544,11 @@ int bwd(const KmbLayerNorm *a, cudaStream_t s) {
     constexpr int V = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;
     const int sums = a->dweight || a->dbias;
     const long parts = kmb_layernorm_parts(a->rows, a->D);
-    const bool vec = a->D % V == 0 && aligned(a->x, a->ld_x, a->x_type, V) &&
-                     aligned(a->dy, a->ld_dy, a->y_type, V) && aligned(a->dx, a->ld_dx, a->x_type, V) &&
-                     aligned(a->dres, a->ld_dres, a->x_type, V);
-    if (a->rows && a->D <= kMaxD) {
-        vec ? run_bwd<TX, TY, V, kEpt / V>(a, sums, s) : run_bwd<TX, TY, 1, kEpt>(a, sums, s);
+    const bool vec = a->D % V == 0 && aligned(a->x, a->ld_x, sizeof(TX), V) &&
+                     aligned(a->dy, a->ld_dy, sizeof(TY), V) && aligned(a->dx, a->ld_dx, sizeof(TX), V) &&
+                     aligned(a->dres, a->ld_dres, sizeof(TX), V);
+    if (a->rows && a->D <= kBwdMax) {
+        vec ? bwd_v<TX, TY, V>(a, sums, s) : bwd_v<TX, TY, 1>(a, sums, s);
     } else if (a->rows) {
         const size_t bytes = 8 * (size_t)a->D;
         const int shared = sums && bytes <= kColsShared;
@@ -561,7 +569,7 @@ int bwd(const KmbLayerNorm *a, cudaStream_t s) {
 } // namespace
 
 extern "C" long kmb_layernorm_parts(long rows, long D) {
-    if (D <= kMaxD) return ctas(rows, D, kEpt);
+    if (D <= kBwdMax) return ctas(rows, warps_of(D, bwd_ept(D)));
     const long most = 8 * D <= (long)kColsShared ? kSMs : 4 * kSMs;
     return rows < most ? (rows > 0 ? rows : 1) : most;
 }
