@@ -351,6 +351,9 @@ typedef struct {
 
 int kmb_layernorm_fwd(const KmbLayerNorm *args);
 int kmb_layernorm_bwd(const KmbLayerNorm *args);
+/* KMB_ETIMEOUT when a bounded wait for a row's copy gave up since the last
+ * check (synchronous calls check it themselves). */
+int kmb_layernorm_check_error(void);
 /* Workspace of kmb_layernorm_bwd for args->rows and args->D (0 when the
  * sizes are invalid). */
 size_t kmb_layernorm_workspace_bytes(const KmbLayerNorm *args);

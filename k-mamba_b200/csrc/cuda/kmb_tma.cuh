@@ -1,0 +1,62 @@
+/*
+ * Transaction barriers and bulk copies into shared memory (sm_90+), with
+ * bounded waits.
+ */
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+__device__ __forceinline__ uint32_t kmb_smem(const void *p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+__device__ __forceinline__ void kmb_mbar_init(uint64_t *bar, uint32_t arrivals) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(kmb_smem(bar)), "r"(arrivals) : "memory");
+}
+/* makes the initialised barriers visible to the copies' completion */
+__device__ __forceinline__ void kmb_mbar_init_fence() {
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+/* one arrival that also announces `bytes` of copies */
+__device__ __forceinline__ void kmb_mbar_expect(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kmb_smem(bar)), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void kmb_mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(kmb_smem(bar)) : "memory");
+}
+__device__ __forceinline__ bool kmb_mbar_done(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(kmb_smem(bar)), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+/* Waits for the phase with `parity`, at most about 2^31 cycles; then *error
+ * is set, and later waits of the launch give up at once.  False when it gave
+ * up. */
+__device__ __forceinline__ bool kmb_mbar_wait(uint64_t *bar, uint32_t parity, int *error) {
+    if (kmb_mbar_done(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (int n = 1;; ++n) {
+        if (kmb_mbar_done(bar, parity)) return true;
+        if ((n & 15) == 0) {
+            const bool late = clock64() - t0 > (1ll << 31);
+            if (late) atomicExch(error, 1);
+            if (late || *reinterpret_cast<volatile int *>(error)) return false;
+        }
+    }
+}
+
+/* `bytes` (a multiple of 16, both addresses 16-byte aligned) from global to
+ * this CTA's shared memory, counted on bar. */
+__device__ __forceinline__ void kmb_bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     kmb_smem(dst)),
+                 "l"(src), "r"(bytes), "r"(kmb_smem(bar))
+                 : "memory");
+}

@@ -17,12 +17,14 @@
 #include <cuda_bf16.h>
 
 #include "kmb_common.cuh"
+#include "kmb_tma.cuh"
 #include "../kmb_internal.h"
 
 namespace {
 
 constexpr int kSMs = 148;
-constexpr int kWarps = 8;      /* warps of a CTA whose warps have a row each */
+constexpr int kWarps = 8;      /* warps of a CTA whose warps have their own rows */
+constexpr int kStages = 3;     /* rows of a ring */
 constexpr int kLoop = 512;     /* threads for rows that do not stay in registers */
 
 __device__ __forceinline__ float ld(const float *p) { return *p; }
@@ -37,6 +39,7 @@ template <>
 struct Vec<float, 1> {
     float v;
     __device__ __forceinline__ void load(const float *p) { v = __ldcs(p); }
+    __device__ __forceinline__ void take(const float *p) { v = *p; }
     __device__ __forceinline__ void get(float *f) const { f[0] = v; }
     static __device__ __forceinline__ void store(float *p, const float *f) { __stcs(p, f[0]); }
 };
@@ -44,6 +47,7 @@ template <>
 struct Vec<float, 4> {
     float4 v;
     __device__ __forceinline__ void load(const float *p) { v = __ldcs(reinterpret_cast<const float4 *>(p)); }
+    __device__ __forceinline__ void take(const float *p) { v = *reinterpret_cast<const float4 *>(p); }
     __device__ __forceinline__ void get(float *f) const {
         f[0] = v.x;
         f[1] = v.y;
@@ -68,6 +72,7 @@ struct Vec<__nv_bfloat16, 1> {
     __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
         v = __ldcs(reinterpret_cast<const unsigned short *>(p));
     }
+    __device__ __forceinline__ void take(const __nv_bfloat16 *p) { v = *reinterpret_cast<const unsigned short *>(p); }
     __device__ __forceinline__ void get(float *f) const { f[0] = __uint_as_float((unsigned)v << 16); }
     static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float *f) {
         __stcs(reinterpret_cast<unsigned short *>(p), (unsigned short)pack2(f[0], 0.f));
@@ -77,6 +82,7 @@ template <>
 struct Vec<__nv_bfloat16, 4> {
     uint2 v;
     __device__ __forceinline__ void load(const __nv_bfloat16 *p) { v = __ldcs(reinterpret_cast<const uint2 *>(p)); }
+    __device__ __forceinline__ void take(const __nv_bfloat16 *p) { v = *reinterpret_cast<const uint2 *>(p); }
     __device__ __forceinline__ void get(float *f) const {
         unpack2(v.x, f);
         unpack2(v.y, f + 2);
@@ -89,6 +95,7 @@ template <>
 struct Vec<__nv_bfloat16, 8> {
     uint4 v;
     __device__ __forceinline__ void load(const __nv_bfloat16 *p) { v = __ldcs(reinterpret_cast<const uint4 *>(p)); }
+    __device__ __forceinline__ void take(const __nv_bfloat16 *p) { v = *reinterpret_cast<const uint4 *>(p); }
     __device__ __forceinline__ void get(float *f) const {
         unpack2(v.x, f);
         unpack2(v.y, f + 2);
@@ -101,8 +108,9 @@ struct Vec<__nv_bfloat16, 8> {
     }
 };
 
-/* Sums over the threads of a row: a warp, or with more than one warp a row
+/* Sums over the threads of a row: L lanes, or with more than one warp a row
  * the whole CTA, through two slots in turn, so that one barrier a sum does. */
+template <int L>
 struct Reducer {
     float2 (*slot)[32];
     int warps; /* of a row */
@@ -111,7 +119,7 @@ struct Reducer {
     template <bool TWO>
     __device__ __forceinline__ float2 sum(float a, float b) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
+        for (int o = L / 2; o; o >>= 1) {
             a += __shfl_xor_sync(~0u, a, o);
             if (TWO) b += __shfl_xor_sync(~0u, b, o);
         }
@@ -129,6 +137,9 @@ struct Reducer {
     }
     __device__ __forceinline__ float2 two(float a, float b) { return sum<true>(a, b); }
     __device__ __forceinline__ float one(float a) { return sum<false>(a, 0.f).x; }
+    /* whether p holds for one of the rows that sum together: a warp's threads
+     * have to take the same way to the next sum */
+    __device__ __forceinline__ bool any(bool p) const { return L < 32 ? __any_sync(~0u, p) : p; }
 };
 
 /* Sums of rows whose plain fp32 sums overflow are taken again on scaled
@@ -137,40 +148,56 @@ struct Reducer {
 constexpr float kDown = 0x1p-32f, kUp = 0x1p32f, kSqDown = 0x1p-80f;
 
 /* sum(f): the sum of f(pair) over the row's values, pairs of values */
-template <typename Sum>
-__device__ __forceinline__ void row_stats(Sum sum, float n, float eps, float &mean, float &rstd) {
+template <typename Red, typename Sum>
+__device__ __forceinline__ void row_stats(const Red &red, Sum sum, float n, float eps, float &mean,
+                                          float &rstd) {
     mean = sum([](float2 x) { return x; }) / n;
-    if (!isfinite(mean)) mean = sum([](float2 x) { return kmb_mul2(x, kmb_f2s(kDown)); }) / n * kUp;
+    if (red.any(!isfinite(mean))) {
+        const float t = sum([](float2 x) { return kmb_mul2(x, kmb_f2s(kDown)); }) / n * kUp;
+        if (!isfinite(mean)) mean = t;
+    }
     const float2 m = kmb_f2s(-mean);
     const float s = sum([&](float2 x) {
         const float2 c = kmb_add2(x, m);
         return kmb_mul2(c, c);
     });
     rstd = 1.f / sqrtf(s / n + eps);
-    if (!isfinite(s)) {
+    if (red.any(!isfinite(s))) {
         const float t = sum([&](float2 x) {
             const float2 c = kmb_mul2(kmb_add2(x, m), kmb_f2s(kSqDown));
             return kmb_mul2(c, c);
         });
-        rstd = kSqDown / sqrtf(t / n + eps * kSqDown * kSqDown);
+        if (!isfinite(s)) rstd = kSqDown / sqrtf(t / n + eps * kSqDown * kSqDown);
     }
 }
 
-/* The thread's columns of a row of `tpr` threads, EPT of them at most:
- * vector k begins at col(k); all of a vector's columns exist or none.  FULL:
- * all exist. */
-template <int V, int EPT, bool FULL>
+/* The thread's columns of a row: each block of L threads has L * EPT
+ * columns in a row, EPT / V vectors a thread, a vector of the block's
+ * threads side by side.  All of a vector's columns exist or none.  FULL: all
+ * exist. */
+template <int V, int EPT, int L, bool FULL>
 struct Cols {
     static constexpr int NV = EPT / V;
-    int t, tpr, D;
-    __device__ __forceinline__ int col(int k) const { return (t + k * tpr) * V; }
+    int base, D; /* the first column */
+    __device__ __forceinline__ Cols(int t, int d) : base((t / L) * L * EPT + (t % L) * V), D(d) {}
+    __device__ __forceinline__ int col(int k) const { return base + k * (L * V); }
     __device__ __forceinline__ bool in(int k) const { return FULL || col(k) < D; }
     __device__ __forceinline__ bool has(int e) const { return in(e / V); } /* value e */
     __device__ __forceinline__ void vector(const float *p, float none, float *out) const {
 #pragma unroll
         for (int e = 0; e < EPT; ++e) out[e] = p && has(e) ? p[col(e / V) + e % V] : none;
     }
-    /* values that do not exist are 0 */
+    /* from shared memory; values that do not exist are 0 */
+    template <typename T>
+    __device__ __forceinline__ void take(const T *p, float2 (&x)[EPT / 2]) const {
+        Vec<T, V> raw[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (in(k)) raw[k].take(p + col(k));
+            else raw[k] = Vec<T, V>{};
+        }
+        unpack(raw, x);
+    }
     template <typename T>
     __device__ __forceinline__ void fetch(const T *p, Vec<T, V> (&raw)[NV]) const {
 #pragma unroll
@@ -221,30 +248,123 @@ struct Cols {
 /* forward                                                              */
 /* ------------------------------------------------------------------ */
 
-/* KEEP: weight and bias stay in registers */
-template <typename TX, typename TY, int V, int EPT, bool FULL, bool KEEP>
+/* set when a wait for a row gave up (kmb_layernorm_check_error) */
+__device__ int g_ln_error;
+
+/* Threads that share rows: `rows` consecutive ones of the walk at a time.
+ * With one warp a row (or several rows a warp) each warp walks on its own. */
+template <int L>
+struct Walk {
+    int wpr, group, groups, t; /* t: the thread's place among a row's */
+    __device__ __forceinline__ explicit Walk(int w) : wpr(w) {
+        constexpr int per = 32 / L;
+        group = w == 1 ? (int)threadIdx.x / L : 0;
+        groups = w == 1 ? (int)blockDim.x / 32 * per : 1;
+        t = w == 1 ? (int)threadIdx.x % L : (int)threadIdx.x;
+    }
+    __device__ __forceinline__ long first() const { return (long)blockIdx.x * groups + group; }
+    __device__ __forceinline__ long step() const { return (long)gridDim.x * groups; }
+};
+
+/*
+ * A ring of kStages rows in shared memory, filled by bulk copies: the rows
+ * behind the one in work are under way, whatever the registers hold.  A
+ * stage is filled again one row late, behind the barrier of the next row's
+ * sums, when every thread is done with it.
+ */
+__host__ __device__ constexpr int ring_head(int rings) { return (rings * kStages * 8 + 127) / 128 * 128; }
+
+struct Ring {
+    char *buf;     /* kStages stages */
+    uint64_t *bar; /* one a stage */
+    int stride;    /* bytes of a stage */
+    int stage, parity;
+    bool leader;
+
+    __device__ __forceinline__ void start(char *smem, int row_bytes, int wpr) {
+        const int own = wpr == 1 ? (int)threadIdx.x / 32 : 0, rings = wpr == 1 ? (int)blockDim.x / 32 : 1;
+        stride = row_bytes;
+        bar = reinterpret_cast<uint64_t *>(smem) + own * kStages;
+        buf = smem + ring_head(rings) + (long)own * kStages * row_bytes;
+        leader = wpr == 1 ? threadIdx.x % 32 == 0 : threadIdx.x == 0;
+        stage = parity = 0;
+        if (leader)
+            for (int k = 0; k < kStages; ++k) kmb_mbar_init(bar + k, 1);
+        kmb_mbar_init_fence();
+        if (wpr == 1) __syncwarp();
+        else __syncthreads();
+    }
+    __device__ __forceinline__ char *at(int k) const { return buf + k * stride; }
+    __device__ __forceinline__ char *row() const { return at(stage); }
+    __device__ __forceinline__ void wait() {
+        if (!kmb_mbar_wait(bar + stage, parity, &g_ln_error)) /* once more, for the copies under way */
+            kmb_mbar_wait(bar + stage, parity, &g_ln_error);
+    }
+    __device__ __forceinline__ int before() const { return stage ? stage - 1 : kStages - 1; }
+    __device__ __forceinline__ void next() {
+        if (++stage == kStages) {
+            stage = 0;
+            parity ^= 1;
+        }
+    }
+};
+
+/* KEEP: weight and bias stay in registers.  RING: rows come through a ring. */
+template <typename TX, typename TY, int V, int EPT, int L, bool FULL, bool KEEP, bool RING>
 __global__ void __launch_bounds__(KEEP ? 512 : 1024) k_ln_fwd(const __grid_constant__ KmbLayerNorm a, int wpr) {
+    extern __shared__ __align__(128) char smem[];
     __shared__ float2 slot[2][32];
-    typedef Cols<V, EPT, FULL> C;
-    const bool single = wpr == 1;
-    const int groups = single ? (int)blockDim.x / 32 : 1;
-    const C c = {single ? (int)threadIdx.x % 32 : (int)threadIdx.x, wpr * 32, (int)a.D};
-    Reducer red(slot, wpr);
+    typedef Cols<V, EPT, L, FULL> C;
+    const Walk<L> walk(wpr);
+    const C c(walk.t, (int)a.D);
+    Reducer<L> red(slot, wpr);
     float w[KEEP ? EPT : 2], b[KEEP ? EPT : 2];
     if (KEEP) {
         c.vector(a.weight, 1.f, w);
         c.vector(a.bias, 0.f, b);
     }
-    for (long r = (long)blockIdx.x * groups + (single ? threadIdx.x / 32 : 0); r < a.rows;
-         r += (long)gridDim.x * groups) {
+    const long step = walk.step();
+    const int bytes = (int)(a.D * sizeof(TX));
+    Ring ring = {};
+    const auto fill = [&](int k, long row) {
+        if (!ring.leader || row >= a.rows) return;
+        kmb_mbar_expect(ring.bar + k, bytes);
+        kmb_bulk_load(ring.at(k), (const TX *)a.x + row * a.ld_x, bytes, ring.bar + k);
+    };
+    if (RING) {
+        ring.start(smem, bytes, wpr);
+        for (int k = 0; k < kStages - 1; ++k) fill(k, walk.first() + k * step);
+    }
+    /* with several rows a warp all of its lanes walk as long as one of them */
+    for (long r = walk.first(); L < 32 ? r - walk.group % (32 / L) < a.rows : r < a.rows; r += step) {
+        const bool live = L == 32 || r < a.rows;
         float2 x[EPT / 2];
-        {
+        if (RING) {
+            ring.wait();
+            c.take((const TX *)ring.row(), x);
+        } else if (live) {
             Vec<TX, V> raw[C::NV];
             c.fetch((const TX *)a.x + r * a.ld_x, raw);
             C::unpack(raw, x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPT / 2; ++e) x[e] = kmb_f2s(0.f);
         }
         float mean, rstd;
-        row_stats([&](auto f) { return red.one(c.sum(x, f)); }, (float)a.D, a.eps, mean, rstd);
+        bool filled = !RING;
+        row_stats(
+            red,
+            [&](auto f) {
+                const float v = red.one(c.sum(x, f));
+                if (!filled) { /* every thread is done with the row before */
+                    if (wpr == 1) __syncwarp();
+                    fill(ring.before(), r + (kStages - 1) * step);
+                    filled = true;
+                }
+                return v;
+            },
+            (float)a.D, a.eps, mean, rstd);
+        if (RING) ring.next();
         const float2 m = kmb_f2s(-mean), s = kmb_f2s(rstd);
 #pragma unroll
         for (int e = 0; e < EPT / 2; ++e) {
@@ -260,8 +380,9 @@ __global__ void __launch_bounds__(KEEP ? 512 : 1024) k_ln_fwd(const __grid_const
             }
             x[e] = kmb_fma2(kmb_mul2(kmb_add2(x[e], m), s), wv, bv);
         }
+        if (!live) continue;
         c.store((TY *)a.y + r * a.ld_y, x);
-        if (c.t == 0) {
+        if (walk.t == 0) {
             if (a.mean) a.mean[r] = mean;
             if (a.rstd) a.rstd[r] = rstd;
         }
@@ -272,12 +393,13 @@ __global__ void __launch_bounds__(KEEP ? 512 : 1024) k_ln_fwd(const __grid_const
 template <typename TX, typename TY>
 __global__ void __launch_bounds__(kLoop) k_ln_fwd_loop(const __grid_constant__ KmbLayerNorm a) {
     __shared__ float2 slot[2][32];
-    Reducer red(slot, kLoop / 32);
+    Reducer<32> red(slot, kLoop / 32);
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const TX *x = (const TX *)a.x + r * a.ld_x;
         TY *y = (TY *)a.y + r * a.ld_y;
         float mean, rstd;
         row_stats(
+            red,
             [&](auto f) {
                 float s = 0.f;
                 for (long j = threadIdx.x; j < a.D; j += kLoop) s += f(kmb_f2s(ld(x + j))).x;
@@ -297,43 +419,60 @@ __global__ void __launch_bounds__(kLoop) k_ln_fwd_loop(const __grid_constant__ K
 /* backward                                                             */
 /* ------------------------------------------------------------------ */
 
-/* The next row's loads are in flight while a row is reduced. */
-template <typename TX, typename TY, int V, int EPT, bool FULL>
+template <typename TX, typename TY, int V, int EPT, int L, bool FULL, bool RING>
 __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayerNorm a, int wpr, int sums) {
+    extern __shared__ __align__(128) char smem[];
     __shared__ float2 slot[2][32];
-    __shared__ float fold[kWarps][32 * EPT];
-    typedef Cols<V, EPT, FULL> C;
-    const bool single = wpr == 1;
-    const int groups = single ? (int)blockDim.x / 32 : 1, warp = threadIdx.x / 32;
-    const C c = {single ? (int)threadIdx.x % 32 : (int)threadIdx.x, wpr * 32, (int)a.D};
-    Reducer red(slot, wpr);
-    const long step = (long)gridDim.x * groups;
-    long r = (long)blockIdx.x * groups + (single ? warp : 0);
+    typedef Cols<V, EPT, L, FULL> C;
+    const Walk<L> walk(wpr);
+    const C c(walk.t, (int)a.D);
+    Reducer<L> red(slot, wpr);
     const float inv = 1.f / (float)a.D;
     float w[EPT];
     c.vector(a.weight, 1.f, w);
     float2 pw[EPT / 2], pb[EPT / 2];
 #pragma unroll
     for (int e = 0; e < EPT / 2; ++e) pw[e] = pb[e] = kmb_f2s(0.f);
-    Vec<TX, V> rx[C::NV];
-    Vec<TY, V> rd[C::NV];
-    float mean = 0.f, rstd = 0.f;
-    const auto fetch = [&](long row) {
-        c.fetch((const TX *)a.x + row * a.ld_x, rx);
-        c.fetch((const TY *)a.dy + row * a.ld_dy, rd);
-        if (a.mean) {
-            mean = a.mean[row];
-            rstd = a.rstd[row];
-        }
+    const long step = walk.step();
+    const int xb = (int)(a.D * sizeof(TX)), yb = (int)(a.D * sizeof(TY));
+    const int bytes = xb + yb + (a.dres ? xb : 0);
+    Ring ring = {};
+    const auto fill = [&](int k, long row) {
+        if (!ring.leader || row >= a.rows) return;
+        kmb_mbar_expect(ring.bar + k, bytes);
+        kmb_bulk_load(ring.at(k), (const TX *)a.x + row * a.ld_x, xb, ring.bar + k);
+        kmb_bulk_load(ring.at(k) + xb, (const TY *)a.dy + row * a.ld_dy, yb, ring.bar + k);
+        if (a.dres)
+            kmb_bulk_load(ring.at(k) + xb + yb, (const TX *)a.dres + row * a.ld_dres, xb, ring.bar + k);
     };
-    if (r < a.rows) fetch(r);
-    for (; r < a.rows; r += step) {
+    if (RING) {
+        ring.start(smem, bytes, wpr);
+        for (int k = 0; k < kStages - 1; ++k) fill(k, walk.first() + k * step);
+    }
+    for (long r = walk.first(); L < 32 ? r - walk.group % (32 / L) < a.rows : r < a.rows; r += step) {
+        const bool live = L == 32 || r < a.rows;
         float2 h[EPT / 2], d[EPT / 2];
-        C::unpack(rx, h);
-        C::unpack(rd, d);
-        float m = mean, s = rstd;
-        if (r + step < a.rows) fetch(r + step);
-        if (!a.mean) row_stats([&](auto f) { return red.one(c.sum(h, f)); }, (float)a.D, a.eps, m, s);
+        float m = 0.f, s = 0.f;
+        if (live && a.mean) {
+            m = a.mean[r];
+            s = a.rstd[r];
+        }
+        if (RING) {
+            ring.wait();
+            c.take((const TX *)ring.row(), h);
+            c.take((const TY *)(ring.row() + xb), d);
+        } else if (live) {
+            Vec<TX, V> rx[C::NV];
+            Vec<TY, V> rd[C::NV];
+            c.fetch((const TX *)a.x + r * a.ld_x, rx);
+            c.fetch((const TY *)a.dy + r * a.ld_dy, rd);
+            C::unpack(rx, h);
+            C::unpack(rd, d);
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPT / 2; ++e) h[e] = d[e] = kmb_f2s(0.f);
+        }
+        if (!a.mean) row_stats(red, [&](auto f) { return red.one(c.sum(h, f)); }, (float)a.D, a.eps, m, s);
         float2 t1 = kmb_f2s(0.f), t2 = t1;
         const float2 m2 = kmb_f2s(-m), sd = kmb_f2s(s);
 #pragma unroll
@@ -346,34 +485,45 @@ __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayer
             t2 = kmb_fma2(d[e], h[e], t2);
         }
         const float2 t = red.two(t1.x + t1.y, t2.x + t2.y);
+        if (RING) { /* every thread is done with the row before */
+            if (wpr == 1) __syncwarp();
+            fill(ring.before(), r + (kStages - 1) * step);
+        }
         const float2 s1 = kmb_f2s(-t.x * inv), s2 = kmb_f2s(-t.y * inv);
 #pragma unroll
         for (int e = 0; e < EPT / 2; ++e) d[e] = kmb_mul2(kmb_fma2(h[e], s2, kmb_add2(d[e], s1)), sd);
-        if (a.dres) {
-            Vec<TX, V> raw[C::NV];
-            c.fetch((const TX *)a.dres + r * a.ld_dres, raw);
-            C::unpack(raw, h);
+        if (a.dres && live) {
+            if (RING) {
+                c.take((const TX *)(ring.row() + xb + yb), h);
+            } else {
+                Vec<TX, V> raw[C::NV];
+                c.fetch((const TX *)a.dres + r * a.ld_dres, raw);
+                C::unpack(raw, h);
+            }
 #pragma unroll
             for (int e = 0; e < EPT / 2; ++e) d[e] = kmb_add2(d[e], h[e]);
         }
-        c.store((TX *)a.dx + r * a.ld_dx, d);
+        if (RING) ring.next();
+        if (live) c.store((TX *)a.dx + r * a.ld_dx, d);
     }
     if (!sums) return;
     float *part = (float *)a.workspace + (long)blockIdx.x * 2 * a.D;
+    if (wpr > 1) {
+        c.columns(part, pw);
+        c.columns(part + a.D, pb);
+        return;
+    }
+    /* one row a group: added through shared memory, the ring's stages when there is one */
+    float *fold = reinterpret_cast<float *>(smem + (RING ? ring_head(blockDim.x / 32) : 0));
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-        float2 (&v)[EPT / 2] = which ? pb : pw;
-        if (!single) {
-            c.columns(part + which * a.D, v);
-            continue;
-        }
         __syncthreads();
-        c.columns(fold[warp], v);
+        c.columns(fold + walk.group * (L * EPT), which ? pb : pw);
         __syncthreads();
         for (int j = threadIdx.x; j < a.D; j += blockDim.x) {
-            float t = 0.f;
-            for (int g = 0; g < groups; ++g) t += fold[g][j];
-            part[which * a.D + j] = t;
+            float v = 0.f;
+            for (int g = 0; g < walk.groups; ++g) v += fold[g * (L * EPT) + j];
+            part[which * a.D + j] = v;
         }
     }
 }
@@ -386,7 +536,7 @@ __global__ void __launch_bounds__(kLoop) k_ln_bwd_loop(const __grid_constant__ K
                                                        int in_shared) {
     extern __shared__ float cols[];
     __shared__ float2 slot[2][32];
-    Reducer red(slot, kLoop / 32);
+    Reducer<32> red(slot, kLoop / 32);
     float *part = (float *)a.workspace + (long)blockIdx.x * 2 * a.D;
     float *pw = in_shared ? cols : part, *pb = pw + a.D;
     if (sums)
@@ -403,6 +553,7 @@ __global__ void __launch_bounds__(kLoop) k_ln_bwd_loop(const __grid_constant__ K
             rstd = a.rstd[r];
         } else {
             row_stats(
+                red,
                 [&](auto f) {
                     float s = 0.f;
                     for (long j = threadIdx.x; j < a.D; j += kLoop) s += f(kmb_f2s(ld(x + j))).x;
@@ -463,25 +614,40 @@ __global__ void __launch_bounds__(1024) k_ln_sums(const float *part, long parts,
 /* ------------------------------------------------------------------ */
 
 /* Values of a thread.  More of them mean fewer sums across threads (each
- * costs a warp 5 shuffles and a barrier), fewer mean more rows in flight. */
-int fwd_ept(long D) { return D <= 256 ? 8 : D <= 512 ? 16 : 32; }
-int bwd_ept(long D) { return D <= 256 ? 8 : 16; }
-constexpr long kFwdKeep = 512 * 32, kFwdWide = 1024 * 32, kBwdMax = 512 * 16;
+ * costs a warp 5 shuffles and a barrier), fewer mean more rows in flight.  Up
+ * to 128 columns four rows share a warp. */
+int fwd_ept(long D) { return D <= 128 ? 16 : D <= 256 ? 8 : D <= 512 ? 16 : 32; }
+int bwd_ept(long D) { return D <= 128 ? 16 : D <= 256 ? 8 : 16; }
+constexpr long kNarrow = 128, kFwdKeep = 512 * 32, kFwdWide = 1024 * 32, kBwdMax = 512 * 16;
 
-int warps_of(long D, int ept) { return (int)((D + 32 * ept - 1) / (32 * ept)); }
+int warps_of(long D, int ept) { return D <= kNarrow ? 1 : (int)((D + 32 * ept - 1) / (32 * ept)); }
 int threads_of(int wpr) { return 32 * (wpr == 1 ? kWarps : wpr); }
 
 /* CTAs of a resident kernel of 512 threads an SM (128 registers each), no
  * more than there are rows (or groups of rows) */
-long ctas(long rows, int wpr) {
-    const long need = wpr == 1 ? (rows + kWarps - 1) / kWarps : rows;
+long ctas(long rows, long D, int wpr) {
+    const int per = wpr > 1 ? 1 : D <= kNarrow ? 4 * kWarps : kWarps;
+    const long need = (rows + per - 1) / per;
     const int fit = 512 / threads_of(wpr);
     const long most = (long)kSMs * (fit > 0 ? fit : 1);
     return need < most ? (need > 0 ? need : 1) : most;
 }
 
+/* Shared memory of a ring of rows of `bytes`, 0 when a row's CTAs would not
+ * fit side by side (512 threads an SM). */
+size_t ring_bytes(int wpr, size_t bytes) {
+    const int rings = wpr == 1 ? kWarps : 1, t = threads_of(wpr);
+    const size_t n = ring_head(rings) + (size_t)rings * kStages * bytes;
+    const int fit = 512 / t > 0 ? 512 / t : 1;
+    return n * fit <= 208 * 1024 ? n : 0;
+}
+
 bool aligned(const void *p, long ld, size_t es, int v) {
     return !p || ((size_t)p % (es * v) == 0 && ld % v == 0);
+}
+/* rows that a bulk copy can take */
+bool bulk(const void *p, long ld, long D, size_t es) {
+    return !p || ((size_t)p % 16 == 0 && ld * es % 16 == 0 && D * es % 16 == 0);
 }
 
 int done() {
@@ -489,24 +655,45 @@ int done() {
     return e == cudaSuccess ? KMB_OK : kmb_cuda_fail(e, "layernorm: launch");
 }
 
-template <typename TX, typename TY, int V, int EPT, bool KEEP>
-void run_fwd(const KmbLayerNorm *a, cudaStream_t s) {
+template <typename K>
+int more_shared(K kernel, size_t bytes) {
+    if (bytes <= 48 * 1024) return KMB_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return e == cudaSuccess ? KMB_OK : kmb_cuda_fail(e, "layernorm: shared memory");
+}
+
+template <typename TX, typename TY, int V, int EPT, int L, bool KEEP>
+int run_fwd(const KmbLayerNorm *a, cudaStream_t s) {
     const int wpr = warps_of(a->D, EPT), t = threads_of(wpr);
-    const unsigned n = (unsigned)ctas(a->rows, wpr);
-    if (V > 1 && a->D == 32L * wpr * EPT)
-        k_ln_fwd<TX, TY, V, EPT, (V > 1), KEEP><<<n, t, 0, s>>>(*a, wpr);
+    const unsigned n = (unsigned)ctas(a->rows, a->D, wpr);
+    constexpr bool VEC = V > 1;
+    if (VEC && L == 32 && bulk(a->x, a->ld_x, a->D, sizeof(TX))) {
+        const size_t ring = ring_bytes(wpr, a->D * sizeof(TX));
+        if (ring && a->rows > n) { /* more than a row a group */
+            auto k = a->D == 32L * wpr * EPT ? k_ln_fwd<TX, TY, V, EPT, L, VEC, KEEP, VEC && L == 32>
+                                             : k_ln_fwd<TX, TY, V, EPT, L, false, KEEP, VEC && L == 32>;
+            const int rc = more_shared(k, ring);
+            if (rc) return rc;
+            k<<<n, t, ring, s>>>(*a, wpr);
+            return done();
+        }
+    }
+    if (VEC && a->D == (long)L * wpr * EPT)
+        k_ln_fwd<TX, TY, V, EPT, L, VEC, KEEP, false><<<n, t, 0, s>>>(*a, wpr);
     else
-        k_ln_fwd<TX, TY, V, EPT, false, KEEP><<<n, t, 0, s>>>(*a, wpr);
+        k_ln_fwd<TX, TY, V, EPT, L, false, KEEP, false><<<n, t, 0, s>>>(*a, wpr);
+    return done();
 }
 
 template <typename TX, typename TY, int V>
-bool fwd_v(const KmbLayerNorm *a, cudaStream_t s) {
-    if (a->D > (V > 1 ? kFwdWide : kFwdKeep)) return false;
-    if (a->D > kFwdKeep) run_fwd<TX, TY, V, 32, V == 1>(a, s);
-    else if (fwd_ept(a->D) == 8) run_fwd<TX, TY, V, 8, true>(a, s);
-    else if (fwd_ept(a->D) == 16) run_fwd<TX, TY, V, 16, true>(a, s);
-    else run_fwd<TX, TY, V, 32, true>(a, s);
-    return true;
+int fwd_v(const KmbLayerNorm *a, cudaStream_t s) {
+    if (a->D <= kNarrow) return run_fwd<TX, TY, V, 16, 8, true>(a, s);
+    if (fwd_ept(a->D) == 8) return run_fwd<TX, TY, V, 8, 32, true>(a, s);
+    if (fwd_ept(a->D) == 16) return run_fwd<TX, TY, V, 16, 32, true>(a, s);
+    if (a->D <= kFwdKeep) return run_fwd<TX, TY, V, 32, 32, true>(a, s);
+    if (V > 1 && a->D <= kFwdWide) return run_fwd<TX, TY, V, 32, 32, V == 1>(a, s);
+    k_ln_fwd_loop<TX, TY><<<(unsigned)(a->rows < 4 * kSMs ? a->rows : 4 * kSMs), kLoop, 0, s>>>(*a);
+    return done();
 }
 
 template <typename TX, typename TY>
@@ -516,25 +703,40 @@ int fwd(const KmbLayerNorm *a, cudaStream_t s) {
     const bool vec = a->D % V == 0 && aligned(a->x, a->ld_x, sizeof(TX), V) &&
                      aligned(a->y, a->ld_y, sizeof(TY), V) &&
                      (a->D <= kFwdKeep || (aligned(a->weight, 0, 4, 2) && aligned(a->bias, 0, 4, 2)));
-    if (!(vec ? fwd_v<TX, TY, V>(a, s) : fwd_v<TX, TY, 1>(a, s)))
-        k_ln_fwd_loop<TX, TY><<<(unsigned)(a->rows < 4 * kSMs ? a->rows : 4 * kSMs), kLoop, 0, s>>>(*a);
+    return vec ? fwd_v<TX, TY, V>(a, s) : fwd_v<TX, TY, 1>(a, s);
+}
+
+template <typename TX, typename TY, int V, int EPT, int L>
+int run_bwd(const KmbLayerNorm *a, int sums, cudaStream_t s) {
+    const int wpr = warps_of(a->D, EPT), t = threads_of(wpr);
+    const unsigned n = (unsigned)ctas(a->rows, a->D, wpr);
+    const size_t fold = sums && wpr == 1 ? (size_t)kWarps * (32 / L) * L * EPT * 4 : 0;
+    constexpr bool VEC = V > 1;
+    if (VEC && L == 32 && bulk(a->x, a->ld_x, a->D, sizeof(TX)) && bulk(a->dy, a->ld_dy, a->D, sizeof(TY)) &&
+        bulk(a->dres, a->ld_dres, a->D, sizeof(TX))) {
+        size_t ring = ring_bytes(wpr, a->D * (sizeof(TX) * (a->dres ? 2 : 1) + sizeof(TY)));
+        if (ring && a->rows > n) {
+            auto k = a->D == 32L * wpr * EPT ? k_ln_bwd<TX, TY, V, EPT, L, VEC, VEC && L == 32>
+                                             : k_ln_bwd<TX, TY, V, EPT, L, false, VEC && L == 32>;
+            if (fold && ring < ring_head(kWarps) + fold) ring = ring_head(kWarps) + fold;
+            const int rc = more_shared(k, ring);
+            if (rc) return rc;
+            k<<<n, t, ring, s>>>(*a, wpr, sums);
+            return done();
+        }
+    }
+    if (VEC && a->D == (long)L * wpr * EPT)
+        k_ln_bwd<TX, TY, V, EPT, L, VEC, false><<<n, t, fold, s>>>(*a, wpr, sums);
+    else
+        k_ln_bwd<TX, TY, V, EPT, L, false, false><<<n, t, fold, s>>>(*a, wpr, sums);
     return done();
 }
 
-template <typename TX, typename TY, int V, int EPT>
-void run_bwd(const KmbLayerNorm *a, int sums, cudaStream_t s) {
-    const int wpr = warps_of(a->D, EPT), t = threads_of(wpr);
-    const unsigned n = (unsigned)ctas(a->rows, wpr);
-    if (V > 1 && a->D == 32L * wpr * EPT)
-        k_ln_bwd<TX, TY, V, EPT, (V > 1)><<<n, t, 0, s>>>(*a, wpr, sums);
-    else
-        k_ln_bwd<TX, TY, V, EPT, false><<<n, t, 0, s>>>(*a, wpr, sums);
-}
-
 template <typename TX, typename TY, int V>
-void bwd_v(const KmbLayerNorm *a, int sums, cudaStream_t s) {
-    if (bwd_ept(a->D) == 8) run_bwd<TX, TY, V, 8>(a, sums, s);
-    else run_bwd<TX, TY, V, 16>(a, sums, s);
+int bwd_v(const KmbLayerNorm *a, int sums, cudaStream_t s) {
+    if (a->D <= kNarrow) return run_bwd<TX, TY, V, 16, 8>(a, sums, s);
+    if (bwd_ept(a->D) == 8) return run_bwd<TX, TY, V, 8, 32>(a, sums, s);
+    return run_bwd<TX, TY, V, 16, 32>(a, sums, s);
 }
 
 constexpr size_t kColsShared = 200 * 1024; /* of the 227 KB an SM can give a CTA */
@@ -548,7 +750,8 @@ int bwd(const KmbLayerNorm *a, cudaStream_t s) {
                      aligned(a->dy, a->ld_dy, sizeof(TY), V) && aligned(a->dx, a->ld_dx, sizeof(TX), V) &&
                      aligned(a->dres, a->ld_dres, sizeof(TX), V);
     if (a->rows && a->D <= kBwdMax) {
-        vec ? bwd_v<TX, TY, V>(a, sums, s) : bwd_v<TX, TY, 1>(a, sums, s);
+        const int rc = vec ? bwd_v<TX, TY, V>(a, sums, s) : bwd_v<TX, TY, 1>(a, sums, s);
+        if (rc) return rc;
     } else if (a->rows) {
         const size_t bytes = 8 * (size_t)a->D;
         const int shared = sums && bytes <= kColsShared;
@@ -569,7 +772,7 @@ int bwd(const KmbLayerNorm *a, cudaStream_t s) {
 } // namespace
 
 extern "C" long kmb_layernorm_parts(long rows, long D) {
-    if (D <= kBwdMax) return ctas(rows, warps_of(D, bwd_ept(D)));
+    if (D <= kBwdMax) return ctas(rows, D, warps_of(D, bwd_ept(D)));
     const long most = 8 * D <= (long)kColsShared ? kSMs : 4 * kSMs;
     return rows < most ? (rows > 0 ? rows : 1) : most;
 }
@@ -584,4 +787,18 @@ extern "C" int kmb_launch_layernorm_bwd(const KmbLayerNorm *a, cudaStream_t s) {
     const int x16 = a->x_type == KMB_BF16, y16 = a->y_type == KMB_BF16;
     if (x16) return y16 ? bwd<__nv_bfloat16, __nv_bfloat16>(a, s) : bwd<__nv_bfloat16, float>(a, s);
     return y16 ? bwd<float, __nv_bfloat16>(a, s) : bwd<float, float>(a, s);
+}
+
+/* KMB_ETIMEOUT (and the word cleared) when a wait for a row gave up since
+ * the last check. */
+extern "C" int kmb_layernorm_check_error(void) {
+    int flag = 0;
+    const cudaError_t e = cudaMemcpyFromSymbol(&flag, g_ln_error, sizeof flag);
+    if (e != cudaSuccess) return kmb_cuda_fail(e, "layernorm: error word");
+    if (flag) {
+        const int zero = 0;
+        (void)cudaMemcpyToSymbol(g_ln_error, &zero, sizeof zero);
+        return kmb_fail(KMB_ETIMEOUT, "layernorm: a wait for a row expired");
+    }
+    return KMB_OK;
 }

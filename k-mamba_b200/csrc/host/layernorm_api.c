@@ -56,7 +56,8 @@ int kmb_layernorm_fwd(const KmbLayerNorm *a) {
     if ((rc = kmb_check_capture("layernorm", kmb_stream(), 0))) return rc;
     kmb_stage_begin(&st);
     rc = a->rows ? kmb_launch_layernorm_fwd(a, st.s) : KMB_OK;
-    return kmb_stage_finish(&st, rc);
+    rc = kmb_stage_finish(&st, rc);
+    return !rc && kmb_sync_enabled() ? kmb_layernorm_check_error() : rc;
 }
 
 int kmb_layernorm_bwd(const KmbLayerNorm *a) {
@@ -81,5 +82,6 @@ int kmb_layernorm_bwd(const KmbLayerNorm *a) {
     d = *a;
     if (need && !d.workspace) d.workspace = kmb_scratch(&st, need);
     rc = st.status ? st.status : kmb_launch_layernorm_bwd(&d, st.s);
-    return kmb_stage_finish(&st, rc);
+    rc = kmb_stage_finish(&st, rc);
+    return !rc && kmb_sync_enabled() ? kmb_layernorm_check_error() : rc;
 }

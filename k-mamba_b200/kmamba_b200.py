@@ -328,6 +328,7 @@ PROTOTYPES = {
     # layer norm
     "kmb_layernorm_fwd": (C.c_int, [C.POINTER(KmbLayerNorm)]),
     "kmb_layernorm_bwd": (C.c_int, [C.POINTER(KmbLayerNorm)]),
+    "kmb_layernorm_check_error": (C.c_int, []),
     "kmb_layernorm_workspace_bytes": (C.c_size_t, [C.POINTER(KmbLayerNorm)]),
     # gated linear recurrence
     "kmb_glr_ckpt_elems": (lg, [C.POINTER(KmbGLR)]),
