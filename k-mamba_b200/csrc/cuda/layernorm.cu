@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kSMs = 148;
 constexpr int kWarps = 8;      /* warps of a CTA whose warps have their own rows */
-constexpr int kStages = 3;     /* rows of a ring */
+constexpr int kStages = 8;     /* most stages of a ring */
 constexpr int kLoop = 512;     /* threads for rows that do not stay in registers */
 
 __device__ __forceinline__ float ld(const float *p) { return *p; }
@@ -173,38 +173,73 @@ __device__ __forceinline__ void row_stats(const Red &red, Sum sum, float n, floa
 
 /* The thread's columns of a row: each block of L threads has L * EPT
  * columns in a row, EPT / V vectors a thread, a vector of the block's
- * threads side by side.  All of a vector's columns exist or none.  FULL: all
- * exist. */
-template <int V, int EPT, int L, bool FULL>
+ * threads side by side.  All of a vector's columns exist or none. */
+template <int V, int EPT, int L>
 struct Cols {
     static constexpr int NV = EPT / V;
-    int base, D; /* the first column */
-    __device__ __forceinline__ Cols(int t, int d) : base((t / L) * L * EPT + (t % L) * V), D(d) {}
-    __device__ __forceinline__ int col(int k) const { return base + k * (L * V); }
-    __device__ __forceinline__ bool in(int k) const { return FULL || col(k) < D; }
-    __device__ __forceinline__ bool has(int e) const { return in(e / V); } /* value e */
-    __device__ __forceinline__ void vector(const float *p, float none, float *out) const {
-#pragma unroll
-        for (int e = 0; e < EPT; ++e) out[e] = p && has(e) ? p[col(e / V) + e % V] : none;
+    int base, left; /* the first column, columns from there to the row's end */
+    bool full;      /* all columns of the block exist: asked once, not for each value */
+    __device__ __forceinline__ Cols(int t, int D) : base((t / L) * L * EPT + (t % L) * V) {
+        left = D - base;
+        full = (t / L + 1) * L * EPT <= D;
     }
-    /* from shared memory; values that do not exist are 0 */
-    template <typename T>
-    __device__ __forceinline__ void take(const T *p, float2 (&x)[EPT / 2]) const {
-        Vec<T, V> raw[NV];
+    static __device__ __forceinline__ constexpr int off(int k) { return k * (L * V); }
+    __device__ __forceinline__ bool in(int k) const { return off(k) < left; }
+    /* f(k) for the vectors that exist, else g(k) */
+    template <typename F, typename G>
+    __device__ __forceinline__ void each(F f, G g) const {
+        if (full) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (in(k)) raw[k].take(p + col(k));
-            else raw[k] = Vec<T, V>{};
+            for (int k = 0; k < NV; ++k) f(k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                if (in(k)) f(k);
+                else g(k);
+            }
         }
-        unpack(raw, x);
     }
-    template <typename T>
-    __device__ __forceinline__ void fetch(const T *p, Vec<T, V> (&raw)[NV]) const {
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        each(f, [](int) {});
+    }
+    /* a [D] vector, `none` where NULL or not there; vectors of 4 where its address allows */
+    __device__ __forceinline__ void vector(const float *p, float none, float2 (&out)[EPT / 2]) const {
+        float f[EPT];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (in(k)) raw[k].load(p + col(k));
-            else raw[k] = Vec<T, V>{};
+        for (int e = 0; e < EPT; ++e) f[e] = none;
+        if (p) {
+            p += base;
+            if (V >= 4 && ((size_t)p & 15) == 0)
+                each([&](int k) {
+#pragma unroll
+                    for (int e = 0; e < V / 4; ++e)
+                        *reinterpret_cast<float4 *>(f + k * V + 4 * e) =
+                            *reinterpret_cast<const float4 *>(p + off(k) + 4 * e);
+                });
+            else
+                each([&](int k) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) f[k * V + e] = p[off(k) + e];
+                });
         }
+#pragma unroll
+        for (int e = 0; e < EPT / 2; ++e) out[e] = kmb_f2(f[2 * e], f[2 * e + 1]);
+    }
+    /* to a [D] vector whose address allows vectors of 4 (V >= 4) */
+    __device__ __forceinline__ void columns(float *p, const float2 (&x)[EPT / 2]) const {
+        p += base;
+        each([&](int k) {
+            if (V >= 4) {
+#pragma unroll
+                for (int e = 0; e < V / 4; ++e) {
+                    const float2 l = x[(k * V + 4 * e) / 2], h = x[(k * V + 4 * e) / 2 + 1];
+                    *reinterpret_cast<float4 *>(p + off(k) + 4 * e) = make_float4(l.x, l.y, h.x, h.y);
+                }
+            } else {
+                p[off(k)] = k % 2 ? x[k / 2].y : x[k / 2].x;
+            }
+        });
     }
     template <typename T>
     static __device__ __forceinline__ void unpack(const Vec<T, V> (&raw)[NV], float2 (&x)[EPT / 2]) {
@@ -214,6 +249,19 @@ struct Cols {
 #pragma unroll
         for (int e = 0; e < EPT / 2; ++e) x[e] = kmb_f2(f[2 * e], f[2 * e + 1]);
     }
+    /* the row's values from shared memory (RING) or global memory; 0 where there are none */
+    template <bool RING, typename T>
+    __device__ __forceinline__ void fetch(const T *p, Vec<T, V> (&raw)[NV]) const {
+        p += base;
+        each([&](int k) { RING ? raw[k].take(p + off(k)) : raw[k].load(p + off(k)); },
+             [&](int k) { raw[k] = Vec<T, V>{}; });
+    }
+    template <bool RING, typename T>
+    __device__ __forceinline__ void load(const T *p, float2 (&x)[EPT / 2]) const {
+        Vec<T, V> raw[NV];
+        fetch<RING>(p, raw);
+        unpack(raw, x);
+    }
     template <typename T>
     __device__ __forceinline__ void store(T *p, const float2 (&x)[EPT / 2]) const {
         float f[EPT];
@@ -222,24 +270,24 @@ struct Cols {
             f[2 * e] = x[e].x;
             f[2 * e + 1] = x[e].y;
         }
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (in(k)) Vec<T, V>::store(p + col(k), f + k * V);
+        p += base;
+        each([&](int k) { Vec<T, V>::store(p + off(k), f + k * V); });
     }
-    __device__ __forceinline__ void columns(float *p, const float2 (&x)[EPT / 2]) const {
-#pragma unroll
-        for (int e = 0; e < EPT; ++e)
-            if (has(e)) p[col(e / V) + e % V] = e % 2 ? x[e / 2].y : x[e / 2].x;
-    }
-    /* 0 where a value does not exist */
-    __device__ __forceinline__ float2 mask(int pair, float2 v) const {
-        return kmb_f2(has(2 * pair) ? v.x : 0.f, has(2 * pair + 1) ? v.y : 0.f);
-    }
+    /* the sum of f(pair) over the values that exist */
     template <typename Fn>
     __device__ __forceinline__ float sum(const float2 (&x)[EPT / 2], Fn f) const {
         float2 s = kmb_f2s(0.f);
+        if (full) {
 #pragma unroll
-        for (int e = 0; e < EPT / 2; ++e) s = kmb_add2(s, mask(e, f(x[e])));
+            for (int e = 0; e < EPT / 2; ++e) s = kmb_add2(s, f(x[e]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPT / 2; ++e) {
+                const float2 v = f(x[e]);
+                s.x += in(2 * e / V) ? v.x : 0.f;
+                s.y += in((2 * e + 1) / V) ? v.y : 0.f;
+            }
+        }
         return s.x + s.y;
     }
 };
@@ -267,88 +315,126 @@ struct Walk {
 };
 
 /*
- * A ring of kStages rows in shared memory, filled by bulk copies: the rows
- * behind the one in work are under way, whatever the registers hold.  A
- * stage is filled again one row late, behind the barrier of the next row's
- * sums, when every thread is done with it.
+ * A ring of rows in shared memory, filled by bulk copies: the rows behind
+ * the one in work are under way, whatever the registers hold.  A stage has
+ * one row of each group that walks together, and is filled again one row
+ * late, behind the sums of the next row, when every thread is done with it.
+ *
+ * A bulk copy moves whole 16-byte pieces.  A row that does not begin or end
+ * on one is copied with the rest of its first and last piece, bytes of the
+ * rows beside it, and read from where it begins inside.  A row whose pieces
+ * would leave the tensor (the first or the last, when it is not aligned) is
+ * loaded by its threads.
  */
+enum { kNone, kWhole, kPieces }; /* no ring, rows of whole aligned pieces, any rows */
 __host__ __device__ constexpr int ring_head(int rings) { return (rings * kStages * 8 + 127) / 128 * 128; }
+__host__ __device__ constexpr int ring_slot(long bytes, int mode) {
+    return mode == kPieces ? (int)((bytes + 15) / 16 * 16 + 16) : (int)bytes;
+}
 
+template <int L, int MODE>
 struct Ring {
-    char *buf;     /* kStages stages */
+    char *buf;     /* the group's row of stage 0 */
     uint64_t *bar; /* one a stage */
-    int stride;    /* bytes of a stage */
+    int row_bytes, stage_bytes, stages;
     int stage, parity;
     bool leader;
 
-    __device__ __forceinline__ void start(char *smem, int row_bytes, int wpr) {
+    __device__ __forceinline__ void start(char *smem, int bytes, int n, int wpr) {
+        constexpr int per = 32 / L;
         const int own = wpr == 1 ? (int)threadIdx.x / 32 : 0, rings = wpr == 1 ? (int)blockDim.x / 32 : 1;
-        stride = row_bytes;
+        row_bytes = bytes;
+        stage_bytes = per * bytes;
+        stages = n;
         bar = reinterpret_cast<uint64_t *>(smem) + own * kStages;
-        buf = smem + ring_head(rings) + (long)own * kStages * row_bytes;
-        leader = wpr == 1 ? threadIdx.x % 32 == 0 : threadIdx.x == 0;
+        buf = smem + ring_head(rings) + (long)own * n * stage_bytes + (threadIdx.x % 32) / L * bytes;
+        leader = wpr == 1 ? threadIdx.x % L == 0 : threadIdx.x == 0;
         stage = parity = 0;
-        if (leader)
-            for (int k = 0; k < kStages; ++k) kmb_mbar_init(bar + k, 1);
+        if (wpr == 1 ? threadIdx.x % 32 == 0 : threadIdx.x == 0)
+            for (int k = 0; k < n; ++k) kmb_mbar_init(bar + k, per);
         kmb_mbar_init_fence();
         if (wpr == 1) __syncwarp();
         else __syncthreads();
     }
-    __device__ __forceinline__ char *at(int k) const { return buf + k * stride; }
-    __device__ __forceinline__ char *row() const { return at(stage); }
+    __device__ __forceinline__ char *at(int k) const { return buf + k * stage_bytes; }
     __device__ __forceinline__ void wait() {
         if (!kmb_mbar_wait(bar + stage, parity, &g_ln_error)) /* once more, for the copies under way */
             kmb_mbar_wait(bar + stage, parity, &g_ln_error);
     }
-    __device__ __forceinline__ int before() const { return stage ? stage - 1 : kStages - 1; }
+    __device__ __forceinline__ int before() const { return stage ? stage - 1 : stages - 1; }
     __device__ __forceinline__ void next() {
-        if (++stage == kStages) {
+        if (++stage == stages) {
             stage = 0;
             parity ^= 1;
         }
     }
+    static __device__ __forceinline__ uint32_t lead(const void *p) {
+        return MODE == kPieces ? (uint32_t)(uintptr_t)p & 15u : 0u;
+    }
+    static __device__ __forceinline__ uint32_t span(const void *p, int bytes) {
+        return MODE == kPieces ? (lead(p) + (uint32_t)bytes + 15u) & ~15u : (uint32_t)bytes;
+    }
+    /* whether the pieces of the row leave the tensor: its threads load it */
+    static __device__ __forceinline__ bool odd(const void *p, int bytes, const void *base, long past) {
+        if (MODE != kPieces) return false;
+        return (const char *)p - lead(p) < (const char *)base ||
+               (const char *)p - lead(p) + span(p, bytes) > (const char *)base + past;
+    }
+    __device__ __forceinline__ void copy(int k, int where, const void *p, int bytes) const {
+        kmb_bulk_load(at(k) + where, (const char *)p - lead(p), span(p, bytes), bar + k);
+    }
 };
 
-/* KEEP: weight and bias stay in registers.  RING: rows come through a ring. */
-template <typename TX, typename TY, int V, int EPT, int L, bool FULL, bool KEEP, bool RING>
-__global__ void __launch_bounds__(KEEP ? 512 : 1024) k_ln_fwd(const __grid_constant__ KmbLayerNorm a, int wpr) {
+/* KEEP: weight and bias stay in registers.  MODE: whether rows come through
+ * a ring of `stages`; narrow rows without one are loaded a turn ahead. */
+template <typename TX, typename TY, int V, int EPT, int L, bool KEEP, int MODE>
+__global__ void __launch_bounds__(KEEP ? 512 : 1024) k_ln_fwd(const __grid_constant__ KmbLayerNorm a, int wpr,
+                                                             int stages) {
     extern __shared__ __align__(128) char smem[];
     __shared__ float2 slot[2][32];
-    typedef Cols<V, EPT, L, FULL> C;
+    typedef Cols<V, EPT, L> C;
+    constexpr bool RING = MODE != kNone, AHEAD = !RING && L < 32;
     const Walk<L> walk(wpr);
     const C c(walk.t, (int)a.D);
     Reducer<L> red(slot, wpr);
-    float w[KEEP ? EPT : 2], b[KEEP ? EPT : 2];
-    if (KEEP) {
+    float2 w[KEEP ? EPT / 2 : 1], b[KEEP ? EPT / 2 : 1];
+    if constexpr (KEEP) {
         c.vector(a.weight, 1.f, w);
         c.vector(a.bias, 0.f, b);
     }
     const long step = walk.step();
     const int bytes = (int)(a.D * sizeof(TX));
-    Ring ring = {};
+    const auto at = [&](long row) { return (const TX *)a.x + row * a.ld_x; };
+    const long past = ((a.rows - 1) * a.ld_x + a.D) * (long)sizeof(TX);
+    Ring<L, MODE> ring = {};
     const auto fill = [&](int k, long row) {
-        if (!ring.leader || row >= a.rows) return;
-        kmb_mbar_expect(ring.bar + k, bytes);
-        kmb_bulk_load(ring.at(k), (const TX *)a.x + row * a.ld_x, bytes, ring.bar + k);
+        if (!ring.leader) return;
+        if (row >= a.rows || ring.odd(at(row), bytes, a.x, past)) {
+            kmb_mbar_arrive(ring.bar + k);
+        } else {
+            kmb_mbar_expect(ring.bar + k, ring.span(at(row), bytes));
+            ring.copy(k, 0, at(row), bytes);
+        }
     };
     if (RING) {
-        ring.start(smem, bytes, wpr);
-        for (int k = 0; k < kStages - 1; ++k) fill(k, walk.first() + k * step);
+        ring.start(smem, ring_slot(bytes, MODE), stages, wpr);
+        for (int k = 0; k < stages - 1; ++k) fill(k, walk.first() + k * step);
     }
+    Vec<TX, V> raw[C::NV] = {};
+    if (AHEAD && walk.first() < a.rows) c.template fetch<false>(at(walk.first()), raw);
     /* with several rows a warp all of its lanes walk as long as one of them */
     for (long r = walk.first(); L < 32 ? r - walk.group % (32 / L) < a.rows : r < a.rows; r += step) {
         const bool live = L == 32 || r < a.rows;
         float2 x[EPT / 2];
-        if (RING) {
-            ring.wait();
-            c.take((const TX *)ring.row(), x);
-        } else if (live) {
-            Vec<TX, V> raw[C::NV];
-            c.fetch((const TX *)a.x + r * a.ld_x, raw);
+        if (AHEAD) {
             C::unpack(raw, x);
+            if (r + step < a.rows) c.template fetch<false>(at(r + step), raw);
         } else {
-#pragma unroll
-            for (int e = 0; e < EPT / 2; ++e) x[e] = kmb_f2s(0.f);
+            if (RING) ring.wait();
+            if (RING && !ring.odd(at(r), bytes, a.x, past))
+                c.template load<true>((const TX *)(ring.at(ring.stage) + ring.lead(at(r))), x);
+            else
+                c.template load<false>(at(r), x);
         }
         float mean, rstd;
         bool filled = !RING;
@@ -358,29 +444,28 @@ __global__ void __launch_bounds__(KEEP ? 512 : 1024) k_ln_fwd(const __grid_const
                 const float v = red.one(c.sum(x, f));
                 if (!filled) { /* every thread is done with the row before */
                     if (wpr == 1) __syncwarp();
-                    fill(ring.before(), r + (kStages - 1) * step);
+                    fill(ring.before(), r + (stages - 1) * step);
                     filled = true;
                 }
                 return v;
             },
             (float)a.D, a.eps, mean, rstd);
         if (RING) ring.next();
-        const float2 m = kmb_f2s(-mean), s = kmb_f2s(rstd);
-#pragma unroll
-        for (int e = 0; e < EPT / 2; ++e) {
-            float2 wv, bv;
-            if (KEEP) {
-                wv = kmb_f2(w[2 * e], w[2 * e + 1]);
-                bv = kmb_f2(b[2 * e], b[2 * e + 1]);
-            } else {
-                const int i = c.col(2 * e / V) + 2 * e % V;
-                const bool ok = c.has(2 * e);
-                wv = ok && a.weight ? *reinterpret_cast<const float2 *>(a.weight + i) : kmb_f2s(1.f);
-                bv = ok && a.bias ? *reinterpret_cast<const float2 *>(a.bias + i) : kmb_f2s(0.f);
-            }
-            x[e] = kmb_fma2(kmb_mul2(kmb_add2(x[e], m), s), wv, bv);
-        }
         if (!live) continue;
+        const float2 m = kmb_f2s(-mean), s = kmb_f2s(rstd);
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int e = 0; e < EPT / 2; ++e) x[e] = kmb_fma2(kmb_mul2(kmb_add2(x[e], m), s), w[e], b[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPT / 2; ++e) {
+                const int i = c.base + c.off(2 * e / V) + 2 * e % V;
+                const bool ok = c.in(2 * e / V);
+                const float2 wv = ok && a.weight ? *reinterpret_cast<const float2 *>(a.weight + i) : kmb_f2s(1.f);
+                const float2 bv = ok && a.bias ? *reinterpret_cast<const float2 *>(a.bias + i) : kmb_f2s(0.f);
+                x[e] = kmb_fma2(kmb_mul2(kmb_add2(x[e], m), s), wv, bv);
+            }
+        }
         c.store((TY *)a.y + r * a.ld_y, x);
         if (walk.t == 0) {
             if (a.mean) a.mean[r] = mean;
@@ -419,58 +504,83 @@ __global__ void __launch_bounds__(kLoop) k_ln_fwd_loop(const __grid_constant__ K
 /* backward                                                             */
 /* ------------------------------------------------------------------ */
 
-template <typename TX, typename TY, int V, int EPT, int L, bool FULL, bool RING>
-__global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayerNorm a, int wpr, int sums) {
+template <typename TX, typename TY, int V, int EPT, int L, int MODE>
+__global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayerNorm a, int wpr, int sums,
+                                                int stages) {
     extern __shared__ __align__(128) char smem[];
     __shared__ float2 slot[2][32];
-    typedef Cols<V, EPT, L, FULL> C;
+    typedef Cols<V, EPT, L> C;
+    constexpr bool RING = MODE != kNone, AHEAD = !RING && L < 32;
     const Walk<L> walk(wpr);
     const C c(walk.t, (int)a.D);
     Reducer<L> red(slot, wpr);
     const float inv = 1.f / (float)a.D;
-    float w[EPT];
+    float2 w[EPT / 2], pw[EPT / 2], pb[EPT / 2];
     c.vector(a.weight, 1.f, w);
-    float2 pw[EPT / 2], pb[EPT / 2];
 #pragma unroll
     for (int e = 0; e < EPT / 2; ++e) pw[e] = pb[e] = kmb_f2s(0.f);
     const long step = walk.step();
     const int xb = (int)(a.D * sizeof(TX)), yb = (int)(a.D * sizeof(TY));
-    const int bytes = xb + yb + (a.dres ? xb : 0);
-    Ring ring = {};
+    const int xs = ring_slot(xb, MODE), ys = ring_slot(yb, MODE); /* places of x | dy | dres in a row's slot */
+    const auto x_at = [&](long row) { return (const TX *)a.x + row * a.ld_x; };
+    const auto d_at = [&](long row) { return (const TY *)a.dy + row * a.ld_dy; };
+    const auto r_at = [&](long row) { return (const TX *)a.dres + row * a.ld_dres; };
+    Ring<L, MODE> ring = {};
+    const long x_past = ((a.rows - 1) * a.ld_x + a.D) * (long)sizeof(TX);
+    const long d_past = ((a.rows - 1) * a.ld_dy + a.D) * (long)sizeof(TY);
+    const long r_past = ((a.rows - 1) * a.ld_dres + a.D) * (long)sizeof(TX);
+    const auto odd = [&](long row) {
+        return ring.odd(x_at(row), xb, a.x, x_past) || ring.odd(d_at(row), yb, a.dy, d_past) ||
+               (a.dres && ring.odd(r_at(row), xb, a.dres, r_past));
+    };
     const auto fill = [&](int k, long row) {
-        if (!ring.leader || row >= a.rows) return;
-        kmb_mbar_expect(ring.bar + k, bytes);
-        kmb_bulk_load(ring.at(k), (const TX *)a.x + row * a.ld_x, xb, ring.bar + k);
-        kmb_bulk_load(ring.at(k) + xb, (const TY *)a.dy + row * a.ld_dy, yb, ring.bar + k);
-        if (a.dres)
-            kmb_bulk_load(ring.at(k) + xb + yb, (const TX *)a.dres + row * a.ld_dres, xb, ring.bar + k);
+        if (!ring.leader) return;
+        if (row >= a.rows || odd(row)) {
+            kmb_mbar_arrive(ring.bar + k);
+            return;
+        }
+        kmb_mbar_expect(ring.bar + k, ring.span(x_at(row), xb) + ring.span(d_at(row), yb) +
+                                          (a.dres ? ring.span(r_at(row), xb) : 0u));
+        ring.copy(k, 0, x_at(row), xb);
+        ring.copy(k, xs, d_at(row), yb);
+        if (a.dres) ring.copy(k, xs + ys, r_at(row), xb);
     };
     if (RING) {
-        ring.start(smem, bytes, wpr);
-        for (int k = 0; k < kStages - 1; ++k) fill(k, walk.first() + k * step);
+        ring.start(smem, xs + ys + (a.dres ? xs : 0), stages, wpr);
+        for (int k = 0; k < stages - 1; ++k) fill(k, walk.first() + k * step);
+    }
+    Vec<TX, V> rx[C::NV] = {};
+    Vec<TY, V> rd[C::NV] = {};
+    if (AHEAD && walk.first() < a.rows) {
+        c.template fetch<false>(x_at(walk.first()), rx);
+        c.template fetch<false>(d_at(walk.first()), rd);
     }
     for (long r = walk.first(); L < 32 ? r - walk.group % (32 / L) < a.rows : r < a.rows; r += step) {
         const bool live = L == 32 || r < a.rows;
+        const bool here = RING && !odd(r); /* the row is in the ring */
         float2 h[EPT / 2], d[EPT / 2];
         float m = 0.f, s = 0.f;
         if (live && a.mean) {
             m = a.mean[r];
             s = a.rstd[r];
         }
-        if (RING) {
-            ring.wait();
-            c.take((const TX *)ring.row(), h);
-            c.take((const TY *)(ring.row() + xb), d);
-        } else if (live) {
-            Vec<TX, V> rx[C::NV];
-            Vec<TY, V> rd[C::NV];
-            c.fetch((const TX *)a.x + r * a.ld_x, rx);
-            c.fetch((const TY *)a.dy + r * a.ld_dy, rd);
+        if (RING) ring.wait();
+        if (AHEAD) {
             C::unpack(rx, h);
             C::unpack(rd, d);
-        } else {
+            if (r + step < a.rows) {
+                c.template fetch<false>(x_at(r + step), rx);
+                c.template fetch<false>(d_at(r + step), rd);
+            } else { /* a lane without a row adds nothing to the columns' sums */
 #pragma unroll
-            for (int e = 0; e < EPT / 2; ++e) h[e] = d[e] = kmb_f2s(0.f);
+                for (int k = 0; k < C::NV; ++k) rd[k] = Vec<TY, V>{};
+            }
+        } else if (here) {
+            c.template load<true>((const TX *)(ring.at(ring.stage) + ring.lead(x_at(r))), h);
+            c.template load<true>((const TY *)(ring.at(ring.stage) + xs + ring.lead(d_at(r))), d);
+        } else {
+            c.template load<false>(x_at(r), h);
+            c.template load<false>(d_at(r), d);
         }
         if (!a.mean) row_stats(red, [&](auto f) { return red.one(c.sum(h, f)); }, (float)a.D, a.eps, m, s);
         float2 t1 = kmb_f2s(0.f), t2 = t1;
@@ -480,26 +590,23 @@ __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayer
             h[e] = kmb_mul2(kmb_add2(h[e], m2), sd);
             pw[e] = kmb_fma2(d[e], h[e], pw[e]);
             pb[e] = kmb_add2(pb[e], d[e]);
-            d[e] = kmb_mul2(d[e], kmb_f2(w[2 * e], w[2 * e + 1]));
+            d[e] = kmb_mul2(d[e], w[e]);
             t1 = kmb_add2(t1, d[e]);
             t2 = kmb_fma2(d[e], h[e], t2);
         }
         const float2 t = red.two(t1.x + t1.y, t2.x + t2.y);
         if (RING) { /* every thread is done with the row before */
             if (wpr == 1) __syncwarp();
-            fill(ring.before(), r + (kStages - 1) * step);
+            fill(ring.before(), r + (stages - 1) * step);
         }
         const float2 s1 = kmb_f2s(-t.x * inv), s2 = kmb_f2s(-t.y * inv);
 #pragma unroll
         for (int e = 0; e < EPT / 2; ++e) d[e] = kmb_mul2(kmb_fma2(h[e], s2, kmb_add2(d[e], s1)), sd);
         if (a.dres && live) {
-            if (RING) {
-                c.take((const TX *)(ring.row() + xb + yb), h);
-            } else {
-                Vec<TX, V> raw[C::NV];
-                c.fetch((const TX *)a.dres + r * a.ld_dres, raw);
-                C::unpack(raw, h);
-            }
+            if (here)
+                c.template load<true>((const TX *)(ring.at(ring.stage) + xs + ys + ring.lead(r_at(r))), h);
+            else
+                c.template load<false>(r_at(r), h);
 #pragma unroll
             for (int e = 0; e < EPT / 2; ++e) d[e] = kmb_add2(d[e], h[e]);
         }
@@ -586,26 +693,30 @@ __global__ void __launch_bounds__(kLoop) k_ln_bwd_loop(const __grid_constant__ K
         for (long j = threadIdx.x; j < 2 * a.D; j += kLoop) part[j] = cols[j]; /* its own columns */
 }
 
-/* dweight, dbias from the rows of partial sums: 32 columns a CTA, 32 rows
- * of threads, joined in a fixed order */
+/* dweight, dbias from the rows of partial sums: 32 columns a CTA, joined in
+ * a fixed order */
 __global__ void __launch_bounds__(1024) k_ln_sums(const float *part, long parts, long D, float *dw, float *db,
                                                   int acc) {
     __shared__ float s[32][33];
-    const int tx = threadIdx.x, ty = threadIdx.y;
+    const int tx = threadIdx.x, ty = threadIdx.y, rows = blockDim.y;
     const long j = (long)blockIdx.x * 32 + tx;
     float v = 0.f;
-    if (j < 2 * D)
-        for (long p = ty; p < parts; p += 32) v += part[p * 2 * D + j];
+    if (j < 2 * D) {
+        float u[4] = {0.f, 0.f, 0.f, 0.f};
+        long p = ty;
+        for (; p + 3 * rows < parts; p += 4 * rows)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) u[k] += part[(p + k * rows) * 2 * D + j];
+        for (; p < parts; p += rows) u[0] += part[p * 2 * D + j];
+        v = (u[0] + u[1]) + (u[2] + u[3]);
+    }
     s[ty][tx] = v;
     __syncthreads();
-    v = s[tx][ty]; /* column ty, rows over the lanes */
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-    const long k = (long)blockIdx.x * 32 + ty;
-    if (tx || k >= 2 * D) return;
-    float *to = k < D ? dw : db;
+    if (ty || j >= 2 * D) return;
+    for (int k = 1; k < rows; ++k) v += s[k][tx];
+    float *to = j < D ? dw : db;
     if (!to) return;
-    to += k < D ? k : k - D;
+    to += j < D ? j : j - D;
     *to = acc ? *to + v : v;
 }
 
@@ -633,21 +744,30 @@ long ctas(long rows, long D, int wpr) {
     return need < most ? (need > 0 ? need : 1) : most;
 }
 
-/* Shared memory of a ring of rows of `bytes`, 0 when a row's CTAs would not
- * fit side by side (512 threads an SM). */
-size_t ring_bytes(int wpr, size_t bytes) {
-    const int rings = wpr == 1 ? kWarps : 1, t = threads_of(wpr);
-    const size_t n = ring_head(rings) + (size_t)rings * kStages * bytes;
-    const int fit = 512 / t > 0 ? 512 / t : 1;
-    return n * fit <= 208 * 1024 ? n : 0;
+/* Stages of a ring whose rows take `bytes` each, 0 for no ring: enough that
+ * an SM has 64 KB under way (its share of the memory's bandwidth times the
+ * latency), two rows ahead where they fit. */
+int ring_stages(long D, int wpr, long bytes) {
+    const int rings = wpr == 1 ? kWarps : 1, fit = 512 / threads_of(wpr) > 0 ? 512 / threads_of(wpr) : 1;
+    const long all = bytes * rings * fit; /* of an SM */
+    if (D <= kNarrow) return 0;
+    int n = (int)(2 + (64 * 1024 - 1) / all);
+    if (n < 3) n = 3;
+    if (n > kStages) n = kStages;
+    while (n > 1 && n * all + fit * ring_head(rings) > 208 * 1024) --n;
+    return n > 1 ? n : 0;
+}
+size_t ring_size(int wpr, long bytes, int stages) {
+    const int rings = wpr == 1 ? kWarps : 1;
+    return ring_head(rings) + (size_t)rings * stages * bytes;
+}
+/* whether every row begins and ends on a 16-byte piece */
+bool whole(const void *p, long ld, long D, size_t es) {
+    return !p || ((size_t)p % 16 == 0 && ld * es % 16 == 0 && D * es % 16 == 0);
 }
 
 bool aligned(const void *p, long ld, size_t es, int v) {
     return !p || ((size_t)p % (es * v) == 0 && ld % v == 0);
-}
-/* rows that a bulk copy can take */
-bool bulk(const void *p, long ld, long D, size_t es) {
-    return !p || ((size_t)p % 16 == 0 && ld * es % 16 == 0 && D * es % 16 == 0);
 }
 
 int done() {
@@ -657,7 +777,7 @@ int done() {
 
 template <typename K>
 int more_shared(K kernel, size_t bytes) {
-    if (bytes <= 48 * 1024) return KMB_OK;
+    if (bytes <= 40 * 1024) return KMB_OK; /* 48 KB with the static part */
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     return e == cudaSuccess ? KMB_OK : kmb_cuda_fail(e, "layernorm: shared memory");
 }
@@ -666,22 +786,23 @@ template <typename TX, typename TY, int V, int EPT, int L, bool KEEP>
 int run_fwd(const KmbLayerNorm *a, cudaStream_t s) {
     const int wpr = warps_of(a->D, EPT), t = threads_of(wpr);
     const unsigned n = (unsigned)ctas(a->rows, a->D, wpr);
-    constexpr bool VEC = V > 1;
-    if (VEC && L == 32 && bulk(a->x, a->ld_x, a->D, sizeof(TX))) {
-        const size_t ring = ring_bytes(wpr, a->D * sizeof(TX));
-        if (ring && a->rows > n) { /* more than a row a group */
-            auto k = a->D == 32L * wpr * EPT ? k_ln_fwd<TX, TY, V, EPT, L, VEC, KEEP, VEC && L == 32>
-                                             : k_ln_fwd<TX, TY, V, EPT, L, false, KEEP, VEC && L == 32>;
-            const int rc = more_shared(k, ring);
-            if (rc) return rc;
-            k<<<n, t, ring, s>>>(*a, wpr);
-            return done();
-        }
+    const bool exact = V > 1 && whole(a->x, a->ld_x, a->D, sizeof(TX));
+    const long row = ring_slot(a->D * sizeof(TX), exact ? kWhole : kPieces);
+    /* Rows of 4 KB, one a warp, keep 64 KB of an SM under way by themselves:
+     * 262144 rows of 1024 fp32 take 249 us from global memory and 275 us
+     * through a ring; of 512, 345 and 253 us. */
+    const int stages = V > 1 && wpr == 1 && row >= 4096 ? 0 : ring_stages(a->D, wpr, row);
+    const long per = wpr > 1 ? 1 : kWarps * (32 / L);
+    if (L == 32 && stages && a->rows > n * per) { /* more than a row a group */
+        const size_t bytes = ring_size(wpr, row, stages);
+        constexpr int E = L == 32 && V > 1 ? kWhole : kNone, P = L == 32 ? kPieces : kNone;
+        auto k = exact ? k_ln_fwd<TX, TY, V, EPT, L, KEEP, E> : k_ln_fwd<TX, TY, V, EPT, L, KEEP, P>;
+        const int rc = more_shared(k, bytes);
+        if (rc) return rc;
+        k<<<n, t, bytes, s>>>(*a, wpr, stages);
+    } else {
+        k_ln_fwd<TX, TY, V, EPT, L, KEEP, kNone><<<n, t, 0, s>>>(*a, wpr, 0);
     }
-    if (VEC && a->D == (long)L * wpr * EPT)
-        k_ln_fwd<TX, TY, V, EPT, L, VEC, KEEP, false><<<n, t, 0, s>>>(*a, wpr);
-    else
-        k_ln_fwd<TX, TY, V, EPT, L, false, KEEP, false><<<n, t, 0, s>>>(*a, wpr);
     return done();
 }
 
@@ -710,25 +831,24 @@ template <typename TX, typename TY, int V, int EPT, int L>
 int run_bwd(const KmbLayerNorm *a, int sums, cudaStream_t s) {
     const int wpr = warps_of(a->D, EPT), t = threads_of(wpr);
     const unsigned n = (unsigned)ctas(a->rows, a->D, wpr);
-    const size_t fold = sums && wpr == 1 ? (size_t)kWarps * (32 / L) * L * EPT * 4 : 0;
-    constexpr bool VEC = V > 1;
-    if (VEC && L == 32 && bulk(a->x, a->ld_x, a->D, sizeof(TX)) && bulk(a->dy, a->ld_dy, a->D, sizeof(TY)) &&
-        bulk(a->dres, a->ld_dres, a->D, sizeof(TX))) {
-        size_t ring = ring_bytes(wpr, a->D * (sizeof(TX) * (a->dres ? 2 : 1) + sizeof(TY)));
-        if (ring && a->rows > n) {
-            auto k = a->D == 32L * wpr * EPT ? k_ln_bwd<TX, TY, V, EPT, L, VEC, VEC && L == 32>
-                                             : k_ln_bwd<TX, TY, V, EPT, L, false, VEC && L == 32>;
-            if (fold && ring < ring_head(kWarps) + fold) ring = ring_head(kWarps) + fold;
-            const int rc = more_shared(k, ring);
-            if (rc) return rc;
-            k<<<n, t, ring, s>>>(*a, wpr, sums);
-            return done();
-        }
+    const size_t fold = sums && wpr == 1 ? (size_t)kWarps * 32 * EPT * 4 : 0;
+    const bool exact = V > 1 && whole(a->x, a->ld_x, a->D, sizeof(TX)) &&
+                       whole(a->dy, a->ld_dy, a->D, sizeof(TY)) && whole(a->dres, a->ld_dres, a->D, sizeof(TX));
+    const int mode = exact ? kWhole : kPieces;
+    const long row = ring_slot(a->D * sizeof(TX), mode) * (a->dres ? 2 : 1) + ring_slot(a->D * sizeof(TY), mode);
+    const int stages = ring_stages(a->D, wpr, row);
+    const long per = wpr > 1 ? 1 : kWarps * (32 / L);
+    if (L == 32 && stages && a->rows > n * per) {
+        size_t bytes = ring_size(wpr, row, stages);
+        if (fold && bytes < ring_head(kWarps) + fold) bytes = ring_head(kWarps) + fold;
+        constexpr int E = L == 32 && V > 1 ? kWhole : kNone, P = L == 32 ? kPieces : kNone;
+        auto k = exact ? k_ln_bwd<TX, TY, V, EPT, L, E> : k_ln_bwd<TX, TY, V, EPT, L, P>;
+        const int rc = more_shared(k, bytes);
+        if (rc) return rc;
+        k<<<n, t, bytes, s>>>(*a, wpr, sums, stages);
+    } else {
+        k_ln_bwd<TX, TY, V, EPT, L, kNone><<<n, t, fold, s>>>(*a, wpr, sums, 0);
     }
-    if (VEC && a->D == (long)L * wpr * EPT)
-        k_ln_bwd<TX, TY, V, EPT, L, VEC, false><<<n, t, fold, s>>>(*a, wpr, sums);
-    else
-        k_ln_bwd<TX, TY, V, EPT, L, false, false><<<n, t, fold, s>>>(*a, wpr, sums);
     return done();
 }
 
@@ -764,7 +884,7 @@ int bwd(const KmbLayerNorm *a, cudaStream_t s) {
         k_ln_bwd_loop<TX, TY><<<(unsigned)parts, kLoop, shared ? bytes : 0, s>>>(*a, sums, shared);
     }
     if (sums)
-        k_ln_sums<<<(unsigned)((2 * a->D + 31) / 32), dim3(32, 32), 0, s>>>(
+        k_ln_sums<<<(unsigned)((2 * a->D + 31) / 32), dim3(32, parts > 256 ? 32 : 8), 0, s>>>(
             (const float *)a->workspace, a->rows ? parts : 0, a->D, a->dweight, a->dbias, a->accumulate);
     return done();
 }
