@@ -149,11 +149,11 @@ constexpr float kDown = 0x1p-32f, kUp = 0x1p32f, kSqDown = 0x1p-80f;
 
 /* sum(f): the sum of f(pair) over the row's values, pairs of values */
 template <typename Red, typename Sum>
-__device__ __forceinline__ void row_stats(const Red &red, Sum sum, float n, float eps, float &mean,
+__device__ __forceinline__ void row_stats(const Red &red, Sum sum, float inv, float eps, float &mean,
                                           float &rstd) {
-    mean = sum([](float2 x) { return x; }) / n;
+    mean = sum([](float2 x) { return x; }) * inv;
     if (red.any(!isfinite(mean))) {
-        const float t = sum([](float2 x) { return kmb_mul2(x, kmb_f2s(kDown)); }) / n * kUp;
+        const float t = sum([](float2 x) { return kmb_mul2(x, kmb_f2s(kDown)); }) * inv * kUp;
         if (!isfinite(mean)) mean = t;
     }
     const float2 m = kmb_f2s(-mean);
@@ -161,13 +161,13 @@ __device__ __forceinline__ void row_stats(const Red &red, Sum sum, float n, floa
         const float2 c = kmb_add2(x, m);
         return kmb_mul2(c, c);
     });
-    rstd = 1.f / sqrtf(s / n + eps);
+    rstd = rsqrtf(fmaf(s, inv, eps));
     if (red.any(!isfinite(s))) {
         const float t = sum([&](float2 x) {
             const float2 c = kmb_mul2(kmb_add2(x, m), kmb_f2s(kSqDown));
             return kmb_mul2(c, c);
         });
-        if (!isfinite(s)) rstd = kSqDown / sqrtf(t / n + eps * kSqDown * kSqDown);
+        if (!isfinite(s)) rstd = kSqDown * rsqrtf(fmaf(t, inv, eps * kSqDown * kSqDown));
     }
 }
 
@@ -310,15 +310,16 @@ struct Walk {
         groups = w == 1 ? (int)blockDim.x / 32 * per : 1;
         t = w == 1 ? (int)threadIdx.x % L : (int)threadIdx.x;
     }
-    __device__ __forceinline__ long first() const { return (long)blockIdx.x * groups + group; }
-    __device__ __forceinline__ long step() const { return (long)gridDim.x * groups; }
+    __device__ __forceinline__ unsigned first() const { return blockIdx.x * (unsigned)groups + (unsigned)group; }
+    __device__ __forceinline__ unsigned step() const { return gridDim.x * (unsigned)groups; }
 };
 
 /*
  * A ring of rows in shared memory, filled by bulk copies: the rows behind
  * the one in work are under way, whatever the registers hold.  A stage has
- * one row of each group that walks together, and is filled again one row
+ * one row, and is filled again one row
  * late, behind the sums of the next row, when every thread is done with it.
+ * (Only rows of more than kNarrow columns, at least 16 bytes apart.)
  *
  * A bulk copy moves whole 16-byte pieces.  A row that does not begin or end
  * on one is copied with the rest of its first and last piece, bytes of the
@@ -332,31 +333,29 @@ __host__ __device__ constexpr int ring_slot(long bytes, int mode) {
     return mode == kPieces ? (int)((bytes + 15) / 16 * 16 + 16) : (int)bytes;
 }
 
-template <int L, int MODE>
+template <int MODE>
 struct Ring {
-    char *buf;     /* the group's row of stage 0 */
+    char *buf;     /* stage 0 */
     uint64_t *bar; /* one a stage */
-    int row_bytes, stage_bytes, stages;
+    int bytes, stages;
     int stage, parity;
     bool leader;
 
-    __device__ __forceinline__ void start(char *smem, int bytes, int n, int wpr) {
-        constexpr int per = 32 / L;
+    __device__ __forceinline__ void start(char *smem, int row_bytes, int n, int wpr) {
         const int own = wpr == 1 ? (int)threadIdx.x / 32 : 0, rings = wpr == 1 ? (int)blockDim.x / 32 : 1;
-        row_bytes = bytes;
-        stage_bytes = per * bytes;
+        bytes = row_bytes;
         stages = n;
         bar = reinterpret_cast<uint64_t *>(smem) + own * kStages;
-        buf = smem + ring_head(rings) + (long)own * n * stage_bytes + (threadIdx.x % 32) / L * bytes;
-        leader = wpr == 1 ? threadIdx.x % L == 0 : threadIdx.x == 0;
+        buf = smem + ring_head(rings) + own * n * row_bytes;
+        leader = wpr == 1 ? threadIdx.x % 32 == 0 : threadIdx.x == 0;
         stage = parity = 0;
-        if (wpr == 1 ? threadIdx.x % 32 == 0 : threadIdx.x == 0)
-            for (int k = 0; k < n; ++k) kmb_mbar_init(bar + k, per);
+        if (leader)
+            for (int k = 0; k < n; ++k) kmb_mbar_init(bar + k, 1);
         kmb_mbar_init_fence();
         if (wpr == 1) __syncwarp();
         else __syncthreads();
     }
-    __device__ __forceinline__ char *at(int k) const { return buf + k * stage_bytes; }
+    __device__ __forceinline__ char *at(int k) const { return buf + k * bytes; }
     __device__ __forceinline__ void wait() {
         if (!kmb_mbar_wait(bar + stage, parity, &g_ln_error)) /* once more, for the copies under way */
             kmb_mbar_wait(bar + stage, parity, &g_ln_error);
@@ -368,20 +367,32 @@ struct Ring {
             parity ^= 1;
         }
     }
+};
+
+/* One of the row's tensors in a ring: where its rows are, which of them have
+ * pieces outside the tensor, and the row that the ring is filled with next. */
+template <typename T, int MODE>
+struct Source {
+    const T *next;
+    long step; /* elements between the walk's rows */
+    int bytes, where;
+    bool head, tail; /* the first / the last row of the tensor cannot be copied */
+    __device__ __forceinline__ Source(const void *p, long ld, const KmbLayerNorm &a, unsigned row, unsigned s, int at) {
+        next = (const T *)p + (long)row * ld;
+        step = (long)s * ld;
+        bytes = (int)(a.D * sizeof(T));
+        where = at;
+        head = p && lead(p);
+        tail = p && ((lead((const T *)p + (a.rows - 1) * ld) + bytes) & 15u);
+    }
     static __device__ __forceinline__ uint32_t lead(const void *p) {
         return MODE == kPieces ? (uint32_t)(uintptr_t)p & 15u : 0u;
     }
-    static __device__ __forceinline__ uint32_t span(const void *p, int bytes) {
-        return MODE == kPieces ? (lead(p) + (uint32_t)bytes + 15u) & ~15u : (uint32_t)bytes;
+    __device__ __forceinline__ uint32_t span() const {
+        return MODE == kPieces ? (lead(next) + (uint32_t)bytes + 15u) & ~15u : (uint32_t)bytes;
     }
-    /* whether the pieces of the row leave the tensor: its threads load it */
-    static __device__ __forceinline__ bool odd(const void *p, int bytes, const void *base, long past) {
-        if (MODE != kPieces) return false;
-        return (const char *)p - lead(p) < (const char *)base ||
-               (const char *)p - lead(p) + span(p, bytes) > (const char *)base + past;
-    }
-    __device__ __forceinline__ void copy(int k, int where, const void *p, int bytes) const {
-        kmb_bulk_load(at(k) + where, (const char *)p - lead(p), span(p, bytes), bar + k);
+    __device__ __forceinline__ void copy(const Ring<MODE> &r, int k) const {
+        kmb_bulk_load(r.at(k) + where, (const char *)next - lead(next), span(), r.bar + k);
     }
 };
 
@@ -402,39 +413,47 @@ __global__ void __launch_bounds__(KEEP ? 512 : 1024) k_ln_fwd(const __grid_const
         c.vector(a.weight, 1.f, w);
         c.vector(a.bias, 0.f, b);
     }
-    const long step = walk.step();
-    const int bytes = (int)(a.D * sizeof(TX));
-    const auto at = [&](long row) { return (const TX *)a.x + row * a.ld_x; };
-    const long past = ((a.rows - 1) * a.ld_x + a.D) * (long)sizeof(TX);
-    Ring<L, MODE> ring = {};
-    const auto fill = [&](int k, long row) {
-        if (!ring.leader) return;
-        if (row >= a.rows || ring.odd(at(row), bytes, a.x, past)) {
-            kmb_mbar_arrive(ring.bar + k);
-        } else {
-            kmb_mbar_expect(ring.bar + k, ring.span(at(row), bytes));
-            ring.copy(k, 0, at(row), bytes);
+    const unsigned step = walk.step(), rows = (unsigned)a.rows;
+    const float inv = 1.f / (float)a.D;
+    Ring<MODE> ring = {};
+    Source<TX, MODE> src(a.x, a.ld_x, a, walk.first(), step, 0);
+    unsigned ahead = walk.first(); /* the row that the ring is filled with next */
+    const auto odd = [&](unsigned row) { return (src.head && row == 0) || (src.tail && row == rows - 1); };
+    const auto fill = [&](int k) {
+        if (ring.leader) {
+            if (ahead >= rows || odd(ahead)) {
+                kmb_mbar_arrive(ring.bar + k);
+            } else {
+                kmb_mbar_expect(ring.bar + k, src.span());
+                src.copy(ring, k);
+            }
         }
+        ahead += step;
+        src.next += src.step;
     };
     if (RING) {
-        ring.start(smem, ring_slot(bytes, MODE), stages, wpr);
-        for (int k = 0; k < stages - 1; ++k) fill(k, walk.first() + k * step);
+        ring.start(smem, ring_slot(src.bytes, MODE), stages, wpr);
+        for (int k = 0; k < stages - 1; ++k) fill(k);
     }
+    const TX *px = (const TX *)a.x + (long)walk.first() * a.ld_x;
+    TY *py = (TY *)a.y + (long)walk.first() * a.ld_y;
+    const long sx = (long)step * a.ld_x, sy = (long)step * a.ld_y;
     Vec<TX, V> raw[C::NV] = {};
-    if (AHEAD && walk.first() < a.rows) c.template fetch<false>(at(walk.first()), raw);
+    if (AHEAD && walk.first() < rows) c.template fetch<false>(px, raw);
     /* with several rows a warp all of its lanes walk as long as one of them */
-    for (long r = walk.first(); L < 32 ? r - walk.group % (32 / L) < a.rows : r < a.rows; r += step) {
-        const bool live = L == 32 || r < a.rows;
+    const unsigned base = L < 32 ? walk.group % (32 / L) : 0;
+    for (unsigned r = walk.first(); r - base < rows; r += step, px += sx, py += sy) {
+        const bool live = L == 32 || r < rows;
         float2 x[EPT / 2];
         if (AHEAD) {
             C::unpack(raw, x);
-            if (r + step < a.rows) c.template fetch<false>(at(r + step), raw);
+            if (r + step < rows) c.template fetch<false>(px + sx, raw);
         } else {
             if (RING) ring.wait();
-            if (RING && !ring.odd(at(r), bytes, a.x, past))
-                c.template load<true>((const TX *)(ring.at(ring.stage) + ring.lead(at(r))), x);
+            if (RING && !odd(r))
+                c.template load<true>((const TX *)(ring.at(ring.stage) + src.lead(px)), x);
             else
-                c.template load<false>(at(r), x);
+                c.template load<false>(px, x);
         }
         float mean, rstd;
         bool filled = !RING;
@@ -444,12 +463,12 @@ __global__ void __launch_bounds__(KEEP ? 512 : 1024) k_ln_fwd(const __grid_const
                 const float v = red.one(c.sum(x, f));
                 if (!filled) { /* every thread is done with the row before */
                     if (wpr == 1) __syncwarp();
-                    fill(ring.before(), r + (stages - 1) * step);
+                    fill(ring.before());
                     filled = true;
                 }
                 return v;
             },
-            (float)a.D, a.eps, mean, rstd);
+            inv, a.eps, mean, rstd);
         if (RING) ring.next();
         if (!live) continue;
         const float2 m = kmb_f2s(-mean), s = kmb_f2s(rstd);
@@ -466,7 +485,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 1024) k_ln_fwd(const __grid_const
                 x[e] = kmb_fma2(kmb_mul2(kmb_add2(x[e], m), s), wv, bv);
             }
         }
-        c.store((TY *)a.y + r * a.ld_y, x);
+        c.store(py, x);
         if (walk.t == 0) {
             if (a.mean) a.mean[r] = mean;
             if (a.rstd) a.rstd[r] = rstd;
@@ -479,6 +498,7 @@ template <typename TX, typename TY>
 __global__ void __launch_bounds__(kLoop) k_ln_fwd_loop(const __grid_constant__ KmbLayerNorm a) {
     __shared__ float2 slot[2][32];
     Reducer<32> red(slot, kLoop / 32);
+    const float inv = 1.f / (float)a.D;
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const TX *x = (const TX *)a.x + r * a.ld_x;
         TY *y = (TY *)a.y + r * a.ld_y;
@@ -490,7 +510,7 @@ __global__ void __launch_bounds__(kLoop) k_ln_fwd_loop(const __grid_constant__ K
                 for (long j = threadIdx.x; j < a.D; j += kLoop) s += f(kmb_f2s(ld(x + j))).x;
                 return red.one(s);
             },
-            (float)a.D, a.eps, mean, rstd);
+            inv, a.eps, mean, rstd);
         for (long j = threadIdx.x; j < a.D; j += kLoop)
             st(y + j, fmaf((ld(x + j) - mean) * rstd, a.weight ? a.weight[j] : 1.f, a.bias ? a.bias[j] : 0.f));
         if (threadIdx.x == 0) {
@@ -519,44 +539,49 @@ __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayer
     c.vector(a.weight, 1.f, w);
 #pragma unroll
     for (int e = 0; e < EPT / 2; ++e) pw[e] = pb[e] = kmb_f2s(0.f);
-    const long step = walk.step();
-    const int xb = (int)(a.D * sizeof(TX)), yb = (int)(a.D * sizeof(TY));
-    const int xs = ring_slot(xb, MODE), ys = ring_slot(yb, MODE); /* places of x | dy | dres in a row's slot */
-    const auto x_at = [&](long row) { return (const TX *)a.x + row * a.ld_x; };
-    const auto d_at = [&](long row) { return (const TY *)a.dy + row * a.ld_dy; };
-    const auto r_at = [&](long row) { return (const TX *)a.dres + row * a.ld_dres; };
-    Ring<L, MODE> ring = {};
-    const long x_past = ((a.rows - 1) * a.ld_x + a.D) * (long)sizeof(TX);
-    const long d_past = ((a.rows - 1) * a.ld_dy + a.D) * (long)sizeof(TY);
-    const long r_past = ((a.rows - 1) * a.ld_dres + a.D) * (long)sizeof(TX);
-    const auto odd = [&](long row) {
-        return ring.odd(x_at(row), xb, a.x, x_past) || ring.odd(d_at(row), yb, a.dy, d_past) ||
-               (a.dres && ring.odd(r_at(row), xb, a.dres, r_past));
-    };
-    const auto fill = [&](int k, long row) {
-        if (!ring.leader) return;
-        if (row >= a.rows || odd(row)) {
-            kmb_mbar_arrive(ring.bar + k);
-            return;
+    const unsigned step = walk.step(), rows = (unsigned)a.rows;
+    Ring<MODE> ring = {};
+    const int xs = ring_slot(a.D * sizeof(TX), MODE), ys = ring_slot(a.D * sizeof(TY), MODE);
+    Source<TX, MODE> x_src(a.x, a.ld_x, a, walk.first(), step, 0);
+    Source<TY, MODE> d_src(a.dy, a.ld_dy, a, walk.first(), step, xs);
+    Source<TX, MODE> r_src(a.dres, a.ld_dres, a, walk.first(), step, xs + ys);
+    const bool head = x_src.head || d_src.head || r_src.head, tail = x_src.tail || d_src.tail || r_src.tail;
+    unsigned ahead = walk.first(); /* the row that the ring is filled with next */
+    const auto odd = [&](unsigned row) { return (head && row == 0) || (tail && row == rows - 1); };
+    const auto fill = [&](int k) {
+        if (ring.leader) {
+            if (ahead >= rows || odd(ahead)) {
+                kmb_mbar_arrive(ring.bar + k);
+            } else {
+                kmb_mbar_expect(ring.bar + k, x_src.span() + d_src.span() + (a.dres ? r_src.span() : 0u));
+                x_src.copy(ring, k);
+                d_src.copy(ring, k);
+                if (a.dres) r_src.copy(ring, k);
+            }
         }
-        kmb_mbar_expect(ring.bar + k, ring.span(x_at(row), xb) + ring.span(d_at(row), yb) +
-                                          (a.dres ? ring.span(r_at(row), xb) : 0u));
-        ring.copy(k, 0, x_at(row), xb);
-        ring.copy(k, xs, d_at(row), yb);
-        if (a.dres) ring.copy(k, xs + ys, r_at(row), xb);
+        ahead += step;
+        x_src.next += x_src.step;
+        d_src.next += d_src.step;
+        r_src.next += r_src.step;
     };
     if (RING) {
         ring.start(smem, xs + ys + (a.dres ? xs : 0), stages, wpr);
-        for (int k = 0; k < stages - 1; ++k) fill(k, walk.first() + k * step);
+        for (int k = 0; k < stages - 1; ++k) fill(k);
     }
+    const TX *px = (const TX *)a.x + (long)walk.first() * a.ld_x;
+    const TY *pd = (const TY *)a.dy + (long)walk.first() * a.ld_dy;
+    const TX *pr = (const TX *)a.dres + (long)walk.first() * a.ld_dres;
+    TX *po = (TX *)a.dx + (long)walk.first() * a.ld_dx;
     Vec<TX, V> rx[C::NV] = {};
     Vec<TY, V> rd[C::NV] = {};
-    if (AHEAD && walk.first() < a.rows) {
-        c.template fetch<false>(x_at(walk.first()), rx);
-        c.template fetch<false>(d_at(walk.first()), rd);
+    if (AHEAD && walk.first() < rows) {
+        c.template fetch<false>(px, rx);
+        c.template fetch<false>(pd, rd);
     }
-    for (long r = walk.first(); L < 32 ? r - walk.group % (32 / L) < a.rows : r < a.rows; r += step) {
-        const bool live = L == 32 || r < a.rows;
+    const unsigned base = L < 32 ? walk.group % (32 / L) : 0;
+    for (unsigned r = walk.first(); r - base < rows; r += step, px += x_src.step, pd += d_src.step,
+                  pr += r_src.step, po += (long)step * a.ld_dx) {
+        const bool live = L == 32 || r < rows;
         const bool here = RING && !odd(r); /* the row is in the ring */
         float2 h[EPT / 2], d[EPT / 2];
         float m = 0.f, s = 0.f;
@@ -568,21 +593,21 @@ __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayer
         if (AHEAD) {
             C::unpack(rx, h);
             C::unpack(rd, d);
-            if (r + step < a.rows) {
-                c.template fetch<false>(x_at(r + step), rx);
-                c.template fetch<false>(d_at(r + step), rd);
+            if (r + step < rows) {
+                c.template fetch<false>(px + x_src.step, rx);
+                c.template fetch<false>(pd + d_src.step, rd);
             } else { /* a lane without a row adds nothing to the columns' sums */
 #pragma unroll
                 for (int k = 0; k < C::NV; ++k) rd[k] = Vec<TY, V>{};
             }
         } else if (here) {
-            c.template load<true>((const TX *)(ring.at(ring.stage) + ring.lead(x_at(r))), h);
-            c.template load<true>((const TY *)(ring.at(ring.stage) + xs + ring.lead(d_at(r))), d);
+            c.template load<true>((const TX *)(ring.at(ring.stage) + x_src.lead(px)), h);
+            c.template load<true>((const TY *)(ring.at(ring.stage) + xs + d_src.lead(pd)), d);
         } else {
-            c.template load<false>(x_at(r), h);
-            c.template load<false>(d_at(r), d);
+            c.template load<false>(px, h);
+            c.template load<false>(pd, d);
         }
-        if (!a.mean) row_stats(red, [&](auto f) { return red.one(c.sum(h, f)); }, (float)a.D, a.eps, m, s);
+        if (!a.mean) row_stats(red, [&](auto f) { return red.one(c.sum(h, f)); }, inv, a.eps, m, s);
         float2 t1 = kmb_f2s(0.f), t2 = t1;
         const float2 m2 = kmb_f2s(-m), sd = kmb_f2s(s);
 #pragma unroll
@@ -597,21 +622,21 @@ __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayer
         const float2 t = red.two(t1.x + t1.y, t2.x + t2.y);
         if (RING) { /* every thread is done with the row before */
             if (wpr == 1) __syncwarp();
-            fill(ring.before(), r + (stages - 1) * step);
+            fill(ring.before());
         }
         const float2 s1 = kmb_f2s(-t.x * inv), s2 = kmb_f2s(-t.y * inv);
 #pragma unroll
         for (int e = 0; e < EPT / 2; ++e) d[e] = kmb_mul2(kmb_fma2(h[e], s2, kmb_add2(d[e], s1)), sd);
         if (a.dres && live) {
             if (here)
-                c.template load<true>((const TX *)(ring.at(ring.stage) + xs + ys + ring.lead(r_at(r))), h);
+                c.template load<true>((const TX *)(ring.at(ring.stage) + xs + ys + r_src.lead(pr)), h);
             else
-                c.template load<false>(r_at(r), h);
+                c.template load<false>(pr, h);
 #pragma unroll
             for (int e = 0; e < EPT / 2; ++e) d[e] = kmb_add2(d[e], h[e]);
         }
         if (RING) ring.next();
-        if (live) c.store((TX *)a.dx + r * a.ld_dx, d);
+        if (live) c.store(po, d);
     }
     if (!sums) return;
     float *part = (float *)a.workspace + (long)blockIdx.x * 2 * a.D;
@@ -635,20 +660,38 @@ __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayer
     }
 }
 
-/* wider rows: read a second time for dx, from L2; the column sums in
- * shared memory, or beyond its size in the CTA's row of the workspace, each
- * column one thread's */
-template <typename TX, typename TY>
-__global__ void __launch_bounds__(kLoop) k_ln_bwd_loop(const __grid_constant__ KmbLayerNorm a, int sums,
-                                                       int in_shared) {
-    extern __shared__ float cols[];
+/* Wider rows: a kernel for the columns' sums (first, since dx may be x or
+ * dy), before it one for the statistics when the caller has none, and one
+ * for dx, which reads the row a second time, from L2. */
+template <typename TX>
+__global__ void __launch_bounds__(kLoop) k_ln_stats_loop(const __grid_constant__ KmbLayerNorm a, float *mean,
+                                                         float *rstd) {
     __shared__ float2 slot[2][32];
     Reducer<32> red(slot, kLoop / 32);
-    float *part = (float *)a.workspace + (long)blockIdx.x * 2 * a.D;
-    float *pw = in_shared ? cols : part, *pb = pw + a.D;
-    if (sums)
-        for (long j = threadIdx.x; j < a.D; j += kLoop) pw[j] = pb[j] = 0.f;
+    for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const TX *x = (const TX *)a.x + r * a.ld_x;
+        float m, s;
+        row_stats(
+            red,
+            [&](auto f) {
+                float t = 0.f;
+                for (int j = threadIdx.x; j < (int)a.D; j += kLoop) t += f(kmb_f2s(ld(x + j))).x;
+                return red.one(t);
+            },
+            1.f / (float)a.D, a.eps, m, s);
+        if (threadIdx.x == 0) {
+            mean[r] = m;
+            rstd[r] = s;
+        }
+    }
+}
+
+template <typename TX, typename TY, int V>
+__global__ void __launch_bounds__(kLoop) k_ln_dx_loop(const __grid_constant__ KmbLayerNorm a) {
+    __shared__ float2 slot[2][32];
+    Reducer<32> red(slot, kLoop / 32);
     const float inv = 1.f / (float)a.D;
+    const int D = (int)a.D;
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const TX *x = (const TX *)a.x + r * a.ld_x;
         const TY *dy = (const TY *)a.dy + r * a.ld_dy;
@@ -663,34 +706,88 @@ __global__ void __launch_bounds__(kLoop) k_ln_bwd_loop(const __grid_constant__ K
                 red,
                 [&](auto f) {
                     float s = 0.f;
-                    for (long j = threadIdx.x; j < a.D; j += kLoop) s += f(kmb_f2s(ld(x + j))).x;
+                    for (int j = threadIdx.x; j < D; j += kLoop) s += f(kmb_f2s(ld(x + j))).x;
                     return red.one(s);
                 },
-                (float)a.D, a.eps, mean, rstd);
+                inv, a.eps, mean, rstd);
         }
         float s1 = 0.f, s2 = 0.f;
-        for (long j = threadIdx.x; j < a.D; j += kLoop) {
-            const float h = (ld(x + j) - mean) * rstd, v = ld(dy + j);
-            const float g = a.weight ? v * a.weight[j] : v;
-            s1 += g;
-            s2 = fmaf(g, h, s2);
-            if (sums) {
-                pw[j] = fmaf(v, h, pw[j]);
-                pb[j] += v;
+        /* f(column, x, g) over the thread's values, four vectors under way */
+        const auto each = [&](auto f) {
+#pragma unroll 4
+            for (int j = threadIdx.x * V; j < D; j += kLoop * V) {
+                Vec<TX, V> vx;
+                Vec<TY, V> vd;
+                vx.take(x + j);
+                vd.take(dy + j);
+                float h[V], d[V];
+                vx.get(h);
+                vd.get(d);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    h[e] = (h[e] - mean) * rstd;
+                    if (a.weight) d[e] *= a.weight[j + e];
+                }
+                f(j, h, d);
             }
-        }
+        };
+        each([&](int, const float *h, const float *g) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                s1 += g[e];
+                s2 = fmaf(g[e], h[e], s2);
+            }
+        });
         const float2 t = red.two(s1, s2);
         s1 = t.x * inv;
         s2 = t.y * inv;
-        for (long j = threadIdx.x; j < a.D; j += kLoop) {
-            const float h = (ld(x + j) - mean) * rstd, v = ld(dy + j);
-            const float g = a.weight ? v * a.weight[j] : v;
-            const float d = rstd * (g - s1 - h * s2);
-            st(dx + j, res ? d + ld(res + j) : d);
+        each([&](int j, const float *h, const float *g) {
+            float o[V], q[V];
+            if (res) {
+                Vec<TX, V> v;
+                v.load(res + j);
+                v.get(q);
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                o[e] = rstd * (g[e] - s1 - h[e] * s2);
+                if (res) o[e] += q[e];
+            }
+            Vec<TX, V>::store(dx + j, o);
+        });
+    }
+}
+
+/* CTA (column strip, part): the strip's sums over every gridDim.y-th row */
+constexpr int kColThreads = 128;
+
+template <typename TX, typename TY, int V>
+__global__ void __launch_bounds__(kColThreads) k_ln_cols(const __grid_constant__ KmbLayerNorm a) {
+    const long j = ((long)blockIdx.x * kColThreads + threadIdx.x) * V;
+    if (j >= a.D) return;
+    float w[V] = {}, b[V] = {};
+#pragma unroll 4
+    for (long r = blockIdx.y; r < a.rows; r += gridDim.y) {
+        Vec<TX, V> vx;
+        Vec<TY, V> vd;
+        vx.load((const TX *)a.x + r * a.ld_x + j);
+        vd.load((const TY *)a.dy + r * a.ld_dy + j);
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        float x[V], d[V];
+        vx.get(x);
+        vd.get(d);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            w[e] = fmaf(d[e], (x[e] - mean) * rstd, w[e]);
+            b[e] += d[e];
         }
     }
-    if (sums && in_shared)
-        for (long j = threadIdx.x; j < 2 * a.D; j += kLoop) part[j] = cols[j]; /* its own columns */
+    float *part = (float *)a.workspace + (long)blockIdx.y * 2 * a.D + j;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        part[e] = w[e];
+        part[a.D + e] = b[e];
+    }
 }
 
 /* dweight, dbias from the rows of partial sums: 32 columns a CTA, joined in
@@ -859,42 +956,60 @@ int bwd_v(const KmbLayerNorm *a, int sums, cudaStream_t s) {
     return run_bwd<TX, TY, V, 16, 32>(a, sums, s);
 }
 
-constexpr size_t kColsShared = 200 * 1024; /* of the 227 KB an SM can give a CTA */
+/* Parts of the columns' kernel: some eight CTAs an SM over its strips. */
+long col_parts(long rows, long D) {
+    const long strips = (D / 8 + kColThreads - 1) / kColThreads; /* vectors of 8 */
+    long n = 8L * kSMs / strips;
+    if (n > rows / 4) n = rows / 4;
+    return n > 1 ? n : 1;
+}
+
+long sum_parts(long rows, long D) {
+    return D <= kBwdMax ? ctas(rows, D, warps_of(D, bwd_ept(D))) : col_parts(rows, D);
+}
+
+template <typename TX, typename TY, int V>
+int bwd_wide(const KmbLayerNorm *a, int sums, cudaStream_t s) {
+    KmbLayerNorm d = *a;
+    const long parts = col_parts(a->rows, a->D);
+    const unsigned n = (unsigned)(a->rows < 3 * kSMs ? a->rows : 3 * kSMs);
+    if (sums) {
+        if (!d.mean) {
+            d.mean = (float *)a->workspace + parts * 2 * a->D;
+            d.rstd = d.mean + a->rows;
+            k_ln_stats_loop<TX><<<n, kLoop, 0, s>>>(*a, d.mean, d.rstd);
+        }
+        const dim3 grid((unsigned)((a->D / V + kColThreads - 1) / kColThreads), (unsigned)parts);
+        k_ln_cols<TX, TY, V><<<grid, kColThreads, 0, s>>>(d);
+    }
+    k_ln_dx_loop<TX, TY, V><<<n, kLoop, 0, s>>>(d);
+    return done();
+}
 
 template <typename TX, typename TY>
 int bwd(const KmbLayerNorm *a, cudaStream_t s) {
     constexpr int V = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;
     const int sums = a->dweight || a->dbias;
-    const long parts = kmb_layernorm_parts(a->rows, a->D);
+    const long parts = sum_parts(a->rows, a->D);
     const bool vec = a->D % V == 0 && aligned(a->x, a->ld_x, sizeof(TX), V) &&
                      aligned(a->dy, a->ld_dy, sizeof(TY), V) && aligned(a->dx, a->ld_dx, sizeof(TX), V) &&
                      aligned(a->dres, a->ld_dres, sizeof(TX), V);
-    if (a->rows && a->D <= kBwdMax) {
-        const int rc = vec ? bwd_v<TX, TY, V>(a, sums, s) : bwd_v<TX, TY, 1>(a, sums, s);
-        if (rc) return rc;
-    } else if (a->rows) {
-        const size_t bytes = 8 * (size_t)a->D;
-        const int shared = sums && bytes <= kColsShared;
-        if (shared) {
-            const cudaError_t e = cudaFuncSetAttribute(k_ln_bwd_loop<TX, TY>,
-                                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                       (int)kColsShared);
-            if (e != cudaSuccess) return kmb_cuda_fail(e, "layernorm: shared memory");
-        }
-        k_ln_bwd_loop<TX, TY><<<(unsigned)parts, kLoop, shared ? bytes : 0, s>>>(*a, sums, shared);
-    }
-    if (sums)
-        k_ln_sums<<<(unsigned)((2 * a->D + 31) / 32), dim3(32, parts > 256 ? 32 : 8), 0, s>>>(
-            (const float *)a->workspace, a->rows ? parts : 0, a->D, a->dweight, a->dbias, a->accumulate);
+    int rc = KMB_OK;
+    if (a->rows && a->D <= kBwdMax)
+        rc = vec ? bwd_v<TX, TY, V>(a, sums, s) : bwd_v<TX, TY, 1>(a, sums, s);
+    else if (a->rows)
+        rc = vec ? bwd_wide<TX, TY, V>(a, sums, s) : bwd_wide<TX, TY, 1>(a, sums, s);
+    if (rc || !sums) return rc;
+    k_ln_sums<<<(unsigned)((2 * a->D + 31) / 32), dim3(32, parts > 256 || a->D <= 2048 ? 32 : 8), 0, s>>>(
+        (const float *)a->workspace, a->rows ? parts : 0, a->D, a->dweight, a->dbias, a->accumulate);
     return done();
 }
 
 } // namespace
 
-extern "C" long kmb_layernorm_parts(long rows, long D) {
-    if (D <= kBwdMax) return ctas(rows, D, warps_of(D, bwd_ept(D)));
-    const long most = 8 * D <= (long)kColsShared ? kSMs : 4 * kSMs;
-    return rows < most ? (rows > 0 ? rows : 1) : most;
+/* partial sums, and behind them the statistics of wide rows */
+extern "C" size_t kmb_layernorm_scratch_bytes(long rows, long D) {
+    return 8 * (size_t)sum_parts(rows, D) * (size_t)D + (D > kBwdMax ? 8 * (size_t)rows : 0);
 }
 
 extern "C" int kmb_launch_layernorm_fwd(const KmbLayerNorm *a, cudaStream_t s) {

@@ -13,8 +13,8 @@ static int known(int type) { return type == KMB_F32 || type == KMB_BF16; }
 static int misaligned(const void *p, size_t n) { return p && ((uintptr_t)p & (n - 1)) != 0; }
 
 size_t kmb_layernorm_workspace_bytes(const KmbLayerNorm *a) {
-    if (!a || a->rows < 0 || a->D <= 0 || a->D >= (1L << 31)) return 0;
-    return (size_t)kmb_layernorm_parts(a->rows, a->D) * 2 * (size_t)a->D * sizeof(float);
+    if (!a || a->rows < 0 || a->D <= 0 || a->rows >= (1L << 31) || a->D >= (1L << 31)) return 0;
+    return kmb_layernorm_scratch_bytes(a->rows, a->D);
 }
 
 static int validate(const KmbLayerNorm *a, int bwd) {

@@ -101,11 +101,10 @@ int kmb_scan2d_check_error(void);
 int kmb_launch_gemm_bf16(const KmbGemm *g, cudaStream_t s);
 
 /* Layer norm (csrc/cuda/layernorm.cu); arguments already validated, the
- * workspace in place.  The backward's partial sums take
- * kmb_layernorm_parts(rows, D) rows of 2 D floats. */
+ * workspace in place. */
 int kmb_launch_layernorm_fwd(const KmbLayerNorm *a, cudaStream_t s);
 int kmb_launch_layernorm_bwd(const KmbLayerNorm *a, cudaStream_t s);
-long kmb_layernorm_parts(long rows, long D);
+size_t kmb_layernorm_scratch_bytes(long rows, long D);
 
 /* Gated linear recurrence (csrc/cuda/glr.cu); arguments already validated,
  * the workspace in place. */
