@@ -388,7 +388,7 @@ size_t kmb_layernorm_workspace_bytes(const KmbLayerNorm *args);
  * dh_last.
  *
  * ckpt (optional output of the forward, kmb_glr_ckpt_elems() floats): the
- * state before each KMB_GLR_CHUNK-th row.  The backward reads the ckpt of
+ * state before each KMB_GLR_CHUNK(type)-th row.  The backward reads the ckpt of
  * the same arguments, or with NULL runs the states again into its
  * workspace.
  *
@@ -404,7 +404,7 @@ size_t kmb_layernorm_workspace_bytes(const KmbLayerNorm *args);
  * workspace: kmb_glr_workspace_bytes(args, bwd) bytes of device memory,
  * 16-byte aligned; the rules of KmbLayerNorm's workspace hold.
  */
-#define KMB_GLR_CHUNK 64
+#define KMB_GLR_CHUNK(type) ((type) == KMB_BF16 ? 56 : 28)
 
 typedef struct {
     void *data;
@@ -440,7 +440,7 @@ typedef struct {
     int pad_;
 } KmbGLR;
 
-/* Sizes read batch, L, D and whether offsets is NULL (workspace: also
+/* Sizes read batch, L, D, type and whether offsets is NULL (workspace: also
  * whether ckpt and ddecay are); 0 when the sizes are invalid. */
 long kmb_glr_ckpt_elems(const KmbGLR *args);
 size_t kmb_glr_workspace_bytes(const KmbGLR *args, int bwd);

@@ -13,7 +13,7 @@
  * kappa b, so nothing divides by a vanishing root: kappa -> 1/2 at u = 0.)
  *
  * Both directions are one pass over the data.  A CTA takes a tile of rows x
- * 128 channels: a warp owns a run of consecutive rows, a lane four channels.
+ * channels: a warp owns a run of consecutive rows, a lane 2 or 4 channels.
  * A run is first reduced to its affine map h -> A h + H, the maps of a
  * tile's warps are joined through shared memory, and the maps of the tiles
  * of one channel group through global memory: a tile publishes its map,
@@ -24,105 +24,152 @@
  * to the final state of the one before it, whichever of the two was read,
  * so results do not depend on timing.
  */
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "kmb_common.cuh"
+#include "kmb_tma.cuh"
 #include "../kmb_internal.h"
 
 namespace {
 
-constexpr int kChunk = KMB_GLR_CHUNK;
-constexpr int kV = 4;       /* channels of a lane */
-constexpr int kC = 32 * kV; /* channels of a tile */
 constexpr int kWindow = 12; /* tiles before its own that a tile looks at */
 constexpr unsigned kUnset = 0xffffffffu; /* workspace word not written yet */
 
-/* set when a wait for another tile's state gave up (kmb_glr_check_error) */
+/* set when a wait gave up (kmb_glr_check_error) */
 __device__ int g_glr_error;
 
 /* ------------------------------------------------------------------ */
-/* four channels of one row, as two FFMA2 pairs                          */
+/* V channels of one row, as FFMA2 pairs                                */
 /* ------------------------------------------------------------------ */
 
-struct F4 {
-    float2 l, h;
+template <int V>
+struct Pack;
+template <>
+struct Pack<2> {
+    typedef float2 type;
 };
-__device__ __forceinline__ F4 f4s(float v) { return {kmb_f2s(v), kmb_f2s(v)}; }
-__device__ __forceinline__ F4 f4(float4 v) { return {kmb_f2(v.x, v.y), kmb_f2(v.z, v.w)}; }
-__device__ __forceinline__ float4 v4(F4 a) { return make_float4(a.l.x, a.l.y, a.h.x, a.h.y); }
-__device__ __forceinline__ F4 operator+(F4 a, F4 b) { return {kmb_add2(a.l, b.l), kmb_add2(a.h, b.h)}; }
-__device__ __forceinline__ F4 operator*(F4 a, F4 b) { return {kmb_mul2(a.l, b.l), kmb_mul2(a.h, b.h)}; }
-__device__ __forceinline__ F4 fma4(F4 a, F4 b, F4 c) {
-    return {kmb_fma2(a.l, b.l, c.l), kmb_fma2(a.h, b.h, c.h)};
+template <>
+struct Pack<4> {
+    typedef float4 type;
+};
+
+template <int V>
+struct F {
+    float2 p[V / 2];
+    __device__ __forceinline__ float operator[](int k) const { return k % 2 ? p[k / 2].y : p[k / 2].x; }
+};
+template <int V>
+__device__ __forceinline__ F<V> all(float v) {
+    F<V> r;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.p[i] = kmb_f2s(v);
+    return r;
 }
-template <typename Fn>
-__device__ __forceinline__ F4 each(Fn f) { /* f(channel) */
-    return {kmb_f2(f(0), f(1)), kmb_f2(f(2), f(3))};
+__device__ __forceinline__ F<2> from(float2 v) { return {{v}}; }
+__device__ __forceinline__ F<4> from(float4 v) { return {{kmb_f2(v.x, v.y), kmb_f2(v.z, v.w)}}; }
+__device__ __forceinline__ float2 to(F<2> a) { return a.p[0]; }
+__device__ __forceinline__ float4 to(F<4> a) { return make_float4(a.p[0].x, a.p[0].y, a.p[1].x, a.p[1].y); }
+template <int V>
+__device__ __forceinline__ F<V> operator+(F<V> a, F<V> b) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) a.p[i] = kmb_add2(a.p[i], b.p[i]);
+    return a;
 }
-__device__ __forceinline__ float get(const F4 &a, int k) {
-    return k == 0 ? a.l.x : k == 1 ? a.l.y : k == 2 ? a.h.x : a.h.y;
+template <int V>
+__device__ __forceinline__ F<V> operator*(F<V> a, F<V> b) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) a.p[i] = kmb_mul2(a.p[i], b.p[i]);
+    return a;
+}
+template <int V>
+__device__ __forceinline__ F<V> fma(F<V> a, F<V> b, F<V> c) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) c.p[i] = kmb_fma2(a.p[i], b.p[i], c.p[i]);
+    return c;
+}
+template <int V, typename Fn>
+__device__ __forceinline__ F<V> each(Fn f) { /* f(channel) */
+    F<V> r;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.p[i] = kmb_f2(f(2 * i), f(2 * i + 1));
+    return r;
 }
 
-/* VEC: channels 4 lane .. 4 lane + 3 in one access; else lane + 32 k, for
- * odd widths, strides and addresses (every access still covers a contiguous
- * piece of the row).  m: bit k set where channel k exists. */
-template <typename T>
+__device__ __forceinline__ unsigned pack(float2 v) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+    return *reinterpret_cast<const unsigned *>(&h);
+}
+__device__ __forceinline__ float2 unpack(unsigned v) {
+    return kmb_f2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+/* V channels as stored: of bf16, two in a word, the first in the low half. */
+template <typename T, int V>
 struct Raw;
-template <>
-struct Raw<float> {
-    typedef float4 type;
-    static __device__ __forceinline__ F4 f(float4 v) { return f4(v); }
-    template <bool VEC>
-    static __device__ __forceinline__ float4 load(const float *p, unsigned m) {
-        if (VEC) return m ? __ldcs(reinterpret_cast<const float4 *>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        return make_float4(m & 1 ? __ldcs(p) : 0.f, m & 2 ? __ldcs(p + 32) : 0.f,
-                           m & 4 ? __ldcs(p + 64) : 0.f, m & 8 ? __ldcs(p + 96) : 0.f);
-    }
-    template <bool VEC>
-    static __device__ __forceinline__ void store(float *p, F4 v, unsigned m) {
-        if (VEC) {
-            if (m) __stcs(reinterpret_cast<float4 *>(p), v4(v));
-            return;
-        }
-        if (m & 1) __stcs(p, v.l.x);
-        if (m & 2) __stcs(p + 32, v.l.y);
-        if (m & 4) __stcs(p + 64, v.h.x);
-        if (m & 8) __stcs(p + 96, v.h.y);
-    }
+template <int V>
+struct Raw<float, V> {
+    typedef typename Pack<V>::type type;
+    static __device__ __forceinline__ F<V> f(type v) { return from(v); }
+    static __device__ __forceinline__ type r(F<V> v) { return to(v); }
 };
 template <>
-struct Raw<__nv_bfloat16> {
-    typedef uint2 type; /* the even channels in the low halves */
-    static __device__ __forceinline__ F4 f(uint2 v) {
-        return {kmb_f2(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u)),
-                kmb_f2(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u))};
-    }
-    static __device__ __forceinline__ unsigned pack(float2 v) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
-        return *reinterpret_cast<const unsigned *>(&h);
-    }
-    template <bool VEC>
-    static __device__ __forceinline__ uint2 load(const __nv_bfloat16 *p, unsigned m) {
-        if (VEC) return m ? __ldcs(reinterpret_cast<const uint2 *>(p)) : make_uint2(0u, 0u);
-        const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
-        const unsigned a = m & 1 ? __ldcs(q) : 0u, b = m & 2 ? __ldcs(q + 32) : 0u;
-        const unsigned c = m & 4 ? __ldcs(q + 64) : 0u, d = m & 8 ? __ldcs(q + 96) : 0u;
-        return make_uint2(a | b << 16, c | d << 16);
-    }
-    template <bool VEC>
-    static __device__ __forceinline__ void store(__nv_bfloat16 *p, F4 v, unsigned m) {
-        const uint2 u = make_uint2(pack(v.l), pack(v.h));
-        if (VEC) {
-            if (m) __stcs(reinterpret_cast<uint2 *>(p), u);
-            return;
-        }
-        unsigned short *q = reinterpret_cast<unsigned short *>(p);
-        if (m & 1) __stcs(q, (unsigned short)u.x);
-        if (m & 2) __stcs(q + 32, (unsigned short)(u.x >> 16));
-        if (m & 4) __stcs(q + 64, (unsigned short)u.y);
-        if (m & 8) __stcs(q + 96, (unsigned short)(u.y >> 16));
-    }
+struct Raw<__nv_bfloat16, 4> {
+    typedef uint2 type;
+    static __device__ __forceinline__ F<4> f(uint2 v) { return {{unpack(v.x), unpack(v.y)}}; }
+    static __device__ __forceinline__ uint2 r(F<4> v) { return make_uint2(pack(v.p[0]), pack(v.p[1])); }
 };
+template <>
+struct Raw<__nv_bfloat16, 2> {
+    typedef unsigned type;
+    static __device__ __forceinline__ F<2> f(unsigned v) { return {{unpack(v)}}; }
+    static __device__ __forceinline__ unsigned r(F<2> v) { return pack(v.p[0]); }
+};
+
+/* A lane's four channels in global memory.  VEC: 4 lane .. 4 lane + 3 in one
+ * access; else lane + 32 k, for odd widths, strides and addresses (every
+ * access still covers a contiguous piece of the row).  m: bit k set where
+ * channel k exists. */
+constexpr int kV = 4;
+constexpr int kC = 32 * kV;
+
+template <bool VEC>
+__device__ __forceinline__ float4 load(const float *p, unsigned m) {
+    if (VEC) return m ? __ldcs(reinterpret_cast<const float4 *>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    return make_float4(m & 1 ? __ldcs(p) : 0.f, m & 2 ? __ldcs(p + 32) : 0.f, m & 4 ? __ldcs(p + 64) : 0.f,
+                       m & 8 ? __ldcs(p + 96) : 0.f);
+}
+template <bool VEC>
+__device__ __forceinline__ uint2 load(const __nv_bfloat16 *p, unsigned m) {
+    if (VEC) return m ? __ldcs(reinterpret_cast<const uint2 *>(p)) : make_uint2(0u, 0u);
+    const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
+    const unsigned a = m & 1 ? __ldcs(q) : 0u, b = m & 2 ? __ldcs(q + 32) : 0u;
+    const unsigned c = m & 4 ? __ldcs(q + 64) : 0u, d = m & 8 ? __ldcs(q + 96) : 0u;
+    return make_uint2(a | b << 16, c | d << 16);
+}
+template <bool VEC>
+__device__ __forceinline__ void store(float *p, F<4> v, unsigned m) {
+    if constexpr (VEC) {
+        if (m) __stcs(reinterpret_cast<float4 *>(p), to(v));
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (m >> k & 1) __stcs(p + 32 * k, v[k]);
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void store(__nv_bfloat16 *p, F<4> v, unsigned m) {
+    const uint2 u = Raw<__nv_bfloat16, 4>::r(v);
+    if (VEC) {
+        if (m) __stcs(reinterpret_cast<uint2 *>(p), u);
+        return;
+    }
+    unsigned short *q = reinterpret_cast<unsigned short *>(p);
+    if (m & 1) __stcs(q, (unsigned short)u.x);
+    if (m & 2) __stcs(q + 32, (unsigned short)(u.x >> 16));
+    if (m & 4) __stcs(q + 64, (unsigned short)u.y);
+    if (m & 8) __stcs(q + 96, (unsigned short)(u.y >> 16));
+}
 
 __device__ __forceinline__ float softplus(float v) { return v > 20.f ? v + expf(-v) : log1pf(expf(v)); }
 /* sigmoid / softplus: 1 where both vanish */
@@ -161,146 +208,191 @@ __device__ __forceinline__ float sqrt_mufu(float v) {
  */
 constexpr float kWeak = 0.25f;
 
-__device__ __forceinline__ F4 poly4(F4 u, float c0, float c1, float c2, float c3, float c4) {
-    F4 p = fma4(f4s(c4), u, f4s(c3));
-    p = fma4(p, u, f4s(c2));
-    p = fma4(p, u, f4s(c1));
-    return fma4(p, u, f4s(c0));
+template <int V>
+__device__ __forceinline__ F<V> poly4(F<V> u, float c0, float c1, float c2, float c3, float c4) {
+    F<V> p = fma(all<V>(c4), u, all<V>(c3));
+    p = fma(p, u, all<V>(c2));
+    p = fma(p, u, all<V>(c1));
+    return fma(p, u, all<V>(c0));
 }
-__device__ __forceinline__ F4 poly_expm1(F4 u) {
+template <int V>
+__device__ __forceinline__ F<V> poly_expm1(F<V> u) {
     return poly4(u, -1.f, 0.49999964237213135f, -0.1666528880596161f, 0.04150013253092766f,
                  -0.007530174218118191f);
 }
-__device__ __forceinline__ F4 poly_root(F4 u) {
+template <int V>
+__device__ __forceinline__ F<V> poly_root(F<V> u) {
     return poly4(u, 1.f, -0.49999940395355225f, 0.20831027626991272f, -0.06222091242671013f,
                  0.01236682292073965f);
 }
-__device__ __forceinline__ F4 poly_kappa(F4 u) {
+template <int V>
+__device__ __forceinline__ F<V> poly_kappa(F<V> u) {
     return poly4(u, 0.5f, -0.5000002980232239f, 0.1666753739118576f, -8.377274934900925e-05f,
                  -0.010830916464328766f);
 }
 
 /* Per channel: rate, and sqrt(2 rate) for root = sqrt(2 u) sqrt((1 - e^-2u) / 2u). */
+template <int V>
 struct Rates {
-    F4 rate, sroot;
+    F<V> rate, sroot;
 };
 
 /* Of one row: c is a - 1 (WEAK) or a, q = sqrt(r) = (1 + e^-gate_r)^-1/2, i,
  * and si = root i. */
+template <int V>
 struct Terms {
-    F4 c, q, i, si;
+    F<V> c, q, i, si;
 };
 
-template <bool WEAK>
-__device__ __forceinline__ Terms terms(F4 gr, F4 gi, const Rates &k) {
-    Terms t;
-    const F4 nl = f4s(-KMB_LOG2E), one = f4s(1.f);
+template <bool WEAK, int V>
+__device__ __forceinline__ Terms<V> terms(F<V> gr, F<V> gi, const Rates<V> &k) {
+    Terms<V> t;
+    const F<V> nl = all<V>(-KMB_LOG2E), one = all<V>(1.f);
     gr = gr * nl;
     gi = gi * nl;
-    const F4 er = each([&](int n) { return kmb_ex2(get(gr, n)); }) + one;
-    const F4 ei = each([&](int n) { return kmb_ex2(get(gi, n)); }) + one;
-    t.q = each([&](int n) { return rsqrt_mufu(get(er, n)); });
-    t.i = each([&](int n) { return rcp_mufu(get(ei, n)); });
-    const F4 u = k.rate * (t.q * t.q);
-    const F4 m = u * poly_expm1(u);
-    F4 root = k.sroot * t.q * poly_root(u);
+    const F<V> er = each<V>([&](int n) { return kmb_ex2(gr[n]); }) + one;
+    const F<V> ei = each<V>([&](int n) { return kmb_ex2(gi[n]); }) + one;
+    t.q = each<V>([&](int n) { return rsqrt_mufu(er[n]); });
+    t.i = each<V>([&](int n) { return rcp_mufu(ei[n]); });
+    const F<V> u = k.rate * (t.q * t.q);
+    const F<V> m = u * poly_expm1(u);
+    F<V> root = k.sroot * t.q * poly_root(u);
     if (WEAK) {
         t.c = m;
     } else {
-        const F4 un = u * nl;
-        const F4 e = each([&](int n) { return kmb_ex2(get(un, n)); });
-        t.c = each([&](int n) { return get(u, n) <= kWeak ? 1.f + get(m, n) : get(e, n); });
-        root = each([&](int n) {
-            return get(u, n) <= kWeak ? get(root, n) : sqrt_mufu(fmaf(-get(e, n), get(e, n), 1.f));
-        });
+        const F<V> un = u * nl;
+        const F<V> e = each<V>([&](int n) { return kmb_ex2(un[n]); });
+        t.c = each<V>([&](int n) { return u[n] <= kWeak ? 1.f + m[n] : e[n]; });
+        root = each<V>([&](int n) { return u[n] <= kWeak ? root[n] : sqrt_mufu(fmaf(-e[n], e[n], 1.f)); });
     }
     t.si = root * t.i;
     return t;
 }
 
 /* a h + b */
-template <bool WEAK>
-__device__ __forceinline__ F4 advance(F4 c, F4 h, F4 b) {
-    return WEAK ? h + fma4(c, h, b) : fma4(c, h, b);
+template <bool WEAK, int V>
+__device__ __forceinline__ F<V> advance(F<V> c, F<V> h, F<V> b) {
+    return WEAK ? h + fma(c, h, b) : fma(c, h, b);
 }
 /* a A */
-template <bool WEAK>
-__device__ __forceinline__ F4 shrink(F4 c, F4 A) {
-    return WEAK ? fma4(c, A, A) : c * A;
+template <bool WEAK, int V>
+__device__ __forceinline__ F<V> shrink(F<V> c, F<V> A) {
+    return WEAK ? fma(c, A, A) : c * A;
+}
+
+/* Gradients of one row from G, what the row's state is worth, and hp, the
+ * state before it. */
+template <int V>
+struct Grads {
+    F<V> x, r, i, udu;
+};
+
+template <bool WEAK, int V>
+__device__ __forceinline__ Grads<V> gradients(const Terms<V> &t, F<V> rate, F<V> x, F<V> G, F<V> hp) {
+    const F<V> one = all<V>(1.f), minus = all<V>(-1.f);
+    const F<V> r = t.q * t.q, u = rate * r, b = t.si * x;
+    F<V> kappa = poly_kappa(u), ua; /* ua: -u a */
+    if (WEAK) {
+        ua = fma(t.c, u, u) * minus;
+    } else {
+        /* e^-u is 0 long before u is 100 */
+        ua = each<V>([&](int n) { return u[n] > 100.f ? 0.f : -u[n] * t.c[n]; });
+        kappa = each<V>([&](int n) {
+            return u[n] <= kWeak ? kappa[n] : -ua[n] * t.c[n] * rcp_mufu(fmaf(-t.c[n], t.c[n], 1.f));
+        });
+    }
+    Grads<V> g;
+    g.udu = G * fma(ua, hp, kappa * b);
+    g.x = G * t.si;
+    g.r = g.udu * fma(r, minus, one);
+    g.i = G * b * fma(t.i, minus, one);
+    return g;
 }
 
 /* ------------------------------------------------------------------ */
 /* affine maps h -> A h + H; A = -1 marks a constant one                 */
 /* ------------------------------------------------------------------ */
 
+template <int V>
 struct Map {
-    F4 A, H;
+    F<V> A, H;
 };
 
 /* MARKED: constant maps occur (a sequence began inside, a final state) */
-template <bool MARKED>
-__device__ __forceinline__ F4 apply(const Map &m, F4 h) {
-    const F4 r = fma4(m.A, h, m.H);
+template <bool MARKED, int V>
+__device__ __forceinline__ F<V> apply(const Map<V> &m, F<V> h) {
+    const F<V> r = fma(m.A, h, m.H);
     if (!MARKED) return r;
-    return each([&](int n) { return get(m.A, n) < 0.f ? get(m.H, n) : get(r, n); });
+    return each<V>([&](int n) { return m.A[n] < 0.f ? m.H[n] : r[n]; });
 }
 
 /* the map of `first` then `then` */
-template <bool MARKED>
-__device__ __forceinline__ Map join(const Map &first, const Map &then) {
-    Map r;
+template <bool MARKED, int V>
+__device__ __forceinline__ Map<V> join(const Map<V> &first, const Map<V> &then) {
+    Map<V> r;
     r.H = apply<MARKED>(then, first.H);
     r.A = first.A * then.A;
-    if (MARKED)
-        r.A = each([&](int n) { return get(first.A, n) < 0.f || get(then.A, n) < 0.f ? -1.f : get(r.A, n); });
+    if (MARKED) r.A = each<V>([&](int n) { return first.A[n] < 0.f || then.A[n] < 0.f ? -1.f : r.A[n]; });
     return r;
 }
 
-/* What tiles show one another: [place in the chain][chain][lane] of four
+/* What tiles show one another: [place in the chain][chain][lane] of V
  * channels.  Every word is written once, and was kUnset (the workspace is
  * filled at the start of the call): a word that is not kUnset is the value
  * itself, so no fence orders flags against data. */
 struct Shown {
-    float4 *A, *H, *end; /* map, final state */
-    long step;           /* entries between places of a chain */
+    float *A, *H, *end; /* map, final state */
+    long step;          /* lanes between places of a chain */
 };
 
-__device__ __forceinline__ bool peek(const float4 *p, F4 &v) {
+__device__ __forceinline__ bool peek(const float *p, F<4> &v) {
     unsigned a, b, c, d;
     asm volatile("ld.relaxed.gpu.global.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
                  : "l"(p)
                  : "memory");
-    v = {kmb_f2(__uint_as_float(a), __uint_as_float(b)), kmb_f2(__uint_as_float(c), __uint_as_float(d))};
+    v = {{kmb_f2(__uint_as_float(a), __uint_as_float(b)), kmb_f2(__uint_as_float(c), __uint_as_float(d))}};
     return a != kUnset && b != kUnset && c != kUnset && d != kUnset;
+}
+__device__ __forceinline__ bool peek(const float *p, F<2> &v) {
+    unsigned a, b;
+    asm volatile("ld.relaxed.gpu.global.v2.u32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "l"(p) : "memory");
+    v = {{kmb_f2(__uint_as_float(a), __uint_as_float(b))}};
+    return a != kUnset && b != kUnset;
 }
 __device__ __forceinline__ float not_unset(float v) {
     return __float_as_uint(v) == kUnset ? __uint_as_float(0x7fffffffu) : v;
 }
-__device__ __forceinline__ void show(float4 *p, F4 v) {
-    asm volatile("st.relaxed.gpu.global.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(not_unset(v.l.x)),
-                 "f"(not_unset(v.l.y)), "f"(not_unset(v.h.x)), "f"(not_unset(v.h.y))
+__device__ __forceinline__ void show(float *p, F<4> v) {
+    asm volatile("st.relaxed.gpu.global.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(not_unset(v[0])),
+                 "f"(not_unset(v[1])), "f"(not_unset(v[2])), "f"(not_unset(v[3]))
+                 : "memory");
+}
+__device__ __forceinline__ void show(float *p, F<2> v) {
+    asm volatile("st.relaxed.gpu.global.v2.f32 [%0], {%1, %2};" ::"l"(p), "f"(not_unset(v[0])),
+                 "f"(not_unset(v[1]))
                  : "memory");
 }
 
 /* The map of a place, or as a constant one its final state: waits for
  * whichever comes first (last: for the final state).  Bounded by about 2^31
  * cycles; then the error word is set and later waits return at once. */
-__device__ __forceinline__ Map look(const Shown &s, long o, bool last) {
+template <int V>
+__device__ __forceinline__ Map<V> look(const Shown &s, long o, bool last) {
     const long long t0 = clock64();
-    Map m;
+    Map<V> m;
     for (int n = 0;; ++n) {
-        if (peek(s.end + o, m.H)) {
-            m.A = f4s(-1.f);
+        if (peek(s.end + o * V, m.H)) {
+            m.A = all<V>(-1.f);
             return m;
         }
-        if (!last && peek(s.A + o, m.A) && peek(s.H + o, m.H)) return m;
+        if (!last && peek(s.A + o * V, m.A) && peek(s.H + o * V, m.H)) return m;
         if ((n & 63) == 63) {
             const bool late = clock64() - t0 > (1ll << 31);
             if (late) atomicExch(&g_glr_error, 1);
             if (late || *reinterpret_cast<volatile int *>(&g_glr_error)) {
-                m.A = f4s(-1.f);
-                m.H = f4s(0.f);
+                m.A = all<V>(-1.f);
+                m.H = all<V>(0.f);
                 return m;
             }
         }
@@ -311,39 +403,35 @@ __device__ __forceinline__ Map look(const Shown &s, long o, bool last) {
 /* kernel arguments and a tile's place                                  */
 /* ------------------------------------------------------------------ */
 
+/* rows between checkpoints */
+template <typename T>
+constexpr int chunk_of = KMB_GLR_CHUNK(sizeof(T) == 2 ? KMB_BF16 : KMB_F32);
+
 struct Dev {
     KmbGLR a;
-    long tiles, groups, chains; /* tiles of a chain, channel groups, batch * groups */
-    long chunks;                /* checkpoints of a chain */
-    int states_only;            /* forward: checkpoints alone are wanted */
+    unsigned tiles, groups, chains; /* tiles of a chain, channel groups, batch * groups */
+    long chunks;                    /* checkpoints of a chain */
+    int states_only;                /* forward: checkpoints alone are wanted */
     const float *ckpt_in;
     float *ckpt_out;
-    float *part;                /* [tiles * batch][groups * kC] sums of u dL/du */
+    float *part;                    /* [tiles * chains][channels of a tile] sums of u dL/du */
     unsigned *ticket;
     Shown shown;
 };
 
 struct Place {
-    long pos, chain, b, ch0; /* place in the chain, chain, sequence (0 when packed), first channel */
+    unsigned pos, chain, b, group; /* place in the chain, chain, sequence (0 when packed), channel group */
+    __device__ __forceinline__ Place(const Dev &p, unsigned id) {
+        pos = id / p.chains;
+        chain = id - pos * p.chains;
+        b = chain / p.groups;
+        group = chain - b * p.groups;
+    }
 };
 
 /* Tiles are taken in the order of their places: a tile waits only for tiles
- * that another CTA has taken before. */
-__device__ __forceinline__ Place place(const Dev &p, unsigned *slot) {
-    if (p.tiles > 1) {
-        if (threadIdx.x == 0) *slot = atomicAdd(p.ticket, 1u) + 1u; /* the fill makes it -1 */
-        __syncthreads();
-    }
-    const unsigned id = p.tiles > 1 ? *slot : blockIdx.x;
-    Place t;
-    const unsigned pos = id / (unsigned)p.chains, chain = id - pos * (unsigned)p.chains;
-    const unsigned b = chain / (unsigned)p.groups;
-    t.pos = pos;
-    t.chain = chain;
-    t.b = b;
-    t.ch0 = (long)(chain - b * (unsigned)p.groups) * kC;
-    return t;
-}
+ * that another CTA has taken before.  The fill makes the ticket -1. */
+__device__ __forceinline__ unsigned take_ticket(const Dev &p) { return atomicAdd(p.ticket, 1u) + 1u; }
 
 /* Packed rows: which sequence a row of the tile belongs to and whether it
  * is its first or last. */
@@ -351,6 +439,8 @@ template <int ROWS>
 struct RowMap {
     int seq[ROWS];
     unsigned char edge[ROWS]; /* 1: first row, 2: last row */
+    int whole;                /* every row of the tile that the tensors have is of a sequence */
+    int plain;                /* all rows are, and none begins or ends one */
 };
 
 /* First sequence whose end lies behind `row`: the number of ends <= row,
@@ -370,39 +460,58 @@ __device__ __forceinline__ long first_sequence(const long *off, long n, long row
     return lo;
 }
 
+/* by one warp; ends with its barrier */
 template <int ROWS>
 __device__ void map_rows(RowMap<ROWS> &m, const KmbGLR &a, long row0) {
-    for (int r = threadIdx.x; r < ROWS; r += blockDim.x) {
+    const int lane = threadIdx.x % 32;
+    for (int r = lane; r < ROWS; r += 32) {
         m.seq[r] = -1;
         m.edge[r] = 0;
     }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        const long end = row0 + ROWS < a.L ? row0 + ROWS : a.L;
-        for (long s = first_sequence(a.offsets, a.batch, row0, lane); s < a.batch; s += 32) {
-            long lo = end, hi = end;
-            if (s + lane < a.batch) {
-                lo = a.offsets[s + lane];
-                hi = a.offsets[s + lane + 1];
-            }
-            const long from = lo > row0 ? lo : row0, to = hi < end ? hi : end;
-            for (long r = from; r < to; ++r) {
-                m.seq[r - row0] = (int)(s + lane);
-                m.edge[r - row0] = (unsigned char)((r == (lo < 0 ? 0 : lo) ? 1 : 0) |
-                                                   (r == (hi > a.L ? a.L : hi) - 1 ? 2 : 0));
-            }
-            if (__any_sync(~0u, s + lane < a.batch && lo >= end)) break;
+    __syncwarp();
+    const long end = row0 + ROWS < a.L ? row0 + ROWS : a.L;
+    int count = 0, edges = 0;
+    for (long s = first_sequence(a.offsets, a.batch, row0, lane); s < a.batch; s += 32) {
+        long lo = end, hi = end;
+        if (s + lane < a.batch) {
+            lo = a.offsets[s + lane];
+            hi = a.offsets[s + lane + 1];
         }
+        const bool past = s + lane < a.batch && lo >= end;
+        lo = lo < 0 ? 0 : lo;
+        hi = hi > a.L ? a.L : hi;
+        /* the sequence's rows within the tile, and its edges among them */
+        const int from = (int)((lo > row0 ? lo : row0) - row0), until = (int)((hi < end ? hi : end) - row0);
+        const int first = lo >= row0 ? (int)(lo - row0) : -1, last = hi <= end ? (int)(hi - 1 - row0) : -1;
+        unsigned some = __ballot_sync(~0u, !past && from < until);
+        while (some) {
+            const int k = __ffs(some) - 1;
+            some &= some - 1;
+            const int b = __shfl_sync(~0u, from, k), e = __shfl_sync(~0u, until, k);
+            const int f = __shfl_sync(~0u, first, k), l = __shfl_sync(~0u, last, k);
+            for (int r = b + lane; r < e; r += 32) {
+                m.seq[r] = (int)(s + k);
+                m.edge[r] = (unsigned char)((r == f ? 1 : 0) | (r == l ? 2 : 0));
+            }
+            count += e - b;
+            edges += (f >= 0) + (l >= 0);
+        }
+        if (__any_sync(~0u, past)) break;
     }
-    __syncthreads();
+    if (lane == 0) {
+        m.whole = count >= end - row0;
+        m.plain = count == ROWS && edges == 0;
+    }
+    __syncwarp();
 }
 
-/* What an empty sequence's end is: `from` (zeros when NULL) to `to`. */
-__device__ void empty_sequences(const KmbGLR &a, const float *from, float *to, long ch0) {
+/* What an empty sequence's end is: `from` (zeros when NULL) to `to`, for
+ * the channels [ch0, ch1); by `warps` warps. */
+__device__ void empty_sequences(const KmbGLR &a, const float *from, float *to, long ch0, long ch1, int warp,
+                                int warps) {
     if (!to) return;
-    const int lane = threadIdx.x % 32, warps = blockDim.x / 32;
-    for (long s = (threadIdx.x / 32) * 32L; s < a.batch; s += warps * 32L) {
+    const int lane = threadIdx.x % 32;
+    for (long s = warp * 32L; s < a.batch; s += warps * 32L) {
         bool none = false;
         if (s + lane < a.batch) {
             long lo = a.offsets[s + lane], hi = a.offsets[s + lane + 1];
@@ -414,14 +523,14 @@ __device__ void empty_sequences(const KmbGLR &a, const float *from, float *to, l
         while (m) {
             const long k = s + __ffs(m) - 1;
             m &= m - 1;
-            for (long d = ch0 + lane; d < a.D && d < ch0 + kC; d += 32)
+            for (long d = ch0 + lane; d < a.D && d < ch1; d += 32)
                 to[k * a.D + d] = from ? from[k * a.D + d] : 0.f;
         }
     }
 }
 
 /* The lane's channels: the first, and which exist. */
-template <bool VEC>
+template <bool VEC, int V>
 struct Lane {
     long d;
     unsigned m;
@@ -429,33 +538,256 @@ struct Lane {
     static constexpr int kNext = VEC ? 1 : 32; /* to the next channel */
     __device__ __forceinline__ Lane(long ch0, long D) {
         lane = threadIdx.x % 32;
-        d = ch0 + (VEC ? kV * lane : lane);
+        d = ch0 + (VEC ? V * lane : lane);
         m = 0;
 #pragma unroll
-        for (int k = 0; k < kV; ++k) m |= d + k * kNext < D ? 1u << k : 0u;
+        for (int k = 0; k < V; ++k) m |= d + k * kNext < D ? 1u << k : 0u;
     }
     /* a [.., D] fp32 vector at the channels, 0 where NULL */
-    __device__ __forceinline__ F4 at(const float *p) const {
-        return each([&](int k) { return p && (m >> k & 1) ? p[d + k * kNext] : 0.f; });
+    __device__ __forceinline__ F<V> at(const float *p) const {
+        return each<V>([&](int k) { return p && (m >> k & 1) ? p[d + k * kNext] : 0.f; });
     }
-    __device__ __forceinline__ void put(float *p, F4 v) const {
+    __device__ __forceinline__ void put(float *p, F<V> v) const {
 #pragma unroll
-        for (int k = 0; k < kV; ++k)
-            if (p && (m >> k & 1)) p[d + k * kNext] = get(v, k);
+        for (int k = 0; k < V; ++k)
+            if (p && (m >> k & 1)) p[d + k * kNext] = v[k];
     }
 };
 
 /* A tensor's rows of the run: pointer to the lane's channels of row j. */
-template <typename T, bool VEC>
+template <typename T>
 struct Run {
     T *p;
     long step;
-    __device__ __forceinline__ Run(const KmbRows &r, long b, long row, const Lane<VEC> &ln) {
-        p = (T *)r.data + b * r.batch_stride + row * r.row_stride + ln.d;
+    __device__ __forceinline__ Run(const KmbRows &r, long b, long row, long d) {
+        p = (T *)r.data + b * r.batch_stride + row * r.row_stride + d;
         step = r.row_stride;
     }
     __device__ __forceinline__ T *operator[](int j) const { return p + j * step; }
 };
+
+/* Maps of the warps of a tile. */
+template <int W, int V>
+struct Maps {
+    typename Pack<V>::type A[W][32], H[W][32];
+    __device__ __forceinline__ void put(int w, int lane, F<V> a, F<V> h) {
+        A[w][lane] = to(a);
+        H[w][lane] = to(h);
+    }
+    __device__ __forceinline__ Map<V> at(int w, int lane) const { return {from(A[w][lane]), from(H[w][lane])}; }
+};
+
+/* the CTA's barrier, or that of the first N threads */
+struct WholeCta {
+    static __device__ __forceinline__ void sync() { __syncthreads(); }
+};
+template <int N>
+struct FirstThreads {
+    static __device__ __forceinline__ void sync() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
+    static __device__ __forceinline__ bool any(bool p) {
+        int r;
+        asm volatile("{\n\t.reg .pred p, q;\n\t"
+                     "setp.ne.b32 p, %1, 0;\n\t"
+                     "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
+                     "selp.b32 %0, 1, 0, q;\n\t}"
+                     : "=r"(r)
+                     : "r"((int)p), "n"(N)
+                     : "memory");
+        return r != 0;
+    }
+};
+
+/* Joins the tile with the ones before it in its chain and returns the state
+ * that enters it.  agg: the warps' maps, joined from the last when REVERSE;
+ * first: the state that enters the chain. */
+template <typename Sync, bool VEC, bool MARKED, bool REVERSE, int W, int V>
+__device__ __forceinline__ F<V> enter_tile(const Dev &p, const Place &at, const Lane<VEC, V> &ln,
+                                           const Maps<W, V> &agg, Maps<kWindow, V> &seen, int warps,
+                                           const float *first) {
+    const int warp = threadIdx.x / 32;
+    F<V> h = ln.at(at.pos == 0 ? first : nullptr);
+    if (p.tiles == 1) return h;
+    const Shown &s = p.shown;
+    const long o = at.pos * s.step + at.chain * 32 + ln.lane;
+    Map<V> m = {all<V>(1.f), all<V>(0.f)};
+    if (warp == 0 && at.pos + 1 < p.tiles) {
+        for (int k = 0; k < warps; ++k) m = join<MARKED>(m, agg.at(REVERSE ? warps - 1 - k : k, ln.lane));
+        if (at.pos > 0) {
+            show(s.A + o * V, m.A);
+            show(s.H + o * V, m.H);
+        }
+    }
+    if (at.pos > 0) {
+        const int n = at.pos < kWindow ? (int)at.pos : kWindow;
+        for (int k = warp; k < n; k += warps) {
+            const Map<V> v = look<V>(s, o - (k + 1) * s.step, k == kWindow - 1);
+            seen.put(k, ln.lane, v.A, v.H);
+        }
+        Sync::sync();
+        /* from the nearest final states on; the first tile shows nothing else */
+        int k = 0;
+        for (; k < n - 1; ++k) {
+            const F<V> A = from(seen.A[k][ln.lane]);
+            bool constant = true;
+#pragma unroll
+            for (int e = 0; e < V; ++e) constant &= A[e] < 0.f;
+            if (constant) break;
+        }
+        for (; k >= 0; --k) h = apply<true>(seen.at(k, ln.lane), h);
+    }
+    if (warp == 0 && at.pos + 1 < p.tiles) show(s.end + o * V, apply<MARKED>(m, h));
+    return h;
+}
+
+/* ------------------------------------------------------------------ */
+/* a warp's run of rows                                                 */
+/* ------------------------------------------------------------------ */
+
+/*
+ * What the forward and the backward do with a run of R rows; where the rows
+ * come from and go to is the caller's: io.x(j), io.gr(j), io.gi(j), io.dy(j),
+ * io.y(j, v), io.grads(j, g).  FULL: all rows exist and none begins or ends a
+ * sequence.  Packed rows else look themselves up in `rows`.
+ */
+template <typename Io, bool VEC, bool PACKED, bool FULL, bool WEAK, int R, int ROWS, int V>
+struct RunOf {
+    const Dev &p;
+    const Place &at;
+    const Lane<VEC, V> &ln;
+    const RowMap<ROWS> &rows;
+    Io &io;
+    long row0;
+    int live, warp; /* rows that exist (not PACKED) */
+
+    __device__ __forceinline__ bool in(int j) const {
+        return FULL || (PACKED ? rows.seq[warp * R + j] >= 0 : j < live);
+    }
+    __device__ __forceinline__ bool begins(int j) const {
+        return PACKED && !FULL && (rows.edge[warp * R + j] & 1);
+    }
+    __device__ __forceinline__ bool ends(int j) const { return PACKED && !FULL && (rows.edge[warp * R + j] & 2); }
+    /* the sequence's row of a [batch, D] tensor */
+    __device__ __forceinline__ F<V> of(const float *v, int j) const {
+        return ln.at(v ? v + rows.seq[warp * R + j] * p.a.D : nullptr);
+    }
+    __device__ __forceinline__ void put(float *v, int j, F<V> x) const {
+        if (v) ln.put(v + rows.seq[warp * R + j] * p.a.D, x);
+    }
+
+    template <typename Sync, int W>
+    __device__ __forceinline__ void forward(const Rates<V> &rt, Maps<W, V> &agg, Maps<kWindow, V> &seen, int warps) {
+        F<V> c[R], b[R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const Terms<V> t = terms<WEAK>(io.gr(j), io.gi(j), rt);
+            c[j] = t.c;
+            b[j] = t.si * io.x(j);
+        }
+        F<V> A = all<V>(1.f), H = all<V>(0.f);
+        bool fresh = false; /* a sequence begins in this run */
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            if (in(j)) {
+                if (begins(j)) {
+                    H = of(p.a.h0, j);
+                    fresh = true;
+                }
+                H = advance<WEAK>(c[j], H, b[j]);
+                A = shrink<WEAK>(c[j], A);
+            }
+        }
+        agg.put(warp, ln.lane, fresh ? all<V>(-1.f) : A, H);
+        Sync::sync();
+        const float *first = !PACKED && p.a.h0 ? p.a.h0 + at.b * p.a.D : nullptr;
+        F<V> h = enter_tile<Sync, VEC, PACKED, false>(p, at, ln, agg, seen, warps, first);
+        for (int w = 0; w < warp; ++w) h = apply<PACKED>(agg.at(w, ln.lane), h);
+        /* the run's row with a checkpoint, if any */
+        constexpr int chunk = Io::kChunk;
+        static_assert(chunk >= R, "one checkpoint a run");
+        const int mark = p.ckpt_out ? (int)((row0 + chunk - 1) / chunk * chunk - row0) : -1;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            if (in(j)) {
+                if (j == mark) ln.put(p.ckpt_out + (at.b * p.chunks + (row0 + j) / chunk) * p.a.D, h);
+                if (begins(j)) h = of(p.a.h0, j);
+                h = advance<WEAK>(c[j], h, b[j]);
+                io.y(j, h);
+                if (ends(j)) put(p.a.h_last, j, h);
+            }
+        }
+        if (!PACKED && p.a.h_last && live > 0 && row0 + live == p.a.L) ln.put(p.a.h_last + at.b * p.a.D, h);
+    }
+
+    /* The adjoint that reaches row t - 1 from row t is C_t = a_t (dy_t +
+     * C_{t+1}).  entry: the state before the tile.  Returns the sum of udu. */
+    template <typename Sync, int W>
+    __device__ __forceinline__ F<V> backward(const Rates<V> &rt, F<V> entry, Maps<W, V> &states, Maps<W, V> &agg,
+                                             Maps<kWindow, V> &seen, int warps) {
+        const F<V> zero = all<V>(0.f), minus = all<V>(-1.f);
+        Terms<V> t[R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) t[j] = terms<WEAK>(io.gr(j), io.gi(j), rt);
+        F<V> A = all<V>(1.f), H = zero, K = zero;
+        bool fresh = false, closed = false;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            if (in(j)) {
+                if (begins(j)) {
+                    H = of(p.a.h0, j);
+                    fresh = true;
+                }
+                H = advance<WEAK>(t[j].c, H, t[j].si * io.x(j));
+                A = shrink<WEAK>(t[j].c, A);
+            }
+        }
+        states.put(warp, ln.lane, fresh ? minus : A, H);
+#pragma unroll
+        for (int j = R - 1; j >= 0; --j) {
+            if (in(j)) {
+                if (ends(j)) {
+                    K = of(p.a.dh_last, j);
+                    closed = true;
+                }
+                K = shrink<WEAK>(t[j].c, K + io.dy(j));
+            }
+        }
+        agg.put(warp, ln.lane, closed ? minus : A, K);
+        Sync::sync();
+        const float *last = !PACKED && p.a.dh_last ? p.a.dh_last + at.b * p.a.D : nullptr;
+        F<V> C = enter_tile<Sync, VEC, PACKED, true>(p, at, ln, agg, seen, warps, last);
+        for (int w = warps - 1; w > warp; --w) C = apply<PACKED>(agg.at(w, ln.lane), C);
+        F<V> hp[R]; /* the states before each row */
+        {
+            F<V> h = entry;
+            for (int w = 0; w < warp; ++w) h = apply<PACKED>(states.at(w, ln.lane), h);
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                if (begins(j)) h = of(p.a.h0, j);
+                hp[j] = h;
+                h = advance<WEAK>(t[j].c, h, t[j].si * io.x(j));
+            }
+        }
+        F<V> sum = zero;
+#pragma unroll
+        for (int j = R - 1; j >= 0; --j) {
+            if (in(j)) {
+                if (ends(j)) C = of(p.a.dh_last, j);
+                const F<V> G = C + io.dy(j);
+                const Grads<V> g = gradients<WEAK>(t[j], rt.rate, io.x(j), G, hp[j]);
+                sum = sum + g.udu;
+                io.grads(j, g);
+                C = shrink<WEAK>(t[j].c, G);
+                if (begins(j)) put(p.a.dh0, j, C);
+            }
+        }
+        if (!PACKED && row0 == 0 && p.a.dh0) ln.put(p.a.dh0 + at.b * p.a.D, C);
+        return sum;
+    }
+};
+
+/* ------------------------------------------------------------------ */
+/* kernels for any alignment: rows loaded by the threads that own them   */
+/* ------------------------------------------------------------------ */
 
 /* The channels' rates, one thread a channel, and whether one of them is
  * above kWeak.  Ends with a barrier. */
@@ -475,307 +807,430 @@ __device__ __forceinline__ bool make_rates(const KmbGLR &a, long ch0, float *rat
     return __syncthreads_or(strong);
 }
 
-/* Maps of the warps of a tile. */
-template <int W>
-struct Maps {
-    float4 A[W][32], H[W][32];
-    __device__ __forceinline__ void put(int w, int lane, F4 a, F4 h) {
-        A[w][lane] = v4(a);
-        H[w][lane] = v4(h);
-    }
-    __device__ __forceinline__ Map at(int w, int lane) const { return {f4(A[w][lane]), f4(H[w][lane])}; }
-};
-
-/* Joins the tile with the ones before it in its chain and returns the state
- * that enters it.  agg: the warps' maps, joined from the last when reverse;
- * first: the state that enters the chain. */
-template <bool VEC, bool MARKED, bool REVERSE, int W>
-__device__ __forceinline__ F4 enter_tile(const Dev &p, const Place &at, const Lane<VEC> &ln,
-                                         const Maps<W> &agg, Maps<kWindow> &seen, const float *first) {
-    const int warp = threadIdx.x / 32, warps = blockDim.x / 32;
-    F4 h = ln.at(first);
-    if (p.tiles == 1) return h;
-    Shown s = p.shown;
-    const long o = at.pos * s.step + at.chain * 32 + ln.lane;
-    Map m = {f4s(1.f), f4s(0.f)};
-    if (warp == 0 && at.pos + 1 < p.tiles) {
-        for (int k = 0; k < warps; ++k) m = join<MARKED>(m, agg.at(REVERSE ? warps - 1 - k : k, ln.lane));
-        if (at.pos > 0) {
-            show(s.A + o, m.A);
-            show(s.H + o, m.H);
-        }
-    }
-    if (at.pos > 0) {
-        const int n = at.pos < kWindow ? (int)at.pos : kWindow;
-        for (int k = warp; k < n; k += warps) {
-            const Map v = look(s, o - (k + 1) * s.step, k == kWindow - 1);
-            seen.put(k, ln.lane, v.A, v.H);
-        }
-        __syncthreads();
-        /* from the nearest final states on */
-        int k = 0;
-        for (; k < n - 1; ++k) {
-            const float4 A = seen.A[k][ln.lane];
-            if (A.x < 0.f && A.y < 0.f && A.z < 0.f && A.w < 0.f) break;
-        }
-        for (; k >= 0; --k) h = apply<true>(seen.at(k, ln.lane), h);
-    }
-    if (warp == 0 && at.pos + 1 < p.tiles) show(s.end + o, apply<MARKED>(m, h));
-    return h;
-}
-
-/* ------------------------------------------------------------------ */
-/* forward                                                              */
-/* ------------------------------------------------------------------ */
-
-constexpr int kFR = 8;         /* rows of a warp */
-constexpr int kFW = 8;         /* warps of a full CTA */
-constexpr int kFT = kFR * kFW; /* rows of a tile */
-static_assert(kFT % kChunk == 0 || kChunk % kFT == 0, "checkpoints lie at the beginning of a run");
-
-template <bool PACKED>
-struct FwdShared {
-    Maps<kFW> agg;
-    Maps<kWindow> seen;
+template <int W, int ROWS, bool PACKED>
+struct AnyShared {
+    Maps<W, kV> agg;
+    Maps<kWindow, kV> seen;
     float4 rate[32], sroot[32];
     unsigned slot;
-    RowMap<PACKED ? kFT : 1> rows;
+    RowMap<PACKED ? ROWS : 1> rows;
 };
 
-template <typename T, bool VEC, bool PACKED, bool WEAK>
-__device__ __forceinline__ void fwd_tile(const Dev &p, const Place &at, const Lane<VEC> &ln,
-                                         FwdShared<PACKED> &sh, const typename Raw<T>::type (&x)[kFR],
-                                         const typename Raw<T>::type (&gr)[kFR],
-                                         const typename Raw<T>::type (&gi)[kFR], long row0, int live) {
-    const int warp = threadIdx.x / 32;
-    F4 c[kFR], b[kFR];
-    {
-        const Rates rt = {f4(sh.rate[ln.lane]), f4(sh.sroot[ln.lane])};
-#pragma unroll
-        for (int j = 0; j < kFR; ++j) {
-            const Terms t = terms<WEAK>(Raw<T>::f(gr[j]), Raw<T>::f(gi[j]), rt);
-            c[j] = t.c;
-            b[j] = t.si * Raw<T>::f(x[j]);
-        }
-    }
-    const auto in = [&](int j) { return PACKED ? sh.rows.seq[warp * kFR + j] >= 0 : j < live; };
-    const auto begins = [&](int j) { return PACKED && (sh.rows.edge[warp * kFR + j] & 1); };
-    const auto h0 = [&](int j) { return ln.at(p.a.h0 ? p.a.h0 + sh.rows.seq[warp * kFR + j] * p.a.D : nullptr); };
-    F4 A = f4s(1.f), H = f4s(0.f);
-    bool fresh = false; /* a sequence begins in this run */
-#pragma unroll
-    for (int j = 0; j < kFR; ++j) {
-        if (in(j)) {
-            if (begins(j)) {
-                H = h0(j);
-                fresh = true;
-            }
-            H = advance<WEAK>(c[j], H, b[j]);
-            A = shrink<WEAK>(c[j], A);
-        }
-    }
-    sh.agg.put(warp, ln.lane, fresh ? f4s(-1.f) : A, H);
+/* the tile's number; ends with a barrier when a chain has several tiles */
+__device__ __forceinline__ unsigned tile_id(const Dev &p, unsigned *slot) {
+    if (p.tiles == 1) return blockIdx.x;
+    if (threadIdx.x == 0) *slot = take_ticket(p);
     __syncthreads();
-    const float *first = !PACKED && p.a.h0 ? p.a.h0 + at.b * p.a.D : nullptr;
-    F4 h = enter_tile<VEC, PACKED, false>(p, at, ln, sh.agg, sh.seen, first);
-    for (int w = 0; w < warp; ++w) h = apply<PACKED>(sh.agg.at(w, ln.lane), h);
-    if (p.ckpt_out && row0 % kChunk == 0 && row0 < p.a.L)
-        ln.put(p.ckpt_out + (at.b * p.chunks + row0 / kChunk) * p.a.D, h);
-    const Run<T, VEC> y(p.a.y, at.b, row0, ln);
-#pragma unroll
-    for (int j = 0; j < kFR; ++j) {
-        if (in(j)) {
-            if (begins(j)) h = h0(j);
-            h = advance<WEAK>(c[j], h, b[j]);
-            if (!p.states_only) Raw<T>::template store<VEC>(y[j], h, ln.m);
-            if (PACKED && (sh.rows.edge[warp * kFR + j] & 2) && p.a.h_last)
-                ln.put(p.a.h_last + sh.rows.seq[warp * kFR + j] * p.a.D, h);
-        }
-    }
-    if (!PACKED && p.a.h_last && live > 0 && row0 + live == p.a.L) ln.put(p.a.h_last + at.b * p.a.D, h);
+    return *slot;
 }
+
+constexpr int kFR = 8, kFW = 8, kFT = kFR * kFW;
+
+template <typename T, bool VEC>
+struct AnyFwdIo {
+    static constexpr int kChunk = chunk_of<T>;
+    typename Raw<T, kV>::type rx[kFR], rr[kFR], ri[kFR];
+    Run<T> out;
+    unsigned m;
+    __device__ __forceinline__ F<kV> x(int j) const { return Raw<T, kV>::f(rx[j]); }
+    __device__ __forceinline__ F<kV> gr(int j) const { return Raw<T, kV>::f(rr[j]); }
+    __device__ __forceinline__ F<kV> gi(int j) const { return Raw<T, kV>::f(ri[j]); }
+    __device__ __forceinline__ void y(int j, F<kV> v) const {
+        if (out.p) store<VEC>(out[j], v, m);
+    }
+};
 
 template <typename T, bool VEC, bool PACKED>
 __global__ void __launch_bounds__(kFW * 32, 2) k_glr_fwd(const __grid_constant__ Dev p) {
-    __shared__ FwdShared<PACKED> sh;
-    typedef typename Raw<T>::type raw;
+    __shared__ AnyShared<kFW, kFT, PACKED> sh;
     const int warp = threadIdx.x / 32;
-    const Place at = place(p, &sh.slot);
-    const Lane<VEC> ln(at.ch0, p.a.D);
-    const long tile0 = at.pos * kFT, row0 = tile0 + warp * kFR;
+    const Place at(p, tile_id(p, &sh.slot));
+    const long ch0 = (long)at.group * kC;
+    const Lane<VEC, kV> ln(ch0, p.a.D);
+    const long tile0 = (long)at.pos * kFT, row0 = tile0 + warp * kFR;
     const long left = p.a.L - row0;
     const int live = left < 0 ? 0 : left < kFR ? (int)left : kFR;
-    if (PACKED) map_rows(sh.rows, p.a, tile0);
-    raw x[kFR], gr[kFR], gi[kFR];
+    if (PACKED) {
+        if (warp == 0) map_rows(sh.rows, p.a, tile0);
+        __syncthreads();
+    }
+    AnyFwdIo<T, VEC> io = {{}, {}, {}, Run<T>(p.a.y, at.b, row0, ln.d), ln.m};
+    if (p.states_only) io.out.p = nullptr;
     {
-        const Run<const T, VEC> pr(p.a.gate_r, at.b, row0, ln), pi(p.a.gate_i, at.b, row0, ln),
-            px(p.a.x, at.b, row0, ln);
+        const Run<const T> pr(p.a.gate_r, at.b, row0, ln.d), pi(p.a.gate_i, at.b, row0, ln.d),
+            px(p.a.x, at.b, row0, ln.d);
 #pragma unroll
         for (int j = 0; j < kFR; ++j) {
             const unsigned m = (PACKED ? sh.rows.seq[warp * kFR + j] >= 0 : j < live) ? ln.m : 0u;
-            gr[j] = Raw<T>::template load<VEC>(pr[j], m);
-            gi[j] = Raw<T>::template load<VEC>(pi[j], m);
-            x[j] = Raw<T>::template load<VEC>(px[j], m);
+            io.rr[j] = load<VEC>(pr[j], m);
+            io.ri[j] = load<VEC>(pi[j], m);
+            io.rx[j] = load<VEC>(px[j], m);
         }
     }
-    if (make_rates<VEC>(p.a, at.ch0, (float *)sh.rate, (float *)sh.sroot))
-        fwd_tile<T, VEC, PACKED, false>(p, at, ln, sh, x, gr, gi, row0, live);
-    else
-        fwd_tile<T, VEC, PACKED, true>(p, at, ln, sh, x, gr, gi, row0, live);
-    if (PACKED && at.pos == 0) empty_sequences(p.a, p.a.h0, p.a.h_last, at.ch0);
+    const bool strong = make_rates<VEC>(p.a, ch0, (float *)sh.rate, (float *)sh.sroot);
+    const Rates<kV> rt = {from(sh.rate[ln.lane]), from(sh.sroot[ln.lane])};
+    constexpr int ROWS = PACKED ? kFT : 1;
+    if (strong) {
+        RunOf<AnyFwdIo<T, VEC>, VEC, PACKED, false, false, kFR, ROWS, kV> run = {p, at, ln, sh.rows, io, row0, live, warp};
+        run.template forward<WholeCta>(rt, sh.agg, sh.seen, blockDim.x / 32);
+    } else {
+        RunOf<AnyFwdIo<T, VEC>, VEC, PACKED, false, true, kFR, ROWS, kV> run = {p, at, ln, sh.rows, io, row0, live, warp};
+        run.template forward<WholeCta>(rt, sh.agg, sh.seen, blockDim.x / 32);
+    }
+    if (PACKED && at.pos == 0 && !p.states_only)
+        empty_sequences(p.a, p.a.h0, p.a.h_last, ch0, ch0 + kC, warp, blockDim.x / 32);
 }
 
-/* ------------------------------------------------------------------ */
-/* backward                                                             */
-/* ------------------------------------------------------------------ */
+constexpr int kBR = 4, kBW = 14, kBT = kBR * kBW;
+static_assert(kBT % KMB_GLR_CHUNK(KMB_F32) == 0 && kBT % KMB_GLR_CHUNK(KMB_BF16) == 0,
+              "a backward tile begins at a checkpoint");
 
-constexpr int kBR = 4, kBW = 16, kBT = kBR * kBW;
-static_assert(kBT == kChunk, "a backward tile begins at a checkpoint");
-
-template <bool PACKED>
-struct BwdShared {
-    Maps<kBW> states, agg; /* the warps' maps of the states and of the adjoint */
-    Maps<kWindow> seen;
-    float4 rate[32], sroot[32];
-    unsigned slot;
-    RowMap<PACKED ? kBT : 1> rows;
+template <typename T, bool VEC>
+struct AnyBwdIo {
+    typename Raw<T, kV>::type rx[kBR], rr[kBR], ri[kBR], rd[kBR];
+    Run<T> dx, dgr, dgi;
+    unsigned m;
+    __device__ __forceinline__ F<kV> x(int j) const { return Raw<T, kV>::f(rx[j]); }
+    __device__ __forceinline__ F<kV> gr(int j) const { return Raw<T, kV>::f(rr[j]); }
+    __device__ __forceinline__ F<kV> gi(int j) const { return Raw<T, kV>::f(ri[j]); }
+    __device__ __forceinline__ F<kV> dy(int j) const { return Raw<T, kV>::f(rd[j]); }
+    __device__ __forceinline__ void grads(int j, const Grads<kV> &g) const {
+        store<VEC>(dx[j], g.x, m);
+        store<VEC>(dgr[j], g.r, m);
+        store<VEC>(dgi[j], g.i, m);
+    }
 };
 
-/* The adjoint that reaches row t - 1 from row t is C_t = a_t (dy_t + C_{t+1}). */
-template <typename T, bool VEC, bool PACKED, bool WEAK>
-__device__ __forceinline__ void bwd_tile(const Dev &p, const Place &at, const Lane<VEC> &ln,
-                                         BwdShared<PACKED> &sh, const typename Raw<T>::type (&x)[kBR],
-                                         const typename Raw<T>::type (&gr)[kBR],
-                                         const typename Raw<T>::type (&gi)[kBR],
-                                         const typename Raw<T>::type (&dy)[kBR], long tile, long row0,
-                                         int live) {
+template <int W, int ROWS, bool PACKED>
+struct AnyBwdShared : AnyShared<W, ROWS, PACKED> {
+    Maps<W, kV> states;
+};
+
+template <typename T, bool VEC, bool PACKED>
+__global__ void __launch_bounds__(kBW * 32, 1) k_glr_bwd(const __grid_constant__ Dev p) {
+    __shared__ AnyBwdShared<kBW, kBT, PACKED> sh;
     const int warp = threadIdx.x / 32, warps = blockDim.x / 32;
-    const F4 zero = f4s(0.f), one = f4s(1.f), minus = f4s(-1.f);
-    Terms t[kBR];
+    const Place at(p, tile_id(p, &sh.slot));
+    const long ch0 = (long)at.group * kC;
+    const Lane<VEC, kV> ln(ch0, p.a.D);
+    const long tile0 = (long)(p.tiles - 1 - at.pos) * kBT, row0 = tile0 + warp * kBR;
+    const long left = p.a.L - row0;
+    const int live = left < 0 ? 0 : left < kBR ? (int)left : kBR;
+    if (PACKED) {
+        if (warp == 0) map_rows(sh.rows, p.a, tile0);
+        __syncthreads();
+    }
+    AnyBwdIo<T, VEC> io = {{}, {}, {}, {}, Run<T>(p.a.dx, at.b, row0, ln.d), Run<T>(p.a.dgate_r, at.b, row0, ln.d),
+                           Run<T>(p.a.dgate_i, at.b, row0, ln.d), ln.m};
     {
-        const Rates rt = {f4(sh.rate[ln.lane]), f4(sh.sroot[ln.lane])};
-#pragma unroll
-        for (int j = 0; j < kBR; ++j) t[j] = terms<WEAK>(Raw<T>::f(gr[j]), Raw<T>::f(gi[j]), rt);
-    }
-    const auto in = [&](int j) { return PACKED ? sh.rows.seq[warp * kBR + j] >= 0 : j < live; };
-    const auto begins = [&](int j) { return PACKED && (sh.rows.edge[warp * kBR + j] & 1); };
-    const auto ends = [&](int j) { return PACKED && (sh.rows.edge[warp * kBR + j] & 2); };
-    const auto of = [&](const float *v, int j) { return ln.at(v ? v + sh.rows.seq[warp * kBR + j] * p.a.D : nullptr); };
-    F4 A = one, H = zero, K = zero;
-    bool fresh = false, closed = false;
-#pragma unroll
-    for (int j = 0; j < kBR; ++j) {
-        if (in(j)) {
-            if (begins(j)) {
-                H = of(p.a.h0, j);
-                fresh = true;
-            }
-            H = advance<WEAK>(t[j].c, H, t[j].si * Raw<T>::f(x[j]));
-            A = shrink<WEAK>(t[j].c, A);
-        }
-    }
-    sh.states.put(warp, ln.lane, fresh ? minus : A, H);
-#pragma unroll
-    for (int j = kBR - 1; j >= 0; --j) {
-        if (in(j)) {
-            if (ends(j)) {
-                K = of(p.a.dh_last, j);
-                closed = true;
-            }
-            K = shrink<WEAK>(t[j].c, K + Raw<T>::f(dy[j]));
-        }
-    }
-    sh.agg.put(warp, ln.lane, closed ? minus : A, K);
-    __syncthreads();
-
-    const float *last = !PACKED && p.a.dh_last ? p.a.dh_last + at.b * p.a.D : nullptr;
-    F4 C = enter_tile<VEC, PACKED, true>(p, at, ln, sh.agg, sh.seen, last);
-    for (int w = warps - 1; w > warp; --w) C = apply<PACKED>(sh.agg.at(w, ln.lane), C);
-
-    /* the states before each row */
-    F4 hp[kBR];
-    {
-        F4 h = tile < p.chunks ? ln.at(p.ckpt_in + (at.b * p.chunks + tile) * p.a.D) : zero;
-        for (int w = 0; w < warp; ++w) h = apply<PACKED>(sh.states.at(w, ln.lane), h);
+        const Run<const T> pr(p.a.gate_r, at.b, row0, ln.d), pi(p.a.gate_i, at.b, row0, ln.d),
+            px(p.a.x, at.b, row0, ln.d), pd(p.a.dy, at.b, row0, ln.d);
 #pragma unroll
         for (int j = 0; j < kBR; ++j) {
-            if (begins(j)) h = of(p.a.h0, j);
-            hp[j] = h;
-            h = advance<WEAK>(t[j].c, h, t[j].si * Raw<T>::f(x[j]));
+            const unsigned m = (PACKED ? sh.rows.seq[warp * kBR + j] >= 0 : j < live) ? ln.m : 0u;
+            io.rr[j] = load<VEC>(pr[j], m);
+            io.ri[j] = load<VEC>(pi[j], m);
+            io.rx[j] = load<VEC>(px[j], m);
+            io.rd[j] = load<VEC>(pd[j], m);
         }
     }
-    F4 sum = zero;
-    const F4 rate = f4(sh.rate[ln.lane]);
-    const Run<T, VEC> dx(p.a.dx, at.b, row0, ln), dgr(p.a.dgate_r, at.b, row0, ln), dgi(p.a.dgate_i, at.b, row0, ln);
-#pragma unroll
-    for (int j = kBR - 1; j >= 0; --j) {
-        if (in(j)) {
-            if (ends(j)) C = of(p.a.dh_last, j);
-            const F4 c = t[j].c, G = C + Raw<T>::f(dy[j]);
-            const F4 r = t[j].q * t[j].q, u = rate * r, b = t[j].si * Raw<T>::f(x[j]);
-            F4 kappa = poly_kappa(u), ua; /* ua: -u a */
-            if (WEAK) {
-                ua = fma4(c, u, u) * minus;
-            } else {
-                /* e^-u is 0 long before u is 100 */
-                ua = each([&](int n) { return get(u, n) > 100.f ? 0.f : -get(u, n) * get(c, n); });
-                kappa = each([&](int n) {
-                    const float a = get(c, n);
-                    return get(u, n) <= kWeak ? get(kappa, n) : -get(ua, n) * a * rcp_mufu(fmaf(-a, a, 1.f));
-                });
-            }
-            const F4 udu = G * fma4(ua, hp[j], kappa * b);
-            sum = sum + udu;
-            Raw<T>::template store<VEC>(dx[j], G * t[j].si, ln.m);
-            Raw<T>::template store<VEC>(dgr[j], udu * fma4(r, minus, one), ln.m);
-            Raw<T>::template store<VEC>(dgi[j], G * b * fma4(t[j].i, minus, one), ln.m);
-            C = shrink<WEAK>(c, G);
-            if (begins(j) && p.a.dh0) ln.put(p.a.dh0 + sh.rows.seq[warp * kBR + j] * p.a.D, C);
-        }
+    const F<kV> entry = ln.at(tile0 < p.a.L ? p.ckpt_in + (at.b * p.chunks + tile0 / chunk_of<T>) * p.a.D : nullptr);
+    const bool strong = make_rates<VEC>(p.a, ch0, (float *)sh.rate, (float *)sh.sroot);
+    const Rates<kV> rt = {from(sh.rate[ln.lane]), from(sh.sroot[ln.lane])};
+    constexpr int ROWS = PACKED ? kBT : 1;
+    F<kV> sum;
+    if (strong) {
+        RunOf<AnyBwdIo<T, VEC>, VEC, PACKED, false, false, kBR, ROWS, kV> run = {p, at, ln, sh.rows, io, row0, live, warp};
+        sum = run.template backward<WholeCta>(rt, entry, sh.states, sh.agg, sh.seen, warps);
+    } else {
+        RunOf<AnyBwdIo<T, VEC>, VEC, PACKED, false, true, kBR, ROWS, kV> run = {p, at, ln, sh.rows, io, row0, live, warp};
+        sum = run.template backward<WholeCta>(rt, entry, sh.states, sh.agg, sh.seen, warps);
     }
-    if (!PACKED && tile == 0 && warp == 0 && p.a.dh0) ln.put(p.a.dh0 + at.b * p.a.D, C);
     if (p.part) {
         __syncthreads(); /* every warp is done with the states' maps */
-        sh.states.H[warp][ln.lane] = v4(sum);
+        sh.states.H[warp][ln.lane] = to(sum);
         __syncthreads();
         for (int k = threadIdx.x; k < kC; k += blockDim.x) {
             float v = 0.f;
             for (int w = 0; w < warps; ++w) v += ((const float *)sh.states.H[w])[k];
             const int ch = VEC ? k : (k % kV) * 32 + k / kV;
-            p.part[(at.pos * p.chains + at.chain) * kC + ch] = v;
+            p.part[((long)at.pos * p.chains + at.chain) * kC + ch] = v;
         }
+    }
+    if (PACKED && tile0 == 0) empty_sequences(p.a, p.a.dh_last, p.a.dh0, ch0, ch0 + kC, warp, warps);
+}
+
+/* ------------------------------------------------------------------ */
+/* resident kernels: tiles through a ring of tensor copies               */
+/* ------------------------------------------------------------------ */
+
+/*
+ * For tensors that tensor copies can take, and more tiles than the GPU holds
+ * at once.  Two CTAs an SM stay for the whole call.  Their last warp takes
+ * tickets, brings the next tile into the other stage of a ring of two while
+ * the others work on theirs, prepares what depends on the channel (rates,
+ * the checkpoint) or the row (which sequence), and stores results, which the
+ * working warps leave in place of the inputs that they came from.  The
+ * working warps thus read and write shared memory only, at fixed offsets.
+ * 56 rows x 128 channels of bf16 x 3 tensors are 42 KB: 84 KB of an SM's
+ * inputs are on their way at any time.  Seven working warps: with the eighth,
+ * two CTAs have 128 registers a thread (a ninth would leave 96, and spills).
+ */
+constexpr int kW = 7;              /* working warps */
+constexpr int kWork = 32 * kW;
+
+template <typename T, bool BWD>
+struct Shape {
+    static constexpr bool kHalf = sizeof(T) == 2;
+    static constexpr int V = !BWD && kHalf ? 4 : 2;   /* channels of a lane */
+    static constexpr int R = BWD && !kHalf ? 4 : 8;   /* rows of a warp */
+    static constexpr int C = 32 * V, ROWS = R * kW;
+    static constexpr int N = BWD ? 4 : 3;             /* tensors in */
+    static constexpr int kTile = ROWS * C * (int)sizeof(T); /* bytes of one */
+    static constexpr int kStage = N * kTile;
+};
+
+static_assert(Shape<float, true>::ROWS % KMB_GLR_CHUNK(KMB_F32) == 0 &&
+                  Shape<__nv_bfloat16, true>::ROWS % KMB_GLR_CHUNK(KMB_BF16) == 0,
+              "a backward tile begins at a checkpoint");
+
+struct TensorMaps {
+    CUtensorMap in[4], out[3]; /* x, gate_r, gate_i, dy; y or dx, dgate_r, dgate_i */
+};
+
+template <typename T, bool BWD, bool PACKED>
+struct Stage { /* what the last warp prepares beside the tile */
+    typedef Shape<T, BWD> S;
+    typename Pack<S::V>::type rate[32], sroot[32], entry[32];
+    unsigned id;
+    int strong, more;
+    RowMap<PACKED ? S::ROWS : 1> rows;
+};
+
+template <typename T, bool BWD, bool PACKED>
+struct RingShared {
+    typedef Shape<T, BWD> S;
+    Maps<kW, S::V> agg;
+    Maps<BWD ? kW : 1, S::V> states;
+    Maps<kWindow, S::V> seen;
+    Stage<T, BWD, PACKED> stage[2];
+    uint64_t full[2], done[2];
+};
+
+__device__ __forceinline__ void tensor_load(void *dst, const CUtensorMap *m, int x, int y, int z, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+                 "[%2];" ::"r"(kmb_smem(dst)),
+                 "l"(m), "r"(kmb_smem(bar)), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void tensor_store(const CUtensorMap *m, int x, int y, int z, const void *src) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(m),
+                 "r"(kmb_smem(src)), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+
+template <typename T, bool BWD, bool PACKED>
+__device__ __forceinline__ void feed(const Dev &p, const TensorMaps &tm, char *tiles, RingShared<T, BWD, PACKED> &sh) {
+    typedef Shape<T, BWD> S;
+    const int lane = threadIdx.x % 32;
+    const unsigned total = p.tiles * p.chains;
+    const auto first_row = [&](const Place &at) {
+        return (int)((BWD ? p.tiles - 1 - at.pos : at.pos) * (unsigned)S::ROWS);
+    };
+    /* the results of the tile in stage k leave it; false when a wait gave up */
+    const auto leave = [&](int k, int parity) {
+        if (!kmb_mbar_wait(&sh.done[k], parity, &g_glr_error)) return false;
+        if (!p.states_only && (!PACKED || sh.stage[k].rows.whole) && lane == 0) {
+            const Place at(p, sh.stage[k].id);
+            char *tile = tiles + k * S::kStage;
+            for (int n = 0; n < (BWD ? 3 : 1); ++n)
+                tensor_store(&tm.out[n], (int)at.group * S::C, first_row(at), (int)at.b, tile + n * S::kTile);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        }
+        __syncwarp();
+        return true;
+    };
+    int n = 0;
+    bool ok = true;
+    for (;; ++n) {
+        const int k = n & 1;
+        Stage<T, BWD, PACKED> &st = sh.stage[k];
+        if (n >= 2 && !(ok = leave(k, ((n >> 1) - 1) & 1))) break;
+        unsigned id = 0;
+        if (lane == 0) id = take_ticket(p);
+        id = __shfl_sync(~0u, id, 0);
+        if (id >= total) {
+            if (lane == 0) {
+                st.more = 0;
+                kmb_mbar_arrive(&sh.full[k]);
+                kmb_mbar_arrive(&sh.full[k]);
+            }
+            break;
+        }
+        const Place at(p, id);
+        const int row = first_row(at), ch0 = (int)at.group * S::C;
+        if (lane == 0) {
+            char *tile = tiles + k * S::kStage;
+            kmb_mbar_expect(&sh.full[k], S::kStage);
+            /* the gates first: work begins with them */
+            const int order[4] = {1, 2, 0, 3};
+            for (int t = 0; t < S::N; ++t)
+                tensor_load(tile + order[t] * S::kTile, &tm.in[order[t]], ch0, row, (int)at.b, &sh.full[k]);
+            st.id = id;
+            st.more = 1;
+        }
+        const Lane<true, S::V> ln(ch0, p.a.D);
+        const F<S::V> decay = ln.at(p.a.decay);
+        bool strong = false;
+        const F<S::V> rate = each<S::V>([&](int e) {
+            const float r = ln.m >> e & 1 ? p.a.scale * softplus(decay[e]) : 0.f;
+            strong |= !(r <= kWeak);
+            return r;
+        });
+        st.rate[lane] = to(rate);
+        st.sroot[lane] = to(each<S::V>([&](int e) { return sqrtf(2.f * rate[e]); }));
+        if (BWD) st.entry[lane] = to(ln.at(row < p.a.L ? p.ckpt_in + (at.b * p.chunks + row / chunk_of<T>) * p.a.D : nullptr));
+        strong = __any_sync(~0u, strong);
+        if (lane == 0) st.strong = strong;
+        if constexpr (PACKED) map_rows(st.rows, p.a, row);
+        __syncwarp();
+        if (lane == 0) kmb_mbar_arrive(&sh.full[k]);
+    }
+    if (ok && n >= 1) ok = leave((n - 1) & 1, ((n - 1) >> 1) & 1);
+    if (!ok) { /* copies that may still be under way land before the CTA ends, or a second goes by */
+        const long long t0 = clock64();
+        for (int m = n > 1 ? n - 2 : 0; m <= n; ++m)
+            while (!kmb_mbar_done(&sh.full[m & 1], (m >> 1) & 1) && clock64() - t0 < (1ll << 31)) {
+            }
     }
 }
 
-template <typename T, bool VEC, bool PACKED>
-__global__ void __launch_bounds__(kBW * 32, 1) k_glr_bwd(const __grid_constant__ Dev p) {
-    __shared__ BwdShared<PACKED> sh;
-    typedef typename Raw<T>::type raw;
-    const int warp = threadIdx.x / 32;
-    const Place at = place(p, &sh.slot);
-    const Lane<VEC> ln(at.ch0, p.a.D);
-    const long tile = p.tiles - 1 - at.pos, tile0 = tile * kBT, row0 = tile0 + warp * kBR;
-    const long left = p.a.L - row0;
-    const int live = left < 0 ? 0 : left < kBR ? (int)left : kBR;
-    if (PACKED) map_rows(sh.rows, p.a, tile0);
-    raw x[kBR], gr[kBR], gi[kBR], dy[kBR];
-    {
-        const Run<const T, VEC> pr(p.a.gate_r, at.b, row0, ln), pi(p.a.gate_i, at.b, row0, ln),
-            px(p.a.x, at.b, row0, ln), pd(p.a.dy, at.b, row0, ln);
-#pragma unroll
-        for (int j = 0; j < kBR; ++j) {
-            const unsigned m = (PACKED ? sh.rows.seq[warp * kBR + j] >= 0 : j < live) ? ln.m : 0u;
-            gr[j] = Raw<T>::template load<VEC>(pr[j], m);
-            gi[j] = Raw<T>::template load<VEC>(pi[j], m);
-            x[j] = Raw<T>::template load<VEC>(px[j], m);
-            dy[j] = Raw<T>::template load<VEC>(pd[j], m);
+/* the lane's channels of the tile in shared memory, rows of the warp's run */
+template <typename T, bool BWD>
+struct TileIo {
+    typedef Shape<T, BWD> S;
+    [[maybe_unused]] static constexpr int kChunk = chunk_of<T>;
+    typedef Raw<T, S::V> W;
+    typedef typename W::type raw;
+    raw *base;     /* row 0 of the run in the first tensor */
+    const Dev *p;  /* rows go to global memory themselves when some are of no sequence */
+    long b, row0;
+    int lane_ch;   /* the lane's first channel */
+    unsigned m;
+    bool direct, skip;
+    __device__ __forceinline__ raw *at(int n, int j) const {
+        return base + (n * S::kTile + j * S::C * (int)sizeof(T)) / (int)sizeof(raw);
+    }
+    __device__ __forceinline__ F<S::V> x(int j) const { return W::f(*at(0, j)); }
+    __device__ __forceinline__ F<S::V> gr(int j) const { return W::f(*at(1, j)); }
+    __device__ __forceinline__ F<S::V> gi(int j) const { return W::f(*at(2, j)); }
+    __device__ __forceinline__ F<S::V> dy(int j) const { return W::f(*at(3, j)); }
+    __device__ __forceinline__ void out(int n, int j, F<S::V> v, const KmbRows &r) const {
+        if (!direct) {
+            *at(n, j) = W::r(v);
+        } else if (m) {
+            *reinterpret_cast<raw *>((T *)r.data + b * r.batch_stride + (row0 + j) * r.row_stride + lane_ch) = W::r(v);
         }
     }
-    if (make_rates<VEC>(p.a, at.ch0, (float *)sh.rate, (float *)sh.sroot))
-        bwd_tile<T, VEC, PACKED, false>(p, at, ln, sh, x, gr, gi, dy, tile, row0, live);
-    else
-        bwd_tile<T, VEC, PACKED, true>(p, at, ln, sh, x, gr, gi, dy, tile, row0, live);
-    if (PACKED && tile == 0) empty_sequences(p.a, p.a.dh_last, p.a.dh0, at.ch0);
+    __device__ __forceinline__ void y(int j, F<S::V> v) const {
+        if (!skip) out(0, j, v, p->a.y);
+    }
+    __device__ __forceinline__ void grads(int j, const Grads<S::V> &g) const {
+        out(0, j, g.x, p->a.dx);
+        out(1, j, g.r, p->a.dgate_r);
+        out(2, j, g.i, p->a.dgate_i);
+    }
+};
+
+template <typename T, bool BWD, bool PACKED, bool FULL, bool WEAK>
+__device__ __forceinline__ void work(const Dev &p, const Place &at, TileIo<T, BWD> &io, RingShared<T, BWD, PACKED> &sh,
+                                     int k, const Lane<true, Shape<T, BWD>::V> &ln, long row0, int live, int warp) {
+    typedef Shape<T, BWD> S;
+    typedef FirstThreads<kWork> Sync;
+    const Stage<T, BWD, PACKED> &st = sh.stage[k];
+    const Rates<S::V> rt = {from(st.rate[ln.lane]), from(st.sroot[ln.lane])};
+    RunOf<TileIo<T, BWD>, true, PACKED, FULL, WEAK, S::R, PACKED ? S::ROWS : 1, S::V> run = {p,  at,   ln,   st.rows,
+                                                                                             io, row0, live, warp};
+    if constexpr (BWD) {
+        const F<S::V> sum = run.template backward<Sync>(rt, from(st.entry[ln.lane]), sh.states, sh.agg, sh.seen, kW);
+        if (p.part) {
+            Sync::sync(); /* every warp is done with the states' maps */
+            sh.states.H[warp][ln.lane] = to(sum);
+            Sync::sync();
+            if (threadIdx.x < S::C) {
+                float v = 0.f;
+                for (int w = 0; w < kW; ++w) v += ((const float *)sh.states.H[w])[threadIdx.x];
+                p.part[((long)at.pos * p.chains + at.chain) * S::C + threadIdx.x] = v;
+            }
+        }
+    } else {
+        run.template forward<Sync>(rt, sh.agg, sh.seen, kW);
+    }
+}
+
+template <typename T, bool BWD, bool PACKED>
+__global__ void __launch_bounds__(kWork + 32, 2) k_glr_ring(const __grid_constant__ Dev p,
+                                                            const __grid_constant__ TensorMaps tm) {
+    typedef Shape<T, BWD> S;
+    extern __shared__ __align__(128) char tiles[];
+    RingShared<T, BWD, PACKED> &sh = *reinterpret_cast<RingShared<T, BWD, PACKED> *>(tiles + 2 * S::kStage);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (threadIdx.x == 0) {
+        for (int k = 0; k < 2; ++k) {
+            kmb_mbar_init(&sh.full[k], 2);
+            kmb_mbar_init(&sh.done[k], kW);
+        }
+        kmb_mbar_init_fence();
+    }
+    __syncthreads();
+    if (warp == kW) {
+        feed(p, tm, tiles, sh);
+        return;
+    }
+    for (int n = 0;; ++n) {
+        const int k = n & 1;
+        const bool ok = kmb_mbar_wait(&sh.full[k], (n >> 1) & 1, &g_glr_error);
+        /* all or none go on; also, every warp is done with the maps of the tile before */
+        if (FirstThreads<kWork>::any(!ok)) return;
+        const Stage<T, BWD, PACKED> &st = sh.stage[k];
+        if (!st.more) return;
+        const Place at(p, st.id);
+        const long ch0 = (long)at.group * S::C;
+        const Lane<true, S::V> ln(ch0, p.a.D);
+        const long tile0 = (long)(BWD ? p.tiles - 1 - at.pos : at.pos) * S::ROWS, row0 = tile0 + warp * S::R;
+        const long left = p.a.L - row0;
+        const int live = left < 0 ? 0 : left < S::R ? (int)left : S::R;
+        bool full = tile0 + S::ROWS <= p.a.L, direct = false;
+        if constexpr (PACKED) {
+            full = st.rows.plain;
+            direct = !st.rows.whole;
+        }
+        TileIo<T, BWD> io;
+        io.base = reinterpret_cast<typename TileIo<T, BWD>::raw *>(tiles + k * S::kStage +
+                                                                   (warp * S::R * S::C + lane * S::V) * (int)sizeof(T));
+        io.p = &p;
+        io.b = at.b;
+        io.row0 = row0;
+        io.lane_ch = (int)ln.d;
+        io.m = ln.m;
+        io.direct = direct;
+        io.skip = p.states_only;
+        if (st.strong) {
+            if (full) work<T, BWD, PACKED, true, false>(p, at, io, sh, k, ln, row0, live, warp);
+            else work<T, BWD, PACKED, false, false>(p, at, io, sh, k, ln, row0, live, warp);
+        } else {
+            if (full) work<T, BWD, PACKED, true, true>(p, at, io, sh, k, ln, row0, live, warp);
+            else work<T, BWD, PACKED, false, true>(p, at, io, sh, k, ln, row0, live, warp);
+        }
+        if (PACKED && tile0 == 0 && !p.states_only) {
+            if (BWD) empty_sequences(p.a, p.a.dh_last, p.a.dh0, ch0, ch0 + S::C, warp, kW);
+            else empty_sequences(p.a, p.a.h0, p.a.h_last, ch0, ch0 + S::C, warp, kW);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); /* the results, for the tensor stores */
+        __syncwarp();
+        if (lane == 0) kmb_mbar_arrive(&sh.done[k]);
+    }
 }
 
 /* ddecay: the sums of all tiles and sequences, 32 columns a CTA, 32 rows of
@@ -825,19 +1280,19 @@ __global__ void __launch_bounds__(kStepThreads) k_glr_step(KmbGLRStep a, long ti
     const long d = (blockIdx.x - k * tiles) * kStepThreads + threadIdx.x;
     if (d >= a.D) return;
     const float rate = a.scale * softplus(a.decay[d]);
-    const Rates rt = {f4s(rate), f4s(sqrtf(2.f * rate))};
+    const Rates<2> rt = {all<2>(rate), all<2>(sqrtf(2.f * rate))};
     const T *px = (const T *)a.x.data + k * a.x.row_stride + d;
     const T *pr = (const T *)a.gate_r.data + k * a.gate_r.row_stride + d;
     const T *pi = (const T *)a.gate_i.data + k * a.gate_i.row_stride + d;
-    const F4 gr = f4s((float)*pr), gi = f4s((float)*pi), x = f4s((float)*px);
+    const F<2> gr = all<2>((float)*pr), gi = all<2>((float)*pi), x = all<2>((float)*px);
     float *s = a.state + slot * a.ld_state + d;
     float h = *s;
     if (rate <= kWeak) {
-        const Terms t = terms<true>(gr, gi, rt);
-        h = advance<true>(t.c, f4s(h), t.si * x).l.x;
+        const Terms<2> t = terms<true>(gr, gi, rt);
+        h = advance<true>(t.c, all<2>(h), t.si * x)[0];
     } else {
-        const Terms t = terms<false>(gr, gi, rt);
-        h = advance<false>(t.c, f4s(h), t.si * x).l.x;
+        const Terms<2> t = terms<false>(gr, gi, rt);
+        h = advance<false>(t.c, all<2>(h), t.si * x)[0];
     }
     *s = h;
     ((T *)a.y.data)[k * a.y.row_stride + d] = (T)h;
@@ -866,75 +1321,196 @@ bool vectors(const KmbGLR *a, const KmbRows *const *rows, int n) {
     return true;
 }
 
+/* Tiles and their order for one of the kernels. */
 struct Plan {
     long tiles, groups, batch, chains;
+    int rows, channels;
+    bool ring;
     size_t words; /* of each of the three shown arrays */
 };
 
-Plan plan(const KmbGLR *a, int rows) {
+Plan plan(const KmbGLR *a, int rows, int channels) {
     Plan q;
+    q.rows = rows;
+    q.channels = channels;
+    q.ring = false;
     q.tiles = (a->L + rows - 1) / rows;
     if (a->offsets && q.tiles == 0) q.tiles = 1; /* for the empty sequences */
-    q.groups = (a->D + kC - 1) / kC;
+    q.groups = (a->D + channels - 1) / channels;
     q.batch = a->offsets ? 1 : a->batch;
     q.chains = q.groups * q.batch;
-    q.words = q.tiles > 1 ? (size_t)q.tiles * q.chains * kC : 0;
+    q.words = q.tiles > 1 ? (size_t)q.tiles * q.chains * channels : 0;
     return q;
+}
+
+constexpr int kSMs = 148;
+
+/* Whether tensor copies can take the tensor: whole 16-byte pieces, batch
+ * after batch, coordinates of 32 bits. */
+bool tensor_ok(const KmbGLR *a, const KmbRows &r) {
+    const long es = a->type == KMB_BF16 ? 2 : 4;
+    if ((size_t)r.data % 16 || r.row_stride * es % 16 || r.row_stride * es >= (1L << 40)) return false;
+    if (a->offsets || a->batch <= 1) return true;
+    return r.batch_stride * es % 16 == 0 && r.batch_stride >= a->L * r.row_stride && r.batch_stride * es < (1L << 40);
+}
+
+/*
+ * The plan of a direction: the resident kernel where the tensors allow it
+ * and there are more tiles than half of its CTAs, else the kernel for any
+ * alignment, one CTA a tile.
+ */
+template <typename T>
+Plan plan_of(const KmbGLR *a, bool bwd) {
+    const Plan any = bwd ? plan(a, kBT, kC) : plan(a, kFT, kC);
+    const KmbRows fwd_rows[] = {a->x, a->gate_r, a->gate_i, a->y};
+    const KmbRows bwd_rows[] = {a->x, a->gate_r, a->gate_i, a->dy, a->dx, a->dgate_r, a->dgate_i};
+    Plan q = bwd ? plan(a, Shape<T, true>::ROWS, Shape<T, true>::C) : plan(a, Shape<T, false>::ROWS, Shape<T, false>::C);
+    if (a->D % kV || a->L >= (1L << 31) - 1024 || q.tiles < 2 || q.tiles * q.chains < kSMs) return any;
+    if (q.tiles * q.chains >= (1L << 31)) return any;
+    for (int i = 0; i < (bwd ? 7 : 4); ++i) {
+        const KmbRows &r = bwd ? bwd_rows[i] : fwd_rows[i];
+        if (r.data && !tensor_ok(a, r)) return any;
+    }
+    q.ring = true;
+    return q;
+}
+Plan plan_of(const KmbGLR *a, bool bwd) {
+    return a->type == KMB_BF16 ? plan_of<__nv_bfloat16>(a, bwd) : plan_of<float>(a, bwd);
 }
 
 constexpr size_t kHead = 64; /* bytes before the shown arrays: the ticket */
 
 size_t shown_bytes(const Plan &q) { return q.words ? kHead + 12 * q.words : 0; }
+/* for either kernel, whatever the pointers turn out to be */
+size_t shown_most(const KmbGLR *a, bool bwd) {
+    const bool half = a->type == KMB_BF16;
+    const Plan any = bwd ? plan(a, kBT, kC) : plan(a, kFT, kC);
+    const Plan ring = bwd ? (half ? plan(a, Shape<__nv_bfloat16, true>::ROWS, Shape<__nv_bfloat16, true>::C)
+                                  : plan(a, Shape<float, true>::ROWS, Shape<float, true>::C))
+                          : (half ? plan(a, Shape<__nv_bfloat16, false>::ROWS, Shape<__nv_bfloat16, false>::C)
+                                  : plan(a, Shape<float, false>::ROWS, Shape<float, false>::C));
+    const size_t m = shown_bytes(any), n = shown_bytes(ring);
+    return m > n ? m : n;
+}
+size_t part_most(const KmbGLR *a) {
+    const Plan any = plan(a, kBT, kC);
+    const Plan ring = a->type == KMB_BF16 ? plan(a, Shape<__nv_bfloat16, true>::ROWS, Shape<__nv_bfloat16, true>::C)
+                                          : plan(a, Shape<float, true>::ROWS, Shape<float, true>::C);
+    const size_t m = (size_t)any.tiles * any.chains * kC, n = (size_t)ring.tiles * ring.chains * ring.channels;
+    return 4 * (m > n ? m : n);
+}
 
 /* Fills the workspace's shown arrays and sets the pointers. */
 int begin(Dev &d, const Plan &q, void *ws, cudaStream_t s) {
     if (q.tiles >= (1L << 31) / q.chains) return kmb_fail(KMB_EUNSUPPORTED, "glr: too many tiles");
-    d.tiles = q.tiles;
-    d.groups = q.groups;
-    d.chains = q.chains;
+    d.tiles = (unsigned)q.tiles;
+    d.groups = (unsigned)q.groups;
+    d.chains = (unsigned)q.chains;
+    const long chunk = KMB_GLR_CHUNK(d.a.type);
+    d.chunks = (d.a.L + chunk - 1) / chunk;
     if (!q.words) return KMB_OK;
     const cudaError_t e = cudaMemsetAsync(ws, 0xff, shown_bytes(q), s);
     if (e != cudaSuccess) return kmb_cuda_fail(e, "glr: workspace fill");
     d.ticket = (unsigned *)ws;
-    d.shown.A = (float4 *)((char *)ws + kHead);
-    d.shown.H = d.shown.A + q.words / kV;
-    d.shown.end = d.shown.H + q.words / kV;
+    d.shown.A = (float *)((char *)ws + kHead);
+    d.shown.H = d.shown.A + q.words;
+    d.shown.end = d.shown.H + q.words;
     d.shown.step = q.chains * 32;
     return KMB_OK;
 }
 
-template <typename T>
-int launch_fwd(const Dev &d, const Plan &q, bool vec, cudaStream_t s) {
-    const long n = q.tiles * q.chains;
-    const long runs = (d.a.L + kFR - 1) / kFR;
-    const unsigned threads = 32u * (unsigned)(runs < 1 ? 1 : runs < kFW ? runs : kFW);
-    if (d.a.offsets) {
-        if (vec) k_glr_fwd<T, true, true><<<(unsigned)n, threads, 0, s>>>(d);
-        else k_glr_fwd<T, false, true><<<(unsigned)n, threads, 0, s>>>(d);
-    } else {
-        if (vec) k_glr_fwd<T, true, false><<<(unsigned)n, threads, 0, s>>>(d);
-        else k_glr_fwd<T, false, false><<<(unsigned)n, threads, 0, s>>>(d);
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    if (!fn) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(p);
+        else
+            (void)cudaGetLastError();
     }
-    return done("glr: forward launch");
+    return fn;
+}
+
+/* [batch, L, D] with boxes of rows x channels; outside, loads give zeros and
+ * stores do nothing */
+int tensor_map(CUtensorMap *m, const KmbGLR &a, const KmbRows &r, const Plan &q) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return kmb_fail(KMB_ECUDA, "glr: cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t es = a.type == KMB_BF16 ? 2 : 4;
+    const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.L, (cuuint64_t)q.batch};
+    const cuuint64_t batch = q.batch > 1 ? (cuuint64_t)r.batch_stride * es : (cuuint64_t)a.L * r.row_stride * es;
+    const cuuint64_t strides[2] = {(cuuint64_t)r.row_stride * es, batch};
+    const cuuint32_t box[3] = {(cuuint32_t)q.channels, (cuuint32_t)q.rows, 1}, one[3] = {1, 1, 1};
+    const CUresult rc = fn(m, a.type == KMB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                           3, r.data, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? KMB_OK : kmb_fail(KMB_EINVAL, "glr: tensor map rejected (CUresult %d)", (int)rc);
+}
+
+template <typename T, bool BWD, bool PACKED>
+int launch_ring(const Dev &d, const Plan &q, const TensorMaps &tm, cudaStream_t s) {
+    typedef Shape<T, BWD> S;
+    auto k = k_glr_ring<T, BWD, PACKED>;
+    const size_t bytes = 2 * S::kStage + sizeof(RingShared<T, BWD, PACKED>);
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) return kmb_cuda_fail(e, "glr: shared memory");
+    const long n = q.tiles * q.chains;
+    k<<<(unsigned)(n < 2 * kSMs ? n : 2 * kSMs), kWork + 32, bytes, s>>>(d, tm);
+    return done("glr: launch");
 }
 
 template <typename T>
-int launch_bwd(const Dev &d, const Plan &q, bool vec, cudaStream_t s) {
-    const long n = q.tiles * q.chains;
-    const long runs = (d.a.L + kBR - 1) / kBR;
-    const unsigned threads = 32u * (unsigned)(runs < 1 ? 1 : runs < kBW ? runs : kBW);
-    if (d.a.offsets) {
-        if (vec) k_glr_bwd<T, true, true><<<(unsigned)n, threads, 0, s>>>(d);
-        else k_glr_bwd<T, false, true><<<(unsigned)n, threads, 0, s>>>(d);
-    } else {
-        if (vec) k_glr_bwd<T, true, false><<<(unsigned)n, threads, 0, s>>>(d);
-        else k_glr_bwd<T, false, false><<<(unsigned)n, threads, 0, s>>>(d);
+int launch(const Dev &d, const Plan &q, bool bwd, bool vec, cudaStream_t s) {
+    const bool packed = d.a.offsets != nullptr;
+    if (q.ring) {
+        TensorMaps tm;
+        const KmbRows in[] = {d.a.x, d.a.gate_r, d.a.gate_i, d.a.dy};
+        const KmbRows out[] = {bwd ? d.a.dx : d.a.y, d.a.dgate_r, d.a.dgate_i};
+        for (int i = 0; i < (bwd ? 4 : 3); ++i) {
+            const int rc = tensor_map(&tm.in[i], d.a, in[i], q);
+            if (rc) return rc;
+        }
+        for (int i = 0; i < (bwd ? 3 : d.states_only ? 0 : 1); ++i) {
+            const int rc = tensor_map(&tm.out[i], d.a, out[i], q);
+            if (rc) return rc;
+        }
+        if (bwd) return packed ? launch_ring<T, true, true>(d, q, tm, s) : launch_ring<T, true, false>(d, q, tm, s);
+        return packed ? launch_ring<T, false, true>(d, q, tm, s) : launch_ring<T, false, false>(d, q, tm, s);
     }
-    return done("glr: backward launch");
+    const unsigned n = (unsigned)(q.tiles * q.chains);
+    const int most = bwd ? kBW : kFW;
+    const long runs = (d.a.L + (bwd ? kBR : kFR) - 1) / (bwd ? kBR : kFR);
+    const unsigned threads = 32u * (unsigned)(runs < 1 ? 1 : runs < most ? runs : most);
+    if (bwd) {
+        auto k = packed ? (vec ? k_glr_bwd<T, true, true> : k_glr_bwd<T, false, true>)
+                        : (vec ? k_glr_bwd<T, true, false> : k_glr_bwd<T, false, false>);
+        k<<<n, threads, 0, s>>>(d);
+    } else {
+        auto k = packed ? (vec ? k_glr_fwd<T, true, true> : k_glr_fwd<T, false, true>)
+                        : (vec ? k_glr_fwd<T, true, false> : k_glr_fwd<T, false, false>);
+        k<<<n, threads, 0, s>>>(d);
+    }
+    return done("glr: launch");
+}
+int launch(const Dev &d, const Plan &q, bool bwd, bool vec, cudaStream_t s) {
+    return d.a.type == KMB_BF16 ? launch<__nv_bfloat16>(d, q, bwd, vec, s) : launch<float>(d, q, bwd, vec, s);
+}
+
+/* packed rows have no batch */
+void drop_batch(KmbGLR &a) {
+    KmbRows *const all[] = {&a.x, &a.gate_r, &a.gate_i, &a.y, &a.dy, &a.dx, &a.dgate_r, &a.dgate_i};
+    if (a.offsets)
+        for (KmbRows *r : all) r->batch_stride = 0;
 }
 
 int run_fwd(const KmbGLR *a, float *ckpt, bool write_y, void *ws, cudaStream_t s) {
-    const Plan q = plan(a, kFT);
     Dev d = {};
     d.a = *a;
     if (!write_y) {
@@ -942,15 +1518,13 @@ int run_fwd(const KmbGLR *a, float *ckpt, bool write_y, void *ws, cudaStream_t s
         d.a.y.data = nullptr;
         d.a.h_last = nullptr;
     }
-    if (a->offsets)
-        d.a.x.batch_stride = d.a.gate_r.batch_stride = d.a.gate_i.batch_stride = d.a.y.batch_stride = 0;
+    drop_batch(d.a);
+    const Plan q = plan_of(&d.a, false);
     d.ckpt_out = ckpt;
-    d.chunks = (a->L + kChunk - 1) / kChunk;
     const int rc = begin(d, q, ws, s);
     if (rc) return rc;
     const KmbRows *rows[] = {&d.a.x, &d.a.gate_r, &d.a.gate_i, &d.a.y};
-    const bool vec = vectors(&d.a, rows, 4);
-    return a->type == KMB_BF16 ? launch_fwd<__nv_bfloat16>(d, q, vec, s) : launch_fwd<float>(d, q, vec, s);
+    return launch(d, q, false, vectors(&d.a, rows, 4), s);
 }
 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
@@ -961,12 +1535,11 @@ size_t align16(size_t n) { return (n + 15) / 16 * 16; }
  * one after the other) | sums of the tiles | checkpoints. */
 extern "C" size_t kmb_glr_scratch_bytes(const KmbGLR *a, int bwd) {
     if (a->batch == 0 || (a->L == 0 && !a->offsets)) return 0;
-    const size_t f = shown_bytes(plan(a, kFT));
+    const size_t f = shown_most(a, false);
     if (!bwd) return f;
-    const Plan q = plan(a, kBT);
-    const size_t b = shown_bytes(q);
+    const size_t b = shown_most(a, true);
     size_t n = align16(a->ckpt || f < b ? b : f);
-    if (a->ddecay) n += align16(4 * (size_t)q.tiles * q.chains * kC);
+    if (a->ddecay) n += align16(part_most(a));
     if (!a->ckpt) n += align16(4 * (size_t)kmb_glr_ckpt_elems(a));
     return n;
 }
@@ -988,21 +1561,18 @@ extern "C" int kmb_launch_glr_bwd(const KmbGLR *a, cudaStream_t s) {
                                                                             a->ddecay, a->accumulate);
         return done("glr: backward launch");
     }
-    const Plan q = plan(a, kBT);
-    const size_t f = shown_bytes(plan(a, kFT)), b = shown_bytes(q);
+    const size_t f = shown_most(a, false), b = shown_most(a, true);
     char *ws = (char *)a->workspace;
     size_t o = align16(a->ckpt || f < b ? b : f);
     Dev d = {};
     d.a = *a;
-    if (a->offsets)
-        d.a.x.batch_stride = d.a.gate_r.batch_stride = d.a.gate_i.batch_stride = d.a.dy.batch_stride =
-            d.a.dx.batch_stride = d.a.dgate_r.batch_stride = d.a.dgate_i.batch_stride = 0;
+    drop_batch(d.a);
+    const Plan q = plan_of(&d.a, true);
     if (a->ddecay) {
         d.part = (float *)(ws + o);
-        o += align16(4 * (size_t)q.tiles * q.chains * kC);
+        o += align16(part_most(a));
     }
     d.ckpt_in = a->ckpt;
-    d.chunks = (a->L + kChunk - 1) / kChunk;
     int rc;
     if (!a->ckpt) {
         d.ckpt_in = (float *)(ws + o);
@@ -1010,11 +1580,10 @@ extern "C" int kmb_launch_glr_bwd(const KmbGLR *a, cudaStream_t s) {
     }
     if ((rc = begin(d, q, ws, s))) return rc;
     const KmbRows *rows[] = {&d.a.x, &d.a.gate_r, &d.a.gate_i, &d.a.dy, &d.a.dx, &d.a.dgate_r, &d.a.dgate_i};
-    const bool vec = vectors(&d.a, rows, 7);
-    rc = a->type == KMB_BF16 ? launch_bwd<__nv_bfloat16>(d, q, vec, s) : launch_bwd<float>(d, q, vec, s);
+    rc = launch(d, q, true, vectors(&d.a, rows, 7), s);
     if (rc || !a->ddecay) return rc;
     k_glr_ddecay<<<(unsigned)((a->D + 31) / 32), dim3(32, 32), 0, s>>>(
-        d.part, q.tiles * q.batch, q.groups * kC, a->D, a->decay, a->ddecay, a->accumulate);
+        d.part, q.tiles * q.batch, q.groups * q.channels, a->D, a->decay, a->ddecay, a->accumulate);
     return done("glr: backward launch");
 }
 

@@ -19,7 +19,7 @@ static int sizes_ok(const KmbGLR *a) {
 
 long kmb_glr_ckpt_elems(const KmbGLR *a) {
     if (!sizes_ok(a)) return 0;
-    const long chunks = (a->L + KMB_GLR_CHUNK - 1) / KMB_GLR_CHUNK;
+    const long chunk = KMB_GLR_CHUNK(a->type), chunks = (a->L + chunk - 1) / chunk;
     return (a->offsets ? 1 : a->batch) * chunks * a->D;
 }
 

@@ -24,7 +24,6 @@ KMB_ETIMEOUT = -4
 KMB_EUNSUPPORTED = -5
 
 KMB_SCAN1D_CHUNK = 8
-KMB_GLR_CHUNK = 64
 
 # element types of KmbLayerNorm, KmbGLR and KmbGLRStep
 KMB_F32 = 0

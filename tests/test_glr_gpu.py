@@ -149,6 +149,70 @@ def test_many_tiles(lib, cuda, batch, L, D, dtype, kind):
     c.check(*c.ref(), ALL)
 
 
+# aligned tensors with more tiles than SMs: the resident kernels
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["mixed", "slow"])
+@pytest.mark.parametrize("batch,L,D", [(2, 1500, 512), (1, 5600, 516), (3, 1121, 260), (40, 113, 256), (1, 5599, 384),
+                                       (20, 57, 1032)])
+def test_resident_kernels(lib, cuda, batch, L, D, kind, dtype):
+    for gap in (0, 8):
+        c = Case(batch, L, D, dtype, seed=L, kind=kind, gap=gap)
+        run(lib, c, ckpt=gap == 0)
+        c.check(*c.ref(), ALL)
+
+
+def ragged(rng, n, total, gap=0):
+    cuts = np.sort(rng.integers(gap, total - gap + 1, n + 1))
+    return cuts.astype(np.int64)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [256, 516])
+@pytest.mark.parametrize("off,tail", [
+    ([0, 5600], 0), ([0, 5600], 1), ([0, 0, 56, 112, 112, 3000, 5599, 5600], 0), ([70, 71, 72, 4000, 5500], 117),
+    ([0, 28, 28, 84, 140, 141, 5600], 500), ("ragged", 300), ("many", 0)])
+def test_resident_kernels_packed(lib, cuda, off, tail, D, dtype):
+    """Sequences that begin and end at and inside tiles; rows of no sequence
+    before, behind and in whole tiles."""
+    rng = np.random.default_rng(D)
+    if off == "ragged":
+        off = ragged(rng, 30, 5700, 60)
+    elif off == "many":
+        off = np.concatenate([[0], np.cumsum(np.minimum(rng.geometric(0.05, 400) - 1, 90))])
+    c = Case(len(off) - 1, int(off[-1]) + tail, D, dtype, offsets=off, seed=D, kind="slow" if tail else "mixed")
+    run(lib, c)
+    c.check(*c.ref(), ALL)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_resident_kernels_in_place_and_same_bits(lib, cuda, packed):
+    for dtype in (F32, BF16):
+        off = [0, 100, 2900, 2900, 4000] if packed else None
+        mk = lambda: Case(4, 4000 if packed else 1000, 512, dtype, offsets=off, seed=9)  # noqa: E731
+        c = mk()
+        run(lib, c)
+        v, e = c.ref()
+        c.check(v, e, ALL)
+        first = {k: getattr(c, k).t.clone() for k in OUT} | {k: c.t[k].clone() for k in ("h_last", "dh0", "ddecay")}
+        for _ in range(4):
+            run(lib, c)
+            for k, t in first.items():
+                assert torch.equal(t, getattr(c, k).t if k in OUT else c.t[k]), k
+        d = mk()
+        a = d.args()
+        d.ckpt = torch.empty(lib.kmb_glr_ckpt_elems(byref(a)), device="cuda")
+        a.ckpt, a.dx, a.dgate_r, a.dgate_i = d.ckpt.data_ptr(), a.x, a.gate_r, a.gate_i
+        kb.check(lib, lib.kmb_glr_fwd(byref(a)))
+        kb.check(lib, lib.kmb_glr_bwd(byref(a)))
+        for k, o in (("dx", d.x), ("dgate_r", d.gate_r), ("dgate_i", d.gate_i)):
+            assert torch.equal(o.t, first[k]), k
+        d = mk()
+        a = d.args()
+        a.y = a.x
+        kb.check(lib, lib.kmb_glr_fwd(byref(a)))
+        assert torch.equal(d.x.t, first["y"])
+
+
 @pytest.mark.parametrize("ckpt,ws", [(False, True), (True, False), (False, False)])
 @pytest.mark.parametrize("offsets", [None, [0, 100, 100, 290]])
 def test_without_checkpoints_or_workspace(lib, cuda, ckpt, ws, offsets):

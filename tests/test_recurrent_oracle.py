@@ -145,8 +145,9 @@ def test_glr_sizes(lib):
     assert lib.kmb_glr_fwd(None) == kb.KMB_EINVAL and lib.kmb_glr_bwd(None) == kb.KMB_EINVAL
     assert lib.kmb_glr_fwd(C.byref(glr_args(batch=1 << 31))) == kb.KMB_EUNSUPPORTED
     assert lib.kmb_glr_fwd(C.byref(glr_args(batch=1 << 20, L=1 << 20))) == kb.KMB_EUNSUPPORTED
-    assert lib.kmb_glr_ckpt_elems(C.byref(glr_args(batch=3, L=65, D=7))) == 3 * 2 * 7
-    assert lib.kmb_glr_ckpt_elems(C.byref(glr_args(batch=3, L=65, D=7, offsets=BAD))) == 2 * 7
+    assert lib.kmb_glr_ckpt_elems(C.byref(glr_args(batch=3, L=65, D=7))) == 3 * 3 * 7
+    assert lib.kmb_glr_ckpt_elems(C.byref(glr_args(batch=3, L=57, D=7, type=kb.KMB_BF16))) == 3 * 2 * 7
+    assert lib.kmb_glr_ckpt_elems(C.byref(glr_args(batch=3, L=65, D=7, offsets=BAD))) == 3 * 7
     assert lib.kmb_glr_ckpt_elems(C.byref(glr_args(batch=3, L=0, D=7))) == 0
     assert lib.kmb_glr_ckpt_elems(C.byref(glr_args(D=-1))) == 0
     # a time-major output passes the overlap check (and then fails on the pointers)
