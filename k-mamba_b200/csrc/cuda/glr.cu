@@ -33,7 +33,9 @@
 
 namespace {
 
-constexpr int kWindow = 12; /* tiles before its own that a tile looks at */
+/* tiles before its own that a tile looks at: the kernels for any alignment,
+ * the resident ones */
+constexpr int kWindow = 12, kRingWindow = 16;
 constexpr unsigned kUnset = 0xffffffffu; /* workspace word not written yet */
 
 /* set when a wait gave up (kmb_glr_check_error) */
@@ -49,10 +51,6 @@ template <>
 struct Pack<2> {
     typedef float2 type;
 };
-template <>
-struct Pack<4> {
-    typedef float4 type;
-};
 
 template <int V>
 struct F {
@@ -67,9 +65,7 @@ __device__ __forceinline__ F<V> all(float v) {
     return r;
 }
 __device__ __forceinline__ F<2> from(float2 v) { return {{v}}; }
-__device__ __forceinline__ F<4> from(float4 v) { return {{kmb_f2(v.x, v.y), kmb_f2(v.z, v.w)}}; }
 __device__ __forceinline__ float2 to(F<2> a) { return a.p[0]; }
-__device__ __forceinline__ float4 to(F<4> a) { return make_float4(a.p[0].x, a.p[0].y, a.p[1].x, a.p[1].y); }
 template <int V>
 __device__ __forceinline__ F<V> operator+(F<V> a, F<V> b) {
 #pragma unroll
@@ -114,61 +110,50 @@ struct Raw<float, V> {
     static __device__ __forceinline__ type r(F<V> v) { return to(v); }
 };
 template <>
-struct Raw<__nv_bfloat16, 4> {
-    typedef uint2 type;
-    static __device__ __forceinline__ F<4> f(uint2 v) { return {{unpack(v.x), unpack(v.y)}}; }
-    static __device__ __forceinline__ uint2 r(F<4> v) { return make_uint2(pack(v.p[0]), pack(v.p[1])); }
-};
-template <>
 struct Raw<__nv_bfloat16, 2> {
     typedef unsigned type;
     static __device__ __forceinline__ F<2> f(unsigned v) { return {{unpack(v)}}; }
     static __device__ __forceinline__ unsigned r(F<2> v) { return pack(v.p[0]); }
 };
 
-/* A lane's four channels in global memory.  VEC: 4 lane .. 4 lane + 3 in one
- * access; else lane + 32 k, for odd widths, strides and addresses (every
- * access still covers a contiguous piece of the row).  m: bit k set where
- * channel k exists. */
-constexpr int kV = 4;
+/* A lane's two channels in global memory.  VEC: 2 lane and 2 lane + 1 in one
+ * access; else lane and lane + 32, for odd widths, strides and addresses
+ * (every access still covers a contiguous piece of the row).  m: bit k set
+ * where channel k exists. */
+constexpr int kV = 2;
 constexpr int kC = 32 * kV;
 
 template <bool VEC>
-__device__ __forceinline__ float4 load(const float *p, unsigned m) {
-    if (VEC) return m ? __ldcs(reinterpret_cast<const float4 *>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
-    return make_float4(m & 1 ? __ldcs(p) : 0.f, m & 2 ? __ldcs(p + 32) : 0.f, m & 4 ? __ldcs(p + 64) : 0.f,
-                       m & 8 ? __ldcs(p + 96) : 0.f);
+__device__ __forceinline__ float2 load(const float *p, unsigned m) {
+    if (VEC) return m ? __ldcs(reinterpret_cast<const float2 *>(p)) : make_float2(0.f, 0.f);
+    return make_float2(m & 1 ? __ldcs(p) : 0.f, m & 2 ? __ldcs(p + 32) : 0.f);
 }
 template <bool VEC>
-__device__ __forceinline__ uint2 load(const __nv_bfloat16 *p, unsigned m) {
-    if (VEC) return m ? __ldcs(reinterpret_cast<const uint2 *>(p)) : make_uint2(0u, 0u);
+__device__ __forceinline__ unsigned load(const __nv_bfloat16 *p, unsigned m) {
+    if (VEC) return m ? __ldcs(reinterpret_cast<const unsigned *>(p)) : 0u;
     const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
     const unsigned a = m & 1 ? __ldcs(q) : 0u, b = m & 2 ? __ldcs(q + 32) : 0u;
-    const unsigned c = m & 4 ? __ldcs(q + 64) : 0u, d = m & 8 ? __ldcs(q + 96) : 0u;
-    return make_uint2(a | b << 16, c | d << 16);
+    return a | b << 16;
 }
 template <bool VEC>
-__device__ __forceinline__ void store(float *p, F<4> v, unsigned m) {
+__device__ __forceinline__ void store(float *p, F<2> v, unsigned m) {
     if constexpr (VEC) {
-        if (m) __stcs(reinterpret_cast<float4 *>(p), to(v));
+        if (m) __stcs(reinterpret_cast<float2 *>(p), to(v));
     } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (m >> k & 1) __stcs(p + 32 * k, v[k]);
+        if (m & 1) __stcs(p, v[0]);
+        if (m & 2) __stcs(p + 32, v[1]);
     }
 }
 template <bool VEC>
-__device__ __forceinline__ void store(__nv_bfloat16 *p, F<4> v, unsigned m) {
-    const uint2 u = Raw<__nv_bfloat16, 4>::r(v);
-    if (VEC) {
-        if (m) __stcs(reinterpret_cast<uint2 *>(p), u);
-        return;
+__device__ __forceinline__ void store(__nv_bfloat16 *p, F<2> v, unsigned m) {
+    const unsigned u = Raw<__nv_bfloat16, 2>::r(v);
+    if constexpr (VEC) {
+        if (m) __stcs(reinterpret_cast<unsigned *>(p), u);
+    } else {
+        unsigned short *q = reinterpret_cast<unsigned short *>(p);
+        if (m & 1) __stcs(q, (unsigned short)u);
+        if (m & 2) __stcs(q + 32, (unsigned short)(u >> 16));
     }
-    unsigned short *q = reinterpret_cast<unsigned short *>(p);
-    if (m & 1) __stcs(q, (unsigned short)u.x);
-    if (m & 2) __stcs(q + 32, (unsigned short)(u.x >> 16));
-    if (m & 4) __stcs(q + 64, (unsigned short)u.y);
-    if (m & 8) __stcs(q + 96, (unsigned short)(u.y >> 16));
 }
 
 __device__ __forceinline__ float softplus(float v) { return v > 20.f ? v + expf(-v) : log1pf(expf(v)); }
@@ -280,15 +265,11 @@ __device__ __forceinline__ F<V> shrink(F<V> c, F<V> A) {
     return WEAK ? fma(c, A, A) : c * A;
 }
 
-/* Gradients of one row from G, what the row's state is worth, and hp, the
- * state before it. */
-template <int V>
-struct Grads {
-    F<V> x, r, i, udu;
-};
-
+/* What multiplies G, what the row's state is worth, in its gradients; hp is
+ * the state before it.  dx = G si; udu = G f; dgate_r = udu q; dgate_i = G i:
+ * q becomes 1 - r, i becomes b (1 - i). */
 template <bool WEAK, int V>
-__device__ __forceinline__ Grads<V> gradients(const Terms<V> &t, F<V> rate, F<V> x, F<V> G, F<V> hp) {
+__device__ __forceinline__ void factors(Terms<V> &t, F<V> rate, F<V> x, F<V> hp, F<V> &f) {
     const F<V> one = all<V>(1.f), minus = all<V>(-1.f);
     const F<V> r = t.q * t.q, u = rate * r, b = t.si * x;
     F<V> kappa = poly_kappa(u), ua; /* ua: -u a */
@@ -301,12 +282,9 @@ __device__ __forceinline__ Grads<V> gradients(const Terms<V> &t, F<V> rate, F<V>
             return u[n] <= kWeak ? kappa[n] : -ua[n] * t.c[n] * rcp_mufu(fmaf(-t.c[n], t.c[n], 1.f));
         });
     }
-    Grads<V> g;
-    g.udu = G * fma(ua, hp, kappa * b);
-    g.x = G * t.si;
-    g.r = g.udu * fma(r, minus, one);
-    g.i = G * b * fma(t.i, minus, one);
-    return g;
+    f = fma(ua, hp, kappa * b);
+    t.q = fma(r, minus, one);
+    t.i = b * fma(t.i, minus, one);
 }
 
 /* ------------------------------------------------------------------ */
@@ -345,15 +323,6 @@ struct Shown {
     long step;          /* lanes between places of a chain */
 };
 
-__device__ __forceinline__ bool peek(const float *p, F<4> &v) {
-    unsigned a, b, c, d;
-    asm volatile("ld.relaxed.gpu.global.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
-                 : "l"(p)
-                 : "memory");
-    v = {{kmb_f2(__uint_as_float(a), __uint_as_float(b)), kmb_f2(__uint_as_float(c), __uint_as_float(d))}};
-    return a != kUnset && b != kUnset && c != kUnset && d != kUnset;
-}
 __device__ __forceinline__ bool peek(const float *p, F<2> &v) {
     unsigned a, b;
     asm volatile("ld.relaxed.gpu.global.v2.u32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "l"(p) : "memory");
@@ -363,40 +332,62 @@ __device__ __forceinline__ bool peek(const float *p, F<2> &v) {
 __device__ __forceinline__ float not_unset(float v) {
     return __float_as_uint(v) == kUnset ? __uint_as_float(0x7fffffffu) : v;
 }
-__device__ __forceinline__ void show(float *p, F<4> v) {
-    asm volatile("st.relaxed.gpu.global.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(not_unset(v[0])),
-                 "f"(not_unset(v[1])), "f"(not_unset(v[2])), "f"(not_unset(v[3]))
-                 : "memory");
-}
 __device__ __forceinline__ void show(float *p, F<2> v) {
     asm volatile("st.relaxed.gpu.global.v2.f32 [%0], {%1, %2};" ::"l"(p), "f"(not_unset(v[0])),
                  "f"(not_unset(v[1]))
                  : "memory");
 }
 
-/* The map of a place, or as a constant one its final state: waits for
- * whichever comes first (last: for the final state).  Bounded by about 2^31
- * cycles; then the error word is set and later waits return at once. */
+template <int V>
+__device__ __forceinline__ void show(const Shown &s, long o, const Map<V> &m) {
+    show(s.A + o * V, m.A);
+    show(s.H + o * V, m.H);
+}
+
+/* whether the lane's maps are all constant ones */
+template <int V>
+__device__ __forceinline__ bool constant(F<V> A) {
+    bool c = true;
+#pragma unroll
+    for (int e = 0; e < V; ++e) c &= A[e] < 0.f;
+    return c;
+}
+
+/* The map of a place, or as a constant one its final state: whichever is
+ * there (last: the final state alone will do).  The three loads take one trip
+ * to the L2 cache together. */
+template <int V>
+__device__ __forceinline__ bool glance(const Shown &s, long o, bool last, Map<V> &m) {
+    F<V> end;
+    const bool done = peek(s.end + o * V, end);
+    const bool map = peek(s.A + o * V, m.A) & peek(s.H + o * V, m.H);
+    if (done) {
+        m.A = all<V>(-1.f);
+        m.H = end;
+    }
+    return done || (map && !last);
+}
+
+/* The same, waiting for it.  Bounded by about 2^31 cycles; then the error
+ * word is set and later waits return at once.  (The clock is read only when
+ * the first glances fail: it costs more than they do.) */
 template <int V>
 __device__ __forceinline__ Map<V> look(const Shown &s, long o, bool last) {
-    const long long t0 = clock64();
     Map<V> m;
-    for (int n = 0;; ++n) {
-        if (peek(s.end + o * V, m.H)) {
+    long long t0 = 0;
+    for (int n = 1; !glance(s, o, last, m); ++n) {
+        if (n % 64) continue;
+        const long long t = clock64();
+        if (n == 64) t0 = t;
+        const bool late = t - t0 > (1ll << 31);
+        if (late) atomicExch(&g_glr_error, 1);
+        if (late || *reinterpret_cast<volatile int *>(&g_glr_error)) {
             m.A = all<V>(-1.f);
+            m.H = all<V>(0.f);
             return m;
         }
-        if (!last && peek(s.A + o * V, m.A) && peek(s.H + o * V, m.H)) return m;
-        if ((n & 63) == 63) {
-            const bool late = clock64() - t0 > (1ll << 31);
-            if (late) atomicExch(&g_glr_error, 1);
-            if (late || *reinterpret_cast<volatile int *>(&g_glr_error)) {
-                m.A = all<V>(-1.f);
-                m.H = all<V>(0.f);
-                return m;
-            }
-        }
     }
+    return m;
 }
 
 /* ------------------------------------------------------------------ */
@@ -417,6 +408,7 @@ struct Dev {
     float *part;                    /* [tiles * chains][channels of a tile] sums of u dL/du */
     unsigned *ticket;
     Shown shown;
+    const float2 *rates;            /* of all groups' channels: rate, sqrt(2 rate) (resident kernels) */
 };
 
 struct Place {
@@ -539,6 +531,10 @@ struct Lane {
     __device__ __forceinline__ Lane(long ch0, long D) {
         lane = threadIdx.x % 32;
         d = ch0 + (VEC ? V * lane : lane);
+        if (VEC) { /* D is a multiple of V */
+            m = d < D ? (1u << V) - 1 : 0u;
+            return;
+        }
         m = 0;
 #pragma unroll
         for (int k = 0; k < V; ++k) m |= d + k * kNext < D ? 1u << k : 0u;
@@ -577,33 +573,13 @@ struct Maps {
     __device__ __forceinline__ Map<V> at(int w, int lane) const { return {from(A[w][lane]), from(H[w][lane])}; }
 };
 
-/* the CTA's barrier, or that of the first N threads */
-struct WholeCta {
-    static __device__ __forceinline__ void sync() { __syncthreads(); }
-};
-template <int N>
-struct FirstThreads {
-    static __device__ __forceinline__ void sync() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
-    static __device__ __forceinline__ bool any(bool p) {
-        int r;
-        asm volatile("{\n\t.reg .pred p, q;\n\t"
-                     "setp.ne.b32 p, %1, 0;\n\t"
-                     "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
-                     "selp.b32 %0, 1, 0, q;\n\t}"
-                     : "=r"(r)
-                     : "r"((int)p), "n"(N)
-                     : "memory");
-        return r != 0;
-    }
-};
-
 /* Joins the tile with the ones before it in its chain and returns the state
  * that enters it.  agg: the warps' maps, joined from the last when REVERSE;
- * first: the state that enters the chain. */
-template <typename Sync, bool VEC, bool MARKED, bool REVERSE, int W, int V>
+ * first: the state that enters the chain.  For kernels with one tile a CTA:
+ * every warp looks at other tiles, then all go through what was seen. */
+template <bool VEC, bool MARKED, bool REVERSE, int W, int N, int V>
 __device__ __forceinline__ F<V> enter_tile(const Dev &p, const Place &at, const Lane<VEC, V> &ln,
-                                           const Maps<W, V> &agg, Maps<kWindow, V> &seen, int warps,
-                                           const float *first) {
+                                           const Maps<W, V> &agg, Maps<N, V> &seen, int warps, const float *first) {
     const int warp = threadIdx.x / 32;
     F<V> h = ln.at(at.pos == 0 ? first : nullptr);
     if (p.tiles == 1) return h;
@@ -612,30 +588,54 @@ __device__ __forceinline__ F<V> enter_tile(const Dev &p, const Place &at, const 
     Map<V> m = {all<V>(1.f), all<V>(0.f)};
     if (warp == 0 && at.pos + 1 < p.tiles) {
         for (int k = 0; k < warps; ++k) m = join<MARKED>(m, agg.at(REVERSE ? warps - 1 - k : k, ln.lane));
-        if (at.pos > 0) {
-            show(s.A + o * V, m.A);
-            show(s.H + o * V, m.H);
-        }
+        if (at.pos > 0) show(s, o, m);
     }
     if (at.pos > 0) {
-        const int n = at.pos < kWindow ? (int)at.pos : kWindow;
-        for (int k = warp; k < n; k += warps) {
-            const Map<V> v = look<V>(s, o - (k + 1) * s.step, k == kWindow - 1);
+        const int n = at.pos < N ? (int)at.pos : N;
+        int k;
+        /* warp 0, which joins the tile's maps, comes last */
+        for (k = warp ? warp - 1 : warps - 1; k < n; k += warps) {
+            const Map<V> v = look<V>(s, o - (k + 1) * s.step, k == N - 1);
             seen.put(k, ln.lane, v.A, v.H);
         }
-        Sync::sync();
+        __syncthreads();
         /* from the nearest final states on; the first tile shows nothing else */
-        int k = 0;
-        for (; k < n - 1; ++k) {
-            const F<V> A = from(seen.A[k][ln.lane]);
-            bool constant = true;
-#pragma unroll
-            for (int e = 0; e < V; ++e) constant &= A[e] < 0.f;
-            if (constant) break;
-        }
+        for (k = 0; k < n - 1; ++k)
+            if (constant(from(seen.A[k][ln.lane]))) break;
         for (; k >= 0; --k) h = apply<true>(seen.at(k, ln.lane), h);
     }
     if (warp == 0 && at.pos + 1 < p.tiles) show(s.end + o * V, apply<MARKED>(m, h));
+    return h;
+}
+
+/*
+ * The same for the resident kernels, by one warp, while the others work or
+ * other CTAs do: m is the tile's map.  Most often the tile before has its
+ * final state, so places are looked at one by one; 8 at a time (24 loads
+ * under way) took 3300 cycles a tile, one 1900.
+ */
+template <bool MARKED, int N, int V>
+__device__ __forceinline__ F<V> enter_chain(const Dev &p, const Place &at, const Lane<true, V> &ln, const Map<V> &m,
+                                            Maps<N, V> &seen, const float *first) {
+    const Shown &s = p.shown;
+    const long o = at.pos * s.step + at.chain * 32 + ln.lane;
+    const bool next = at.pos + 1 < p.tiles; /* a tile waits for this one */
+    if (at.pos == 0) {
+        const F<V> h = ln.at(first);
+        if (next) show(s.end + o * V, apply<MARKED>(m, h));
+        return h;
+    }
+    if (next) show(s, o, m);
+    const int n = at.pos < N ? (int)at.pos : N;
+    int k = 0;
+    for (bool found = false; !found && k < n; ++k) {
+        const Map<V> v = look<V>(s, o - (k + 1) * s.step, k == N - 1);
+        seen.put(k, ln.lane, v.A, v.H);
+        found = __all_sync(~0u, constant(v.A));
+    }
+    F<V> h = all<V>(0.f);
+    while (--k >= 0) h = apply<true>(seen.at(k, ln.lane), h);
+    if (next) show(s.end + o * V, apply<MARKED>(m, h));
     return h;
 }
 
@@ -646,7 +646,7 @@ __device__ __forceinline__ F<V> enter_tile(const Dev &p, const Place &at, const 
 /*
  * What the forward and the backward do with a run of R rows; where the rows
  * come from and go to is the caller's: io.x(j), io.gr(j), io.gi(j), io.dy(j),
- * io.y(j, v), io.grads(j, g).  FULL: all rows exist and none begins or ends a
+ * io.y(j, v), io.grads(j, dx, dgate_r, dgate_i).  FULL: all rows exist and none begins or ends a
  * sequence.  Packed rows else look themselves up in `rows`.
  */
 template <typename Io, bool VEC, bool PACKED, bool FULL, bool WEAK, int R, int ROWS, int V>
@@ -674,37 +674,37 @@ struct RunOf {
         if (v) ln.put(v + rows.seq[warp * R + j] * p.a.D, x);
     }
 
-    template <typename Sync, int W>
-    __device__ __forceinline__ void forward(const Rates<V> &rt, Maps<W, V> &agg, Maps<kWindow, V> &seen, int warps) {
-        F<V> c[R], b[R];
+    /* The forward before the state that enters is known: decays and input
+     * terms of the rows, and the run's map. */
+    __device__ __forceinline__ Map<V> forward_map(const Rates<V> &rt, F<V> (&c)[R], F<V> (&b)[R]) const {
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             const Terms<V> t = terms<WEAK>(io.gr(j), io.gi(j), rt);
             c[j] = t.c;
             b[j] = t.si * io.x(j);
         }
-        F<V> A = all<V>(1.f), H = all<V>(0.f);
+        Map<V> m = {all<V>(1.f), all<V>(0.f)};
         bool fresh = false; /* a sequence begins in this run */
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             if (in(j)) {
                 if (begins(j)) {
-                    H = of(p.a.h0, j);
+                    m.H = of(p.a.h0, j);
                     fresh = true;
                 }
-                H = advance<WEAK>(c[j], H, b[j]);
-                A = shrink<WEAK>(c[j], A);
+                m.H = advance<WEAK>(c[j], m.H, b[j]);
+                m.A = shrink<WEAK>(c[j], m.A);
             }
         }
-        agg.put(warp, ln.lane, fresh ? all<V>(-1.f) : A, H);
-        Sync::sync();
-        const float *first = !PACKED && p.a.h0 ? p.a.h0 + at.b * p.a.D : nullptr;
-        F<V> h = enter_tile<Sync, VEC, PACKED, false>(p, at, ln, agg, seen, warps, first);
-        for (int w = 0; w < warp; ++w) h = apply<PACKED>(agg.at(w, ln.lane), h);
+        if (fresh) m.A = all<V>(-1.f);
+        return m;
+    }
+    /* h: the state that enters the run */
+    __device__ __forceinline__ void forward_rows(F<V> h, const F<V> (&c)[R], const F<V> (&b)[R]) const {
         /* the run's row with a checkpoint, if any */
         constexpr int chunk = Io::kChunk;
-        static_assert(chunk >= R, "one checkpoint a run");
-        const int mark = p.ckpt_out ? (int)((row0 + chunk - 1) / chunk * chunk - row0) : -1;
+        static_assert(chunk >= R, "at most one checkpoint a run");
+        const int mark = p.ckpt_out ? Io::mark(row0, warp) : -1;
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             if (in(j)) {
@@ -718,16 +718,14 @@ struct RunOf {
         if (!PACKED && p.a.h_last && live > 0 && row0 + live == p.a.L) ln.put(p.a.h_last + at.b * p.a.D, h);
     }
 
-    /* The adjoint that reaches row t - 1 from row t is C_t = a_t (dy_t +
-     * C_{t+1}).  entry: the state before the tile.  Returns the sum of udu. */
-    template <typename Sync, int W>
-    __device__ __forceinline__ F<V> backward(const Rates<V> &rt, F<V> entry, Maps<W, V> &states, Maps<W, V> &agg,
-                                             Maps<kWindow, V> &seen, int warps) {
-        const F<V> zero = all<V>(0.f), minus = all<V>(-1.f);
-        Terms<V> t[R];
+    /* The backward, likewise: the terms of the rows and the run's maps, of
+     * the states and of the adjoint.  The adjoint that reaches row t - 1 from
+     * row t is C_t = a_t (dy_t + C_{t+1}). */
+    __device__ __forceinline__ void backward_maps(const Rates<V> &rt, Terms<V> (&t)[R], Map<V> &state,
+                                                  Map<V> &adjoint) const {
 #pragma unroll
         for (int j = 0; j < R; ++j) t[j] = terms<WEAK>(io.gr(j), io.gi(j), rt);
-        F<V> A = all<V>(1.f), H = zero, K = zero;
+        F<V> A = all<V>(1.f), H = all<V>(0.f), K = H;
         bool fresh = false, closed = false;
 #pragma unroll
         for (int j = 0; j < R; ++j) {
@@ -740,7 +738,6 @@ struct RunOf {
                 A = shrink<WEAK>(t[j].c, A);
             }
         }
-        states.put(warp, ln.lane, fresh ? minus : A, H);
 #pragma unroll
         for (int j = R - 1; j >= 0; --j) {
             if (in(j)) {
@@ -751,31 +748,31 @@ struct RunOf {
                 K = shrink<WEAK>(t[j].c, K + io.dy(j));
             }
         }
-        agg.put(warp, ln.lane, closed ? minus : A, K);
-        Sync::sync();
-        const float *last = !PACKED && p.a.dh_last ? p.a.dh_last + at.b * p.a.D : nullptr;
-        F<V> C = enter_tile<Sync, VEC, PACKED, true>(p, at, ln, agg, seen, warps, last);
-        for (int w = warps - 1; w > warp; --w) C = apply<PACKED>(agg.at(w, ln.lane), C);
-        F<V> hp[R]; /* the states before each row */
-        {
-            F<V> h = entry;
-            for (int w = 0; w < warp; ++w) h = apply<PACKED>(states.at(w, ln.lane), h);
+        state = {fresh ? all<V>(-1.f) : A, H};
+        adjoint = {closed ? all<V>(-1.f) : A, K};
+    }
+    /* h: the state that enters the run.  Leaves in t what the gradients are
+     * when a row's adjoint is one: c, si (dx) as they were, q (dgate_r over
+     * udu), i (dgate_i), and udu in f. */
+    __device__ __forceinline__ void backward_factors(F<V> h, F<V> rate, Terms<V> (&t)[R], F<V> (&f)[R]) const {
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
-                if (begins(j)) h = of(p.a.h0, j);
-                hp[j] = h;
-                h = advance<WEAK>(t[j].c, h, t[j].si * io.x(j));
-            }
+        for (int j = 0; j < R; ++j) {
+            if (begins(j)) h = of(p.a.h0, j);
+            const F<V> x = io.x(j), hp = h;
+            h = advance<WEAK>(t[j].c, h, t[j].si * x);
+            factors<WEAK>(t[j], rate, x, hp, f[j]);
         }
-        F<V> sum = zero;
+    }
+    /* C: the adjoint that reaches the run.  Returns the sum of udu. */
+    __device__ __forceinline__ F<V> backward_rows(F<V> C, const Terms<V> (&t)[R], const F<V> (&f)[R]) const {
+        F<V> sum = all<V>(0.f);
 #pragma unroll
         for (int j = R - 1; j >= 0; --j) {
             if (in(j)) {
                 if (ends(j)) C = of(p.a.dh_last, j);
-                const F<V> G = C + io.dy(j);
-                const Grads<V> g = gradients<WEAK>(t[j], rt.rate, io.x(j), G, hp[j]);
-                sum = sum + g.udu;
-                io.grads(j, g);
+                const F<V> G = C + io.dy(j), udu = G * f[j];
+                sum = sum + udu;
+                io.grads(j, G * t[j].si, udu * t[j].q, G * t[j].i);
                 C = shrink<WEAK>(t[j].c, G);
                 if (begins(j)) put(p.a.dh0, j, C);
             }
@@ -811,7 +808,7 @@ template <int W, int ROWS, bool PACKED>
 struct AnyShared {
     Maps<W, kV> agg;
     Maps<kWindow, kV> seen;
-    float4 rate[32], sroot[32];
+    typename Pack<kV>::type rate[32], sroot[32];
     unsigned slot;
     RowMap<PACKED ? ROWS : 1> rows;
 };
@@ -829,6 +826,9 @@ constexpr int kFR = 8, kFW = 8, kFT = kFR * kFW;
 template <typename T, bool VEC>
 struct AnyFwdIo {
     static constexpr int kChunk = chunk_of<T>;
+    static __device__ __forceinline__ int mark(long row0, int) {
+        return (int)((row0 + kChunk - 1) / kChunk * kChunk - row0);
+    }
     typename Raw<T, kV>::type rx[kFR], rr[kFR], ri[kFR];
     Run<T> out;
     unsigned m;
@@ -840,8 +840,24 @@ struct AnyFwdIo {
     }
 };
 
+template <bool WEAK, typename T, bool VEC, bool PACKED>
+__device__ __forceinline__ void any_forward(const Dev &p, const Place &at, const Lane<VEC, kV> &ln,
+                                            AnyShared<kFW, kFT, PACKED> &sh, AnyFwdIo<T, VEC> &io,
+                                            const Rates<kV> &rt, long row0, int live, int warp) {
+    const RunOf<AnyFwdIo<T, VEC>, VEC, PACKED, false, WEAK, kFR, PACKED ? kFT : 1, kV> run = {
+        p, at, ln, sh.rows, io, row0, live, warp};
+    F<kV> c[kFR], b[kFR];
+    const Map<kV> m = run.forward_map(rt, c, b);
+    sh.agg.put(warp, ln.lane, m.A, m.H);
+    __syncthreads();
+    const float *first = !PACKED && p.a.h0 ? p.a.h0 + at.b * p.a.D : nullptr;
+    F<kV> h = enter_tile<VEC, PACKED, false>(p, at, ln, sh.agg, sh.seen, blockDim.x / 32, first);
+    for (int w = 0; w < warp; ++w) h = apply<PACKED>(sh.agg.at(w, ln.lane), h);
+    run.forward_rows(h, c, b);
+}
+
 template <typename T, bool VEC, bool PACKED>
-__global__ void __launch_bounds__(kFW * 32, 2) k_glr_fwd(const __grid_constant__ Dev p) {
+__global__ void __launch_bounds__(kFW * 32, 3) k_glr_fwd(const __grid_constant__ Dev p) {
     __shared__ AnyShared<kFW, kFT, PACKED> sh;
     const int warp = threadIdx.x / 32;
     const Place at(p, tile_id(p, &sh.slot));
@@ -869,35 +885,33 @@ __global__ void __launch_bounds__(kFW * 32, 2) k_glr_fwd(const __grid_constant__
     }
     const bool strong = make_rates<VEC>(p.a, ch0, (float *)sh.rate, (float *)sh.sroot);
     const Rates<kV> rt = {from(sh.rate[ln.lane]), from(sh.sroot[ln.lane])};
-    constexpr int ROWS = PACKED ? kFT : 1;
-    if (strong) {
-        RunOf<AnyFwdIo<T, VEC>, VEC, PACKED, false, false, kFR, ROWS, kV> run = {p, at, ln, sh.rows, io, row0, live, warp};
-        run.template forward<WholeCta>(rt, sh.agg, sh.seen, blockDim.x / 32);
-    } else {
-        RunOf<AnyFwdIo<T, VEC>, VEC, PACKED, false, true, kFR, ROWS, kV> run = {p, at, ln, sh.rows, io, row0, live, warp};
-        run.template forward<WholeCta>(rt, sh.agg, sh.seen, blockDim.x / 32);
-    }
+    if (strong) any_forward<false, T, VEC, PACKED>(p, at, ln, sh, io, rt, row0, live, warp);
+    else any_forward<true, T, VEC, PACKED>(p, at, ln, sh, io, rt, row0, live, warp);
     if (PACKED && at.pos == 0 && !p.states_only)
         empty_sequences(p.a, p.a.h0, p.a.h_last, ch0, ch0 + kC, warp, blockDim.x / 32);
 }
 
-constexpr int kBR = 4, kBW = 14, kBT = kBR * kBW;
-static_assert(kBT % KMB_GLR_CHUNK(KMB_F32) == 0 && kBT % KMB_GLR_CHUNK(KMB_BF16) == 0,
+constexpr int kBW = 7;
+template <typename T>
+constexpr int kBR = sizeof(T) == 2 ? 8 : 4;
+template <typename T>
+constexpr int kBT = kBR<T> * kBW;
+static_assert(kBT<float> % KMB_GLR_CHUNK(KMB_F32) == 0 && kBT<__nv_bfloat16> % KMB_GLR_CHUNK(KMB_BF16) == 0,
               "a backward tile begins at a checkpoint");
 
 template <typename T, bool VEC>
 struct AnyBwdIo {
-    typename Raw<T, kV>::type rx[kBR], rr[kBR], ri[kBR], rd[kBR];
+    typename Raw<T, kV>::type rx[kBR<T>], rr[kBR<T>], ri[kBR<T>], rd[kBR<T>];
     Run<T> dx, dgr, dgi;
     unsigned m;
     __device__ __forceinline__ F<kV> x(int j) const { return Raw<T, kV>::f(rx[j]); }
     __device__ __forceinline__ F<kV> gr(int j) const { return Raw<T, kV>::f(rr[j]); }
     __device__ __forceinline__ F<kV> gi(int j) const { return Raw<T, kV>::f(ri[j]); }
     __device__ __forceinline__ F<kV> dy(int j) const { return Raw<T, kV>::f(rd[j]); }
-    __device__ __forceinline__ void grads(int j, const Grads<kV> &g) const {
-        store<VEC>(dx[j], g.x, m);
-        store<VEC>(dgr[j], g.r, m);
-        store<VEC>(dgi[j], g.i, m);
+    __device__ __forceinline__ void grads(int j, F<kV> x, F<kV> r, F<kV> i) const {
+        store<VEC>(dx[j], x, m);
+        store<VEC>(dgr[j], r, m);
+        store<VEC>(dgi[j], i, m);
     }
 };
 
@@ -906,16 +920,38 @@ struct AnyBwdShared : AnyShared<W, ROWS, PACKED> {
     Maps<W, kV> states;
 };
 
+template <bool WEAK, typename T, bool VEC, bool PACKED>
+__device__ __forceinline__ F<kV> any_backward(const Dev &p, const Place &at, const Lane<VEC, kV> &ln,
+                                              AnyBwdShared<kBW, kBT<T>, PACKED> &sh, AnyBwdIo<T, VEC> &io,
+                                              const Rates<kV> &rt, F<kV> entry, long row0, int live, int warp) {
+    const int warps = blockDim.x / 32;
+    const RunOf<AnyBwdIo<T, VEC>, VEC, PACKED, false, WEAK, kBR<T>, PACKED ? kBT<T> : 1, kV> run = {
+        p, at, ln, sh.rows, io, row0, live, warp};
+    Terms<kV> t[kBR<T>];
+    Map<kV> state, adjoint;
+    run.backward_maps(rt, t, state, adjoint);
+    sh.states.put(warp, ln.lane, state.A, state.H);
+    sh.agg.put(warp, ln.lane, adjoint.A, adjoint.H);
+    __syncthreads();
+    F<kV> f[kBR<T>];
+    for (int w = 0; w < warp; ++w) entry = apply<PACKED>(sh.states.at(w, ln.lane), entry);
+    run.backward_factors(entry, rt.rate, t, f);
+    const float *last = !PACKED && p.a.dh_last ? p.a.dh_last + at.b * p.a.D : nullptr;
+    F<kV> C = enter_tile<VEC, PACKED, true>(p, at, ln, sh.agg, sh.seen, warps, last);
+    for (int w = warps - 1; w > warp; --w) C = apply<PACKED>(sh.agg.at(w, ln.lane), C);
+    return run.backward_rows(C, t, f);
+}
+
 template <typename T, bool VEC, bool PACKED>
-__global__ void __launch_bounds__(kBW * 32, 1) k_glr_bwd(const __grid_constant__ Dev p) {
-    __shared__ AnyBwdShared<kBW, kBT, PACKED> sh;
+__global__ void __launch_bounds__(kBW * 32, 2) k_glr_bwd(const __grid_constant__ Dev p) {
+    __shared__ AnyBwdShared<kBW, kBT<T>, PACKED> sh;
     const int warp = threadIdx.x / 32, warps = blockDim.x / 32;
     const Place at(p, tile_id(p, &sh.slot));
     const long ch0 = (long)at.group * kC;
     const Lane<VEC, kV> ln(ch0, p.a.D);
-    const long tile0 = (long)(p.tiles - 1 - at.pos) * kBT, row0 = tile0 + warp * kBR;
+    const long tile0 = (long)(p.tiles - 1 - at.pos) * kBT<T>, row0 = tile0 + warp * kBR<T>;
     const long left = p.a.L - row0;
-    const int live = left < 0 ? 0 : left < kBR ? (int)left : kBR;
+    const int live = left < 0 ? 0 : left < kBR<T> ? (int)left : kBR<T>;
     if (PACKED) {
         if (warp == 0) map_rows(sh.rows, p.a, tile0);
         __syncthreads();
@@ -926,8 +962,8 @@ __global__ void __launch_bounds__(kBW * 32, 1) k_glr_bwd(const __grid_constant__
         const Run<const T> pr(p.a.gate_r, at.b, row0, ln.d), pi(p.a.gate_i, at.b, row0, ln.d),
             px(p.a.x, at.b, row0, ln.d), pd(p.a.dy, at.b, row0, ln.d);
 #pragma unroll
-        for (int j = 0; j < kBR; ++j) {
-            const unsigned m = (PACKED ? sh.rows.seq[warp * kBR + j] >= 0 : j < live) ? ln.m : 0u;
+        for (int j = 0; j < kBR<T>; ++j) {
+            const unsigned m = (PACKED ? sh.rows.seq[warp * kBR<T> + j] >= 0 : j < live) ? ln.m : 0u;
             io.rr[j] = load<VEC>(pr[j], m);
             io.ri[j] = load<VEC>(pi[j], m);
             io.rx[j] = load<VEC>(px[j], m);
@@ -937,15 +973,8 @@ __global__ void __launch_bounds__(kBW * 32, 1) k_glr_bwd(const __grid_constant__
     const F<kV> entry = ln.at(tile0 < p.a.L ? p.ckpt_in + (at.b * p.chunks + tile0 / chunk_of<T>) * p.a.D : nullptr);
     const bool strong = make_rates<VEC>(p.a, ch0, (float *)sh.rate, (float *)sh.sroot);
     const Rates<kV> rt = {from(sh.rate[ln.lane]), from(sh.sroot[ln.lane])};
-    constexpr int ROWS = PACKED ? kBT : 1;
-    F<kV> sum;
-    if (strong) {
-        RunOf<AnyBwdIo<T, VEC>, VEC, PACKED, false, false, kBR, ROWS, kV> run = {p, at, ln, sh.rows, io, row0, live, warp};
-        sum = run.template backward<WholeCta>(rt, entry, sh.states, sh.agg, sh.seen, warps);
-    } else {
-        RunOf<AnyBwdIo<T, VEC>, VEC, PACKED, false, true, kBR, ROWS, kV> run = {p, at, ln, sh.rows, io, row0, live, warp};
-        sum = run.template backward<WholeCta>(rt, entry, sh.states, sh.agg, sh.seen, warps);
-    }
+    const F<kV> sum = strong ? any_backward<false, T, VEC, PACKED>(p, at, ln, sh, io, rt, entry, row0, live, warp)
+                             : any_backward<true, T, VEC, PACKED>(p, at, ln, sh, io, rt, entry, row0, live, warp);
     if (p.part) {
         __syncthreads(); /* every warp is done with the states' maps */
         sh.states.H[warp][ln.lane] = to(sum);
@@ -965,57 +994,100 @@ __global__ void __launch_bounds__(kBW * 32, 1) k_glr_bwd(const __grid_constant__
 /* ------------------------------------------------------------------ */
 
 /*
- * For tensors that tensor copies can take, and more tiles than the GPU holds
- * at once.  Two CTAs an SM stay for the whole call.  Their last warp takes
- * tickets, brings the next tile into the other stage of a ring of two while
- * the others work on theirs, prepares what depends on the channel (rates,
- * the checkpoint) or the row (which sequence), and stores results, which the
- * working warps leave in place of the inputs that they came from.  The
- * working warps thus read and write shared memory only, at fixed offsets.
- * 56 rows x 128 channels of bf16 x 3 tensors are 42 KB: 84 KB of an SM's
- * inputs are on their way at any time.  Seven working warps: with the eighth,
- * two CTAs have 128 registers a thread (a ninth would leave 96, and spills).
+ * For tensors that tensor copies can take, and enough tiles to fill the GPU.
+ * Two or three CTAs an SM stay for the whole call.  Their last warp, the
+ * feeder, takes tickets, brings tiles into a ring of stages by tensor copies,
+ * prepares what depends on the channel (rates, the checkpoint) or the row
+ * (which sequence), and stores the results, which the seven workers leave in
+ * place of the inputs that they came from.  The workers own a run of rows
+ * each, in shared memory at fixed offsets; the first of them also finds the
+ * state that enters the tile, meanwhile the others (in the backward) work out
+ * the states of their rows and all of the gradients but the factor that comes
+ * along the chain.
+ *
+ * What bounds them: issue and latency.  A tile's terms are 23 instructions a
+ * value in the forward (4 of them MUFU), and the trips to the L2 cache along
+ * the chain are hidden by the other CTAs of the SM only.  Tried and left: four
+ * channels a lane (128 registers, two CTAs; 130 against 105 us on 8 x 4096 x
+ * 1536 bf16), a warp of its own for the chain with the next tile's terms
+ * ahead (113), all warps looking at other tiles (111).
  */
-constexpr int kW = 7;              /* working warps */
-constexpr int kWork = 32 * kW;
+constexpr int kW = 7; /* workers */
+constexpr int kThreads = 32 * (kW + 1);
 
 template <typename T, bool BWD>
 struct Shape {
     static constexpr bool kHalf = sizeof(T) == 2;
-    static constexpr int V = !BWD && kHalf ? 4 : 2;   /* channels of a lane */
-    static constexpr int R = BWD && !kHalf ? 4 : 8;   /* rows of a warp */
+    static constexpr int V = 2;                      /* channels of a lane */
+    static constexpr int R = BWD && !kHalf ? 4 : 8;  /* rows of a worker */
     static constexpr int C = 32 * V, ROWS = R * kW;
-    static constexpr int N = BWD ? 4 : 3;             /* tensors in */
+    static constexpr int N = BWD ? 4 : 3;            /* tensors in */
     static constexpr int kTile = ROWS * C * (int)sizeof(T); /* bytes of one */
     static constexpr int kStage = N * kTile;
+    static constexpr int kStages = 2;
+    static constexpr int kCtas = BWD || !kHalf ? 2 : 3; /* an SM's: 128 or 80 registers a thread */
 };
-
 static_assert(Shape<float, true>::ROWS % KMB_GLR_CHUNK(KMB_F32) == 0 &&
                   Shape<__nv_bfloat16, true>::ROWS % KMB_GLR_CHUNK(KMB_BF16) == 0,
-              "a backward tile begins at a checkpoint");
+              "a tile begins at a checkpoint");
 
 struct TensorMaps {
     CUtensorMap in[4], out[3]; /* x, gate_r, gate_i, dy; y or dx, dgate_r, dgate_i */
 };
 
 template <typename T, bool BWD, bool PACKED>
-struct Stage { /* what the last warp prepares beside the tile */
+struct Stage { /* what the feeder prepares beside the tile, and the sums that it takes away */
     typedef Shape<T, BWD> S;
-    typename Pack<S::V>::type rate[32], sroot[32], entry[32];
-    unsigned id;
+    typedef typename Pack<S::V>::type pack;
+    pack rate[32], sroot[32], entry[32];
+    Place at;
+    int row, ch0; /* the tile's first */
     int strong, more;
     RowMap<PACKED ? S::ROWS : 1> rows;
+    pack sums[BWD ? kW : 1][32];
+    uint64_t full, done;
 };
 
 template <typename T, bool BWD, bool PACKED>
 struct RingShared {
     typedef Shape<T, BWD> S;
-    Maps<kW, S::V> agg;
-    Maps<BWD ? kW : 1, S::V> states;
-    Maps<kWindow, S::V> seen;
-    Stage<T, BWD, PACKED> stage[2];
-    uint64_t full[2], done[2];
+    Stage<T, BWD, PACKED> stage[S::kStages];
+    Maps<kW, S::V> agg, states; /* the workers' maps, of the recurrence and (backward) of the states */
+    Maps<kRingWindow, S::V> seen;
+    typename Pack<S::V>::type in[32]; /* what enters the tile */
 };
+
+/* barrier 1: the workers; 2: the first warp arrives, the others wait */
+struct Workers {
+    static __device__ __forceinline__ void sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kW) : "memory"); }
+    static __device__ __forceinline__ bool any(bool p) {
+        int r;
+        asm volatile("{\n\t.reg .pred p, q;\n\t"
+                     "setp.ne.b32 p, %1, 0;\n\t"
+                     "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
+                     "selp.b32 %0, 1, 0, q;\n\t}"
+                     : "=r"(r)
+                     : "r"((int)p), "n"(32 * kW)
+                     : "memory");
+        return r != 0;
+    }
+    static __device__ __forceinline__ void entered() { asm volatile("bar.arrive 2, %0;" ::"n"(32 * kW) : "memory"); }
+    static __device__ __forceinline__ void enter() { asm volatile("bar.sync 2, %0;" ::"n"(32 * kW) : "memory"); }
+};
+
+/* a stage and the parity of its barriers' phase */
+template <int N>
+struct Turn {
+    int k = 0, parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++k == N) {
+            k = 0;
+            parity ^= 1;
+        }
+    }
+};
+
+__device__ __forceinline__ bool wait(uint64_t *bar, int parity) { return kmb_mbar_wait(bar, parity, &g_glr_error); }
 
 __device__ __forceinline__ void tensor_load(void *dst, const CUtensorMap *m, int x, int y, int z, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
@@ -1032,93 +1104,108 @@ __device__ __forceinline__ void tensor_store(const CUtensorMap *m, int x, int y,
 template <typename T, bool BWD, bool PACKED>
 __device__ __forceinline__ void feed(const Dev &p, const TensorMaps &tm, char *tiles, RingShared<T, BWD, PACKED> &sh) {
     typedef Shape<T, BWD> S;
+    constexpr int N = S::kStages;
     const int lane = threadIdx.x % 32;
     const unsigned total = p.tiles * p.chains;
-    const auto first_row = [&](const Place &at) {
-        return (int)((BWD ? p.tiles - 1 - at.pos : at.pos) * (unsigned)S::ROWS);
-    };
-    /* the results of the tile in stage k leave it; false when a wait gave up */
-    const auto leave = [&](int k, int parity) {
-        if (!kmb_mbar_wait(&sh.done[k], parity, &g_glr_error)) return false;
-        if (!p.states_only && (!PACKED || sh.stage[k].rows.whole) && lane == 0) {
-            const Place at(p, sh.stage[k].id);
-            char *tile = tiles + k * S::kStage;
+    /* the results of the tile in a stage leave it; false when a wait gave up */
+    const auto leave = [&](const Turn<N> &t) {
+        Stage<T, BWD, PACKED> &st = sh.stage[t.k];
+        if (!wait(&st.done, t.parity)) return false;
+        if (!p.states_only && (!PACKED || st.rows.whole) && lane == 0) {
+            char *tile = tiles + t.k * S::kStage;
             for (int n = 0; n < (BWD ? 3 : 1); ++n)
-                tensor_store(&tm.out[n], (int)at.group * S::C, first_row(at), (int)at.b, tile + n * S::kTile);
+                tensor_store(&tm.out[n], st.ch0, st.row, (int)st.at.b, tile + n * S::kTile);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         }
+        if (BWD && p.part) {
+            F<S::V> v = all<S::V>(0.f);
+            for (int w = 0; w < kW; ++w) v = v + from(st.sums[BWD ? w : 0][lane]);
+            typedef typename Pack<S::V>::type pack;
+            *reinterpret_cast<pack *>(p.part + ((long)st.at.pos * p.chains + st.at.chain) * S::C + S::V * lane) = to(v);
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
         return true;
     };
-    int n = 0;
+    Turn<N> turn, out; /* the stage to fill, the oldest one that is in work */
+    int held = 0;      /* stages filled */
     bool ok = true;
-    for (;; ++n) {
-        const int k = n & 1;
-        Stage<T, BWD, PACKED> &st = sh.stage[k];
-        if (n >= 2 && !(ok = leave(k, ((n >> 1) - 1) & 1))) break;
+    for (;;) {
+        if (held == N) {
+            if (!(ok = leave(out))) break;
+            out.next();
+            --held;
+        }
+        Stage<T, BWD, PACKED> &st = sh.stage[turn.k];
+        /* not before the stage is free: a tile that is held and not in work
+         * keeps those behind it in the chain waiting */
         unsigned id = 0;
         if (lane == 0) id = take_ticket(p);
         id = __shfl_sync(~0u, id, 0);
         if (id >= total) {
             if (lane == 0) {
                 st.more = 0;
-                kmb_mbar_arrive(&sh.full[k]);
-                kmb_mbar_arrive(&sh.full[k]);
+                kmb_mbar_arrive(&st.full);
+                kmb_mbar_arrive(&st.full);
             }
             break;
         }
         const Place at(p, id);
-        const int row = first_row(at), ch0 = (int)at.group * S::C;
+        const int row = (int)((BWD ? p.tiles - 1 - at.pos : at.pos) * (unsigned)S::ROWS), ch0 = (int)at.group * S::C;
         if (lane == 0) {
-            char *tile = tiles + k * S::kStage;
-            kmb_mbar_expect(&sh.full[k], S::kStage);
-            /* the gates first: work begins with them */
-            const int order[4] = {1, 2, 0, 3};
-            for (int t = 0; t < S::N; ++t)
-                tensor_load(tile + order[t] * S::kTile, &tm.in[order[t]], ch0, row, (int)at.b, &sh.full[k]);
-            st.id = id;
+            char *tile = tiles + turn.k * S::kStage;
+            kmb_mbar_expect(&st.full, S::kStage);
+            for (int n = 0; n < S::N; ++n)
+                tensor_load(tile + n * S::kTile, &tm.in[n], ch0, row, (int)at.b, &st.full);
+            st.at = at;
+            st.row = row;
+            st.ch0 = ch0;
             st.more = 1;
         }
         const Lane<true, S::V> ln(ch0, p.a.D);
-        const F<S::V> decay = ln.at(p.a.decay);
+        float2 rs[S::V];
+#pragma unroll
+        for (int e = 0; e < S::V; ++e) rs[e] = p.rates[ch0 + S::V * lane + e];
         bool strong = false;
-        const F<S::V> rate = each<S::V>([&](int e) {
-            const float r = ln.m >> e & 1 ? p.a.scale * softplus(decay[e]) : 0.f;
-            strong |= !(r <= kWeak);
-            return r;
-        });
-        st.rate[lane] = to(rate);
-        st.sroot[lane] = to(each<S::V>([&](int e) { return sqrtf(2.f * rate[e]); }));
+#pragma unroll
+        for (int e = 0; e < S::V; ++e) strong |= !(rs[e].x <= kWeak);
+        st.rate[lane] = to(each<S::V>([&](int e) { return rs[e].x; }));
+        st.sroot[lane] = to(each<S::V>([&](int e) { return rs[e].y; }));
         if (BWD) st.entry[lane] = to(ln.at(row < p.a.L ? p.ckpt_in + (at.b * p.chunks + row / chunk_of<T>) * p.a.D : nullptr));
         strong = __any_sync(~0u, strong);
         if (lane == 0) st.strong = strong;
         if constexpr (PACKED) map_rows(st.rows, p.a, row);
         __syncwarp();
-        if (lane == 0) kmb_mbar_arrive(&sh.full[k]);
+        if (lane == 0) kmb_mbar_arrive(&st.full);
+        turn.next();
+        ++held;
     }
-    if (ok && n >= 1) ok = leave((n - 1) & 1, ((n - 1) >> 1) & 1);
+    for (; ok && held; --held, out.next()) ok = leave(out);
     if (!ok) { /* copies that may still be under way land before the CTA ends, or a second goes by */
         const long long t0 = clock64();
-        for (int m = n > 1 ? n - 2 : 0; m <= n; ++m)
-            while (!kmb_mbar_done(&sh.full[m & 1], (m >> 1) & 1) && clock64() - t0 < (1ll << 31)) {
+        for (; held; --held, out.next())
+            while (!kmb_mbar_done(&sh.stage[out.k].full, out.parity) && clock64() - t0 < (1ll << 31)) {
             }
     }
 }
 
-/* the lane's channels of the tile in shared memory, rows of the warp's run */
+/* the lane's channels of the tile in shared memory, rows of the worker's run */
 template <typename T, bool BWD>
 struct TileIo {
     typedef Shape<T, BWD> S;
-    [[maybe_unused]] static constexpr int kChunk = chunk_of<T>;
     typedef Raw<T, S::V> W;
     typedef typename W::type raw;
+    static constexpr int kChunk = chunk_of<T>;
+    static_assert(S::ROWS % kChunk == 0, "a tile begins at a checkpoint");
     raw *base;     /* row 0 of the run in the first tensor */
     const Dev *p;  /* rows go to global memory themselves when some are of no sequence */
     long b, row0;
     int lane_ch;   /* the lane's first channel */
     unsigned m;
     bool direct, skip;
+    static __device__ __forceinline__ int mark(long, int warp) { /* a tile begins at a checkpoint */
+        return (kChunk - warp * S::R % kChunk) % kChunk;
+    }
     __device__ __forceinline__ raw *at(int n, int j) const {
         return base + (n * S::kTile + j * S::C * (int)sizeof(T)) / (int)sizeof(raw);
     }
@@ -1136,101 +1223,148 @@ struct TileIo {
     __device__ __forceinline__ void y(int j, F<S::V> v) const {
         if (!skip) out(0, j, v, p->a.y);
     }
-    __device__ __forceinline__ void grads(int j, const Grads<S::V> &g) const {
-        out(0, j, g.x, p->a.dx);
-        out(1, j, g.r, p->a.dgate_r);
-        out(2, j, g.i, p->a.dgate_i);
+    __device__ __forceinline__ void grads(int j, F<S::V> x, F<S::V> r, F<S::V> i) const {
+        out(0, j, x, p->a.dx);
+        out(1, j, r, p->a.dgate_r);
+        out(2, j, i, p->a.dgate_i);
     }
 };
 
-template <typename T, bool BWD, bool PACKED, bool FULL, bool WEAK>
-__device__ __forceinline__ void work(const Dev &p, const Place &at, TileIo<T, BWD> &io, RingShared<T, BWD, PACKED> &sh,
-                                     int k, const Lane<true, Shape<T, BWD>::V> &ln, long row0, int live, int warp) {
-    typedef Shape<T, BWD> S;
-    typedef FirstThreads<kWork> Sync;
-    const Stage<T, BWD, PACKED> &st = sh.stage[k];
-    const Rates<S::V> rt = {from(st.rate[ln.lane]), from(st.sroot[ln.lane])};
-    RunOf<TileIo<T, BWD>, true, PACKED, FULL, WEAK, S::R, PACKED ? S::ROWS : 1, S::V> run = {p,  at,   ln,   st.rows,
-                                                                                             io, row0, live, warp};
-    if constexpr (BWD) {
-        const F<S::V> sum = run.template backward<Sync>(rt, from(st.entry[ln.lane]), sh.states, sh.agg, sh.seen, kW);
-        if (p.part) {
-            Sync::sync(); /* every warp is done with the states' maps */
-            sh.states.H[warp][ln.lane] = to(sum);
-            Sync::sync();
-            if (threadIdx.x < S::C) {
-                float v = 0.f;
-                for (int w = 0; w < kW; ++w) v += ((const float *)sh.states.H[w])[threadIdx.x];
-                p.part[((long)at.pos * p.chains + at.chain) * S::C + threadIdx.x] = v;
-            }
-        }
+template <bool B>
+struct Const {};
+/* f(Const<FULL>, Const<WEAK>) for the tile's kind */
+template <typename Fn>
+__device__ __forceinline__ void by_kind(bool full, bool strong, Fn f) {
+    if (strong) {
+        if (full) f(Const<true>(), Const<false>());
+        else f(Const<false>(), Const<false>());
     } else {
-        run.template forward<Sync>(rt, sh.agg, sh.seen, kW);
+        if (full) f(Const<true>(), Const<true>());
+        else f(Const<false>(), Const<true>());
     }
 }
 
+/* A worker's place in a tile. */
 template <typename T, bool BWD, bool PACKED>
-__global__ void __launch_bounds__(kWork + 32, 2) k_glr_ring(const __grid_constant__ Dev p,
-                                                            const __grid_constant__ TensorMaps tm) {
+struct Bench {
     typedef Shape<T, BWD> S;
-    extern __shared__ __align__(128) char tiles[];
-    RingShared<T, BWD, PACKED> &sh = *reinterpret_cast<RingShared<T, BWD, PACKED> *>(tiles + 2 * S::kStage);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (threadIdx.x == 0) {
-        for (int k = 0; k < 2; ++k) {
-            kmb_mbar_init(&sh.full[k], 2);
-            kmb_mbar_init(&sh.done[k], kW);
-        }
-        kmb_mbar_init_fence();
-    }
-    __syncthreads();
-    if (warp == kW) {
-        feed(p, tm, tiles, sh);
-        return;
-    }
-    for (int n = 0;; ++n) {
-        const int k = n & 1;
-        const bool ok = kmb_mbar_wait(&sh.full[k], (n >> 1) & 1, &g_glr_error);
-        /* all or none go on; also, every warp is done with the maps of the tile before */
-        if (FirstThreads<kWork>::any(!ok)) return;
-        const Stage<T, BWD, PACKED> &st = sh.stage[k];
-        if (!st.more) return;
-        const Place at(p, st.id);
-        const long ch0 = (long)at.group * S::C;
-        const Lane<true, S::V> ln(ch0, p.a.D);
-        const long tile0 = (long)(BWD ? p.tiles - 1 - at.pos : at.pos) * S::ROWS, row0 = tile0 + warp * S::R;
-        const long left = p.a.L - row0;
-        const int live = left < 0 ? 0 : left < S::R ? (int)left : S::R;
-        bool full = tile0 + S::ROWS <= p.a.L, direct = false;
+    static constexpr int V = S::V, R = S::R;
+    const Dev &p;
+    Stage<T, BWD, PACKED> &st;
+    Lane<true, V> ln;
+    TileIo<T, BWD> io;
+    Place at;
+    int worker, live;
+    bool full;
+
+    __device__ __forceinline__ Bench(const Dev &d, char *tile, Stage<T, BWD, PACKED> &s, int w)
+        : p(d), st(s), ln(s.ch0, d.a.D), at(s.at), worker(w) {
+        const int row0 = st.row + worker * R, left = (int)p.a.L - row0;
+        live = left < 0 ? 0 : left < R ? left : R;
+        full = st.row + S::ROWS <= p.a.L;
+        io.direct = false;
         if constexpr (PACKED) {
             full = st.rows.plain;
-            direct = !st.rows.whole;
+            io.direct = !st.rows.whole;
         }
-        TileIo<T, BWD> io;
-        io.base = reinterpret_cast<typename TileIo<T, BWD>::raw *>(tiles + k * S::kStage +
-                                                                   (warp * S::R * S::C + lane * S::V) * (int)sizeof(T));
+        io.base = reinterpret_cast<typename TileIo<T, BWD>::raw *>(tile + (worker * R * S::C + ln.lane * V) * (int)sizeof(T));
         io.p = &p;
         io.b = at.b;
         io.row0 = row0;
         io.lane_ch = (int)ln.d;
         io.m = ln.m;
-        io.direct = direct;
         io.skip = p.states_only;
-        if (st.strong) {
-            if (full) work<T, BWD, PACKED, true, false>(p, at, io, sh, k, ln, row0, live, warp);
-            else work<T, BWD, PACKED, false, false>(p, at, io, sh, k, ln, row0, live, warp);
-        } else {
-            if (full) work<T, BWD, PACKED, true, true>(p, at, io, sh, k, ln, row0, live, warp);
-            else work<T, BWD, PACKED, false, true>(p, at, io, sh, k, ln, row0, live, warp);
-        }
-        if (PACKED && tile0 == 0 && !p.states_only) {
-            if (BWD) empty_sequences(p.a, p.a.dh_last, p.a.dh0, ch0, ch0 + S::C, warp, kW);
-            else empty_sequences(p.a, p.a.h0, p.a.h_last, ch0, ch0 + S::C, warp, kW);
-        }
+    }
+    template <bool FULL, bool WEAK>
+    using Rows = RunOf<TileIo<T, BWD>, true, PACKED, FULL, WEAK, R, PACKED ? S::ROWS : 1, V>;
+    template <bool FULL, bool WEAK>
+    __device__ __forceinline__ Rows<FULL, WEAK> run(Const<FULL>, Const<WEAK>) {
+        return {p, at, ln, st.rows, io, io.row0, live, worker};
+    }
+    __device__ __forceinline__ Rates<V> rates() const { return {from(st.rate[ln.lane]), from(st.sroot[ln.lane])}; }
+    /* by the first worker, when all maps are there */
+    __device__ __forceinline__ void enter(RingShared<T, BWD, PACKED> &sh) {
+        Map<V> m = sh.agg.at(BWD ? kW - 1 : 0, ln.lane);
+        for (int k = 1; k < kW; ++k) m = join<PACKED>(m, sh.agg.at(BWD ? kW - 1 - k : k, ln.lane));
+        const float *first = BWD ? p.a.dh_last : p.a.h0;
+        first = !PACKED && first ? first + at.b * p.a.D : nullptr;
+        sh.in[ln.lane] = to(enter_chain<PACKED>(p, at, ln, m, sh.seen, first));
+        Workers::entered();
+    }
+    __device__ __forceinline__ void finish() {
+        if (PACKED && st.row == 0 && !p.states_only)
+            empty_sequences(p.a, BWD ? p.a.dh_last : p.a.h0, BWD ? p.a.dh0 : p.a.h_last, st.ch0, st.ch0 + S::C, worker, kW);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); /* the results, for the tensor stores */
         __syncwarp();
-        if (lane == 0) kmb_mbar_arrive(&sh.done[k]);
+        if (ln.lane == 0) kmb_mbar_arrive(&st.done);
     }
+};
+
+template <typename T, bool BWD, bool PACKED>
+__device__ __forceinline__ void work(const Dev &p, char *tiles, RingShared<T, BWD, PACKED> &sh, int worker) {
+    typedef Shape<T, BWD> S;
+    constexpr int V = S::V, R = S::R;
+    for (Turn<S::kStages> t;; t.next()) {
+        Stage<T, BWD, PACKED> &st = sh.stage[t.k];
+        /* all go on or none; and all are done with the maps of the tile before */
+        if (Workers::any(!wait(&st.full, t.parity)) || !st.more) return;
+        Bench<T, BWD, PACKED> bench(p, tiles + t.k * S::kStage, st, worker);
+        const int lane = bench.ln.lane;
+        by_kind(bench.full, st.strong, [&](auto full, auto weak) {
+            const auto run = bench.run(full, weak);
+            if constexpr (BWD) {
+                Terms<V> x[R];
+                F<V> f[R];
+                {
+                    Map<V> state, adjoint;
+                    run.backward_maps(bench.rates(), x, state, adjoint);
+                    sh.states.put(worker, lane, state.A, state.H);
+                    sh.agg.put(worker, lane, adjoint.A, adjoint.H);
+                }
+                Workers::sync();
+                if (worker == 0) bench.enter(sh);
+                F<V> h = from(st.entry[lane]);
+                for (int w = 0; w < worker; ++w) h = apply<PACKED>(sh.states.at(w, lane), h);
+                run.backward_factors(h, from(st.rate[lane]), x, f);
+                if (worker != 0) Workers::enter();
+                F<V> C = from(sh.in[lane]);
+                for (int w = kW - 1; w > worker; --w) C = apply<PACKED>(sh.agg.at(w, lane), C);
+                st.sums[worker][lane] = to(run.backward_rows(C, x, f));
+            } else {
+                F<V> c[R], b[R];
+                {
+                    const Map<V> m = run.forward_map(bench.rates(), c, b);
+                    sh.agg.put(worker, lane, m.A, m.H);
+                }
+                Workers::sync();
+                if (worker == 0) bench.enter(sh);
+                else Workers::enter();
+                F<V> h = from(sh.in[lane]);
+                for (int w = 0; w < worker; ++w) h = apply<PACKED>(sh.agg.at(w, lane), h);
+                run.forward_rows(h, c, b);
+            }
+        });
+        bench.finish();
+    }
+}
+
+template <typename T, bool BWD, bool PACKED>
+__global__ void __launch_bounds__(kThreads, (Shape<T, BWD>::kCtas)) k_glr_ring(const __grid_constant__ Dev p,
+                                                                           const __grid_constant__ TensorMaps tm) {
+    typedef Shape<T, BWD> S;
+    extern __shared__ __align__(128) char tiles[];
+    RingShared<T, BWD, PACKED> &sh = *reinterpret_cast<RingShared<T, BWD, PACKED> *>(tiles + S::kStages * S::kStage);
+    const int warp = threadIdx.x / 32;
+    if (threadIdx.x == 0) {
+        for (int k = 0; k < S::kStages; ++k) {
+            kmb_mbar_init(&sh.stage[k].full, 2);
+            kmb_mbar_init(&sh.stage[k].done, kW);
+        }
+        kmb_mbar_init_fence();
+    }
+    __syncthreads();
+    if (warp == kW) feed(p, tm, tiles, sh);
+    else work(p, tiles, sh, warp);
 }
 
 /* ddecay: the sums of all tiles and sequences, 32 columns a CTA, 32 rows of
@@ -1252,6 +1386,18 @@ __global__ void __launch_bounds__(1024) k_glr_ddecay(const float *part, long row
     if (tx == 0 && e < D) {
         t *= decay_ratio(decay[e]);
         ddecay[e] = acc ? ddecay[e] + t : t;
+    }
+}
+
+/* Before a call whose chains have several tiles: fills the shown arrays and
+ * the ticket, and works out the channels' rates (0 beyond the last). */
+__global__ void __launch_bounds__(256) k_glr_begin(uint4 *fill, long n, float2 *rates, long channels, long D,
+                                                   const float *decay, float scale) {
+    const long at = (long)blockIdx.x * 256 + threadIdx.x, step = (long)gridDim.x * 256;
+    for (long k = at; k < n; k += step) fill[k] = make_uint4(kUnset, kUnset, kUnset, kUnset);
+    for (long c = at; c < channels; c += step) {
+        const float r = c < D ? scale * softplus(decay[c]) : 0.f;
+        rates[c] = make_float2(r, sqrtf(2.f * r));
     }
 }
 
@@ -1307,8 +1453,8 @@ int done(const char *what) {
     return e == cudaSuccess ? KMB_OK : kmb_cuda_fail(e, what);
 }
 
-/* Whether the tensors allow four channels an access: width, strides and
- * addresses are multiples of four elements. */
+/* Whether the tensors allow two channels an access: width, strides and
+ * addresses are multiples of two elements. */
 bool vectors(const KmbGLR *a, const KmbRows *const *rows, int n) {
     const size_t es = a->type == KMB_BF16 ? 2 : 4;
     if (a->D % kV) return false;
@@ -1361,11 +1507,11 @@ bool tensor_ok(const KmbGLR *a, const KmbRows &r) {
  */
 template <typename T>
 Plan plan_of(const KmbGLR *a, bool bwd) {
-    const Plan any = bwd ? plan(a, kBT, kC) : plan(a, kFT, kC);
+    const Plan any = bwd ? plan(a, kBT<T>, kC) : plan(a, kFT, kC);
     const KmbRows fwd_rows[] = {a->x, a->gate_r, a->gate_i, a->y};
     const KmbRows bwd_rows[] = {a->x, a->gate_r, a->gate_i, a->dy, a->dx, a->dgate_r, a->dgate_i};
     Plan q = bwd ? plan(a, Shape<T, true>::ROWS, Shape<T, true>::C) : plan(a, Shape<T, false>::ROWS, Shape<T, false>::C);
-    if (a->D % kV || a->L >= (1L << 31) - 1024 || q.tiles < 2 || q.tiles * q.chains < kSMs) return any;
+    if (a->D % 4 || a->L >= (1L << 31) - 1024 || q.tiles < 2 || q.tiles * q.chains < kSMs) return any;
     if (q.tiles * q.chains >= (1L << 31)) return any;
     for (int i = 0; i < (bwd ? 7 : 4); ++i) {
         const KmbRows &r = bwd ? bwd_rows[i] : fwd_rows[i];
@@ -1380,11 +1526,11 @@ Plan plan_of(const KmbGLR *a, bool bwd) {
 
 constexpr size_t kHead = 64; /* bytes before the shown arrays: the ticket */
 
-size_t shown_bytes(const Plan &q) { return q.words ? kHead + 12 * q.words : 0; }
+size_t shown_bytes(const Plan &q) { return q.words ? kHead + 12 * q.words + 8 * (size_t)q.groups * q.channels : 0; }
 /* for either kernel, whatever the pointers turn out to be */
 size_t shown_most(const KmbGLR *a, bool bwd) {
     const bool half = a->type == KMB_BF16;
-    const Plan any = bwd ? plan(a, kBT, kC) : plan(a, kFT, kC);
+    const Plan any = bwd ? plan(a, half ? kBT<__nv_bfloat16> : kBT<float>, kC) : plan(a, kFT, kC);
     const Plan ring = bwd ? (half ? plan(a, Shape<__nv_bfloat16, true>::ROWS, Shape<__nv_bfloat16, true>::C)
                                   : plan(a, Shape<float, true>::ROWS, Shape<float, true>::C))
                           : (half ? plan(a, Shape<__nv_bfloat16, false>::ROWS, Shape<__nv_bfloat16, false>::C)
@@ -1393,7 +1539,7 @@ size_t shown_most(const KmbGLR *a, bool bwd) {
     return m > n ? m : n;
 }
 size_t part_most(const KmbGLR *a) {
-    const Plan any = plan(a, kBT, kC);
+    const Plan any = plan(a, a->type == KMB_BF16 ? kBT<__nv_bfloat16> : kBT<float>, kC);
     const Plan ring = a->type == KMB_BF16 ? plan(a, Shape<__nv_bfloat16, true>::ROWS, Shape<__nv_bfloat16, true>::C)
                                           : plan(a, Shape<float, true>::ROWS, Shape<float, true>::C);
     const size_t m = (size_t)any.tiles * any.chains * kC, n = (size_t)ring.tiles * ring.chains * ring.channels;
@@ -1409,8 +1555,14 @@ int begin(Dev &d, const Plan &q, void *ws, cudaStream_t s) {
     const long chunk = KMB_GLR_CHUNK(d.a.type);
     d.chunks = (d.a.L + chunk - 1) / chunk;
     if (!q.words) return KMB_OK;
-    const cudaError_t e = cudaMemsetAsync(ws, 0xff, shown_bytes(q), s);
-    if (e != cudaSuccess) return kmb_cuda_fail(e, "glr: workspace fill");
+    const long n = (long)(kHead + 12 * q.words) / 16, channels = q.ring ? q.groups * q.channels : 0;
+    float2 *rates = (float2 *)((char *)ws + kHead + 12 * q.words);
+    const long blocks = ((n > channels ? n : channels) + 255) / 256;
+    k_glr_begin<<<(unsigned)(blocks < 8 * kSMs ? blocks : 8 * kSMs), 256, 0, s>>>((uint4 *)ws, n, rates, channels,
+                                                                                 d.a.D, d.a.decay, d.a.scale);
+    const int rc = done("glr: launch");
+    if (rc) return rc;
+    d.rates = rates;
     d.ticket = (unsigned *)ws;
     d.shown.A = (float *)((char *)ws + kHead);
     d.shown.H = d.shown.A + q.words;
@@ -1458,11 +1610,12 @@ template <typename T, bool BWD, bool PACKED>
 int launch_ring(const Dev &d, const Plan &q, const TensorMaps &tm, cudaStream_t s) {
     typedef Shape<T, BWD> S;
     auto k = k_glr_ring<T, BWD, PACKED>;
-    const size_t bytes = 2 * S::kStage + sizeof(RingShared<T, BWD, PACKED>);
+    const size_t bytes = S::kStages * S::kStage + sizeof(RingShared<T, BWD, PACKED>);
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != cudaSuccess) return kmb_cuda_fail(e, "glr: shared memory");
     const long n = q.tiles * q.chains;
-    k<<<(unsigned)(n < 2 * kSMs ? n : 2 * kSMs), kWork + 32, bytes, s>>>(d, tm);
+    const long most = (long)S::kCtas * kSMs;
+    k<<<(unsigned)(n < most ? n : most), kThreads, bytes, s>>>(d, tm);
     return done("glr: launch");
 }
 
@@ -1486,7 +1639,7 @@ int launch(const Dev &d, const Plan &q, bool bwd, bool vec, cudaStream_t s) {
     }
     const unsigned n = (unsigned)(q.tiles * q.chains);
     const int most = bwd ? kBW : kFW;
-    const long runs = (d.a.L + (bwd ? kBR : kFR) - 1) / (bwd ? kBR : kFR);
+    const long run = bwd ? kBR<T> : kFR, runs = (d.a.L + run - 1) / run;
     const unsigned threads = 32u * (unsigned)(runs < 1 ? 1 : runs < most ? runs : most);
     if (bwd) {
         auto k = packed ? (vec ? k_glr_bwd<T, true, true> : k_glr_bwd<T, false, true>)

@@ -40,16 +40,16 @@ __device__ __forceinline__ bool kmb_mbar_done(uint64_t *bar, uint32_t parity) {
  * is set, and later waits of the launch give up at once.  False when it gave
  * up. */
 __device__ __forceinline__ bool kmb_mbar_wait(uint64_t *bar, uint32_t parity, int *error) {
-    if (kmb_mbar_done(bar, parity)) return true;
-    const long long t0 = clock64();
-    for (int n = 1;; ++n) {
-        if (kmb_mbar_done(bar, parity)) return true;
-        if ((n & 15) == 0) {
-            const bool late = clock64() - t0 > (1ll << 31);
-            if (late) atomicExch(error, 1);
-            if (late || *reinterpret_cast<volatile int *>(error)) return false;
-        }
+    long long t0 = 0;
+    for (int n = 1; !kmb_mbar_done(bar, parity); ++n) {
+        if (n % 16) continue;
+        const long long t = clock64();
+        if (n == 16) t0 = t;
+        const bool late = t - t0 > (1ll << 31);
+        if (late) atomicExch(error, 1);
+        if (late || *reinterpret_cast<volatile int *>(error)) return false;
     }
+    return true;
 }
 
 /* `bytes` (a multiple of 16, both addresses 16-byte aligned) from global to
