@@ -1413,35 +1413,77 @@ __global__ void k_glr_copy(const float *from, float *to, long n) {
 
 constexpr int kStepThreads = 128;
 
-/* a row whose slot an earlier row names is left out */
-template <typename T>
-__global__ void __launch_bounds__(kStepThreads) k_glr_step(KmbGLRStep a, long tiles) {
-    const long k = blockIdx.x / tiles;
-    const long slot = a.slots ? a.slots[k] : k;
+/*
+ * A thread has W channels of a row (4 where the tensors allow vectors).  A
+ * row whose slot an earlier row names is left out: the threads of the CTA
+ * look for it among the slots before, while their channels are on their way.
+ * Memory bounds it, and for a handful of rows the trips to memory: slot, then
+ * state.
+ */
+template <typename T, int W>
+__global__ void __launch_bounds__(kStepThreads) k_glr_step(const __grid_constant__ KmbGLRStep a, unsigned tiles) {
+    const unsigned k = blockIdx.x / tiles;
+    const long slot = a.slots ? a.slots[k] : (long)k;
     if (slot < 0 || slot >= a.n_states) return;
-    int taken = 0;
-    if (a.slots)
-        for (long j = threadIdx.x; j < k; j += kStepThreads) taken |= a.slots[j] == slot;
-    if (__syncthreads_or(taken)) return;
-    const long d = (blockIdx.x - k * tiles) * kStepThreads + threadIdx.x;
-    if (d >= a.D) return;
-    const float rate = a.scale * softplus(a.decay[d]);
-    const Rates<2> rt = {all<2>(rate), all<2>(sqrtf(2.f * rate))};
-    const T *px = (const T *)a.x.data + k * a.x.row_stride + d;
-    const T *pr = (const T *)a.gate_r.data + k * a.gate_r.row_stride + d;
-    const T *pi = (const T *)a.gate_i.data + k * a.gate_i.row_stride + d;
-    const F<2> gr = all<2>((float)*pr), gi = all<2>((float)*pi), x = all<2>((float)*px);
+    const long d = ((long)(blockIdx.x - k * tiles) * kStepThreads + threadIdx.x) * W;
+    const bool in = d < a.D;
+    float x[W], gr[W], gi[W], h[W], rate[W];
+    const auto fetch = [&](const KmbRows &r, float (&v)[W]) {
+        const T *p = (const T *)r.data + k * r.row_stride + d;
+        if constexpr (W == 1) {
+            v[0] = (float)*p;
+        } else if constexpr (sizeof(T) == 4) {
+            const float4 u = __ldcs(reinterpret_cast<const float4 *>(p));
+            v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+        } else {
+            const uint2 u = __ldcs(reinterpret_cast<const uint2 *>(p));
+            const float2 l = unpack(u.x), m = unpack(u.y);
+            v[0] = l.x, v[1] = l.y, v[2] = m.x, v[3] = m.y;
+        }
+    };
     float *s = a.state + slot * a.ld_state + d;
-    float h = *s;
-    if (rate <= kWeak) {
-        const Terms<2> t = terms<true>(gr, gi, rt);
-        h = advance<true>(t.c, all<2>(h), t.si * x)[0];
-    } else {
-        const Terms<2> t = terms<false>(gr, gi, rt);
-        h = advance<false>(t.c, all<2>(h), t.si * x)[0];
+    if (in) {
+        fetch(a.gate_r, gr);
+        fetch(a.gate_i, gi);
+        fetch(a.x, x);
+        if constexpr (W == 4) {
+            const float4 u = *reinterpret_cast<const float4 *>(s);
+            h[0] = u.x, h[1] = u.y, h[2] = u.z, h[3] = u.w;
+        } else {
+            h[0] = *s;
+        }
+#pragma unroll
+        for (int e = 0; e < W; ++e) rate[e] = a.scale * softplus(a.decay[d + e]);
     }
-    *s = h;
-    ((T *)a.y.data)[k * a.y.row_stride + d] = (T)h;
+    if (a.slots) {
+        int taken = 0;
+        for (unsigned j = threadIdx.x; j < k; j += kStepThreads) taken |= a.slots[j] == slot;
+        if (__syncthreads_or(taken)) return;
+    }
+    if (!in) return;
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+        const Rates<2> rt = {all<2>(rate[e]), all<2>(sqrtf(2.f * rate[e]))};
+        if (rate[e] <= kWeak) {
+            const Terms<2> t = terms<true>(all<2>(gr[e]), all<2>(gi[e]), rt);
+            h[e] = advance<true>(t.c, all<2>(h[e]), t.si * all<2>(x[e]))[0];
+        } else {
+            const Terms<2> t = terms<false>(all<2>(gr[e]), all<2>(gi[e]), rt);
+            h[e] = advance<false>(t.c, all<2>(h[e]), t.si * all<2>(x[e]))[0];
+        }
+    }
+    T *y = (T *)a.y.data + k * a.y.row_stride + d;
+    if constexpr (W == 1) {
+        *s = h[0];
+        *y = (T)h[0];
+    } else {
+        *reinterpret_cast<float4 *>(s) = make_float4(h[0], h[1], h[2], h[3]);
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4 *>(y) = make_float4(h[0], h[1], h[2], h[3]);
+        } else {
+            *reinterpret_cast<uint2 *>(y) = make_uint2(pack(kmb_f2(h[0], h[1])), pack(kmb_f2(h[2], h[3])));
+        }
+    }
 }
 
 /* ------------------------------------------------------------------ */
@@ -1740,15 +1782,24 @@ extern "C" int kmb_launch_glr_bwd(const KmbGLR *a, cudaStream_t s) {
     return done("glr: backward launch");
 }
 
-extern "C" int kmb_launch_glr_step(const KmbGLRStep *a, cudaStream_t s) {
-    const long tiles = (a->D + kStepThreads - 1) / kStepThreads;
+template <typename T>
+static int launch_step(const KmbGLRStep *a, cudaStream_t s) {
+    const long es = sizeof(T);
+    bool vec = a->D % 4 == 0 && (size_t)a->state % 16 == 0 && a->ld_state % 4 == 0;
+    for (const KmbRows *r : {&a->x, &a->gate_r, &a->gate_i, &a->y})
+        vec = vec && (size_t)r->data % (4 * es) == 0 && r->row_stride % 4 == 0;
+    /* a few rows are a matter of latency: one channel a thread */
+    if (a->rows * a->D < 4L * kSMs * kStepThreads) vec = false;
+    const long per = kStepThreads * (vec ? 4 : 1), tiles = (a->D + per - 1) / per;
     if (a->rows >= (1L << 31) / tiles) return kmb_fail(KMB_EUNSUPPORTED, "glr: too many rows");
     const unsigned n = (unsigned)(a->rows * tiles);
-    if (a->type == KMB_BF16)
-        k_glr_step<__nv_bfloat16><<<n, kStepThreads, 0, s>>>(*a, tiles);
-    else
-        k_glr_step<float><<<n, kStepThreads, 0, s>>>(*a, tiles);
+    if (vec) k_glr_step<T, 4><<<n, kStepThreads, 0, s>>>(*a, (unsigned)tiles);
+    else k_glr_step<T, 1><<<n, kStepThreads, 0, s>>>(*a, (unsigned)tiles);
     return done("glr: step launch");
+}
+
+extern "C" int kmb_launch_glr_step(const KmbGLRStep *a, cudaStream_t s) {
+    return a->type == KMB_BF16 ? launch_step<__nv_bfloat16>(a, s) : launch_step<float>(a, s);
 }
 
 /* KMB_ETIMEOUT (and the word cleared) when a wait between tiles gave up

@@ -447,7 +447,8 @@ def test_prefill_then_steps(lib, cuda):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows,D,gap,shift", [(0, 8, 0, 0), (1, 1, 0, 0), (1, 1024, 0, 0), (3, 130, 2, 1), (64, 300, 0, 0),
-                                              (301, 64, 1, 0), (700, 96, 0, 0)])
+                                              (301, 64, 1, 0), (700, 96, 0, 0), (64, 1284, 0, 0),
+                                              (64, 1284, 4, 0), (64, 1284, 1, 0)])
 def test_step_slots(lib, cuda, rows, D, gap, shift, dtype):
     """Padded rows (negative, beyond the table) are left out, and of the rows
     that name one slot only the first is taken."""
