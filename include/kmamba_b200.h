@@ -457,7 +457,7 @@ int kmb_glr_check_error(void);
  * slots NULL: state k), which is advanced by one step in place and written
  * to y.  A row whose slot is negative or >= n_states (padding) is left out:
  * nothing of it is read or written.  Of several rows that name one slot
- * the first is taken and the others are left out.
+ * the first is taken, and nothing of the others is written.
  */
 typedef struct {
     KmbRows x;

@@ -36,6 +36,15 @@
  *   W_a [d, d], W_z [d, d], W_out [d, d], W_p [35, d], dt_bias [3, d],
  *   A_log [3, d, 16], conv_kernel [27, d], conv_bias [d].
  * Gradients (kmb_ndmodel_grads) use the same layout.
+ *
+ * Pre-norm models (kmb_ndmodel_create_prenorm) normalise the residual
+ * stream on its way into the projections and into the head,
+ *   a = LN_l(x) W_a^T, z = LN_l(x) W_z^T;   logits = LN_L(x) H^T
+ * with layer norms of their own (kmb_layernorm_fwd / _bwd, kmamba_b200.h):
+ * fp32 rows in, bf16 GEMM operands out, and in the backward the gradient of
+ * the residual path joined in the same pass.  Their parameters follow the
+ * layers': weight [d], bias [d] of norm 0 .. n_layers (the last one before
+ * the head), ones and zeros at first.
  */
 
 #include <stddef.h>
@@ -59,6 +68,9 @@ typedef struct KmbNDModel KmbNDModel;
 
 /* NULL on invalid configuration or allocation failure (kmb_last_error). */
 KmbNDModel *kmb_ndmodel_create(const KmbNDModelConfig *cfg);
+/* The same with a layer norm before each block and before the head;
+ * norm_eps > 0 (NULL otherwise). */
+KmbNDModel *kmb_ndmodel_create_prenorm(const KmbNDModelConfig *cfg, float norm_eps);
 void kmb_ndmodel_free(KmbNDModel *m);
 
 long kmb_ndmodel_param_count(const KmbNDModel *m);

@@ -45,10 +45,15 @@ typedef struct {
     float *row_loss;          /* [T] */
     unsigned *tok, *tgt;      /* [T] */
     float *loss_dev;          /* [1] */
+    float *mean, *rstd;       /* [T] of the last norm (pre-norm models) */
+    void *ln_ws;              /* workspace of the norm's backward */
+    size_t ln_ws_bytes;
 } Work;
 
 struct KmbNDModel {
     KmbNDModelConfig cfg;
+    int pre_norm;
+    float norm_eps;
     long P, d, L, V, per_layer, n;
     float *params, *grads, *m, *v; /* device, flat */
     uint16_t *w16;                 /* bf16 copies: [L][(3 d + 35) d] then head [V d] */
@@ -77,6 +82,13 @@ static LayerPtrs layer_ptrs(float *base, const KmbNDModel *m, long l) {
     r.conv_bias = r.conv_kernel + 27 * d;
     return r;
 }
+
+/* Pre-norm models: weight and bias of norm l, the last one (l = L) before
+ * the head, behind the layers. */
+static float *norm_weight(float *base, const KmbNDModel *m, long l) {
+    return base + 2 * m->V * m->d + m->L * m->per_layer + 2 * l * m->d;
+}
+static long norm_size(const KmbNDModel *m) { return m->pre_norm ? 2 * (m->L + 1) * m->d : 0; }
 
 /* bf16 copies of a layer's W_a, W_z, W_out, W_p (contiguous, as in the
  * fp32 layout), then the head */
@@ -123,6 +135,11 @@ static void init_host(const KmbNDModel *m, float *h) {
         for (long i = 0; i < 27 * d; ++i) p.conv_kernel[i] = (float)(1.0 / sqrt(27.0)) * gauss(k++);
         for (long i = 0; i < d; ++i) p.conv_bias[i] = 0.f;
     }
+    for (long l = 0; m->pre_norm && l <= m->L; ++l)
+        for (long i = 0; i < d; ++i) {
+            norm_weight(h, m, l)[i] = 1.f;
+            norm_weight(h, m, l)[d + i] = 0.f;
+        }
 }
 
 /* ------------------------------------------------------------------ */
@@ -169,7 +186,7 @@ static void work_free(Work *w) {
                    w->Cs,
                    w->dBs, w->dCs, w->h, w->A, w->dA_tmp, w->ck_tmp, w->cb_tmp, w->logits,
                    w->dlogits, w->l16, w->row_loss,
-                   w->tok, w->tgt, w->loss_dev};
+                   w->tok, w->tgt, w->loss_dev, w->mean, w->rstd, w->ln_ws};
     for (size_t i = 0; i < sizeof all / sizeof *all; ++i)
         if (all[i]) cudaFree(all[i]);
     memset(w, 0, sizeof *w);
@@ -216,12 +233,63 @@ static int work_ensure(KmbNDModel *m, long batch) {
     w->tok = dalloc(sizeof(unsigned) * (size_t)T, &rc);
     w->tgt = dalloc(sizeof(unsigned) * (size_t)T, &rc);
     w->loss_dev = dalloc(sizeof(float), &rc);
+    if (m->pre_norm) {
+        w->mean = dalloc(sizeof(float) * (size_t)T, &rc);
+        w->rstd = dalloc(sizeof(float) * (size_t)T, &rc);
+        w->ln_ws_bytes = kmb_layernorm_scratch_bytes(T, d);
+        w->ln_ws = dalloc(w->ln_ws_bytes, &rc);
+    }
     if (rc) {
         work_free(w);
         return rc;
     }
     w->batch = batch;
     return KMB_OK;
+}
+
+/* The GEMM operand of a block's input, or of the head's: x in bf16, in
+ * pre-norm models its layer norm l. */
+static int operand(KmbNDModel *m, long l, const float *x, long T, cudaStream_t s) {
+    Work *w = &m->w;
+    if (!m->pre_norm) return kmb_nd_to_bf16(x, m->d, w->x16, m->d, T, m->d, s);
+    KmbLayerNorm a;
+    memset(&a, 0, sizeof a);
+    a.x = x;
+    a.weight = norm_weight(m->params, m, l);
+    a.bias = a.weight + m->d;
+    a.y = w->x16;
+    a.mean = w->mean;
+    a.rstd = w->rstd;
+    a.rows = T;
+    a.D = a.ld_x = a.ld_y = m->d;
+    a.eps = m->norm_eps;
+    a.y_type = KMB_BF16;
+    return kmb_launch_layernorm_fwd(&a, s);
+}
+
+/* Backward of norm l, whose statistics are the last ones taken: dx (which
+ * may be x) from dn, the gradient of its output, plus dres. */
+static int norm_backward(KmbNDModel *m, long l, const float *x, const float *dn, const float *dres, float *dx,
+                         int acc, long T, cudaStream_t s) {
+    Work *w = &m->w;
+    KmbLayerNorm a;
+    memset(&a, 0, sizeof a);
+    a.x = x;
+    a.weight = norm_weight(m->params, m, l);
+    a.mean = w->mean;
+    a.rstd = w->rstd;
+    a.dy = dn;
+    a.dres = dres;
+    a.dx = dx;
+    a.dweight = norm_weight(m->grads, m, l);
+    a.dbias = a.dweight + m->d;
+    a.workspace = w->ln_ws;
+    a.workspace_bytes = w->ln_ws_bytes;
+    a.rows = T;
+    a.D = a.ld_x = a.ld_dy = a.ld_dres = a.ld_dx = m->d;
+    a.eps = m->norm_eps;
+    a.accumulate = acc;
+    return kmb_launch_layernorm_bwd(&a, s);
 }
 
 /* ------------------------------------------------------------------ */
@@ -236,7 +304,7 @@ static int block_forward(KmbNDModel *m, long l, long batch, const float *x_in, f
     const long d = m->d, P = m->P, T = batch * P;
     LayerPtrs p = layer_ptrs(m->params, m, l);
     const uint16_t *w16 = w16_layer(m, l);
-    int rc = kmb_nd_to_bf16(x_in, d, w->x16, d, T, d, s);
+    int rc = operand(m, l, x_in, T, s);
     if (!rc) rc = gemm16(w->x16, w16, w->a, T, d, d, d, d, d, 0, 0, 0, NULL, 0, s);
     if (!rc) rc = gemm16(w->x16, w16 + d * d, w->z, T, d, d, d, d, d, 0, 0, 0, NULL, 0, s);
     if (rc) return rc;
@@ -358,8 +426,10 @@ static int block_backward(KmbNDModel *m, long l, long batch, const float *x_in,
     /* in_proj: dx_in = dx_out + da W_a + dz W_z; dW_a = da^T x, dW_z = dz^T x */
     uint16_t *da16 = w->d16a;
     if ((rc = kmb_nd_to_bf16(da, d, da16, d, T, d, s))) return rc;
-    if ((rc = gemm16(da16, w16, dx_in, T, d, d, d, d, d, 0, 1, 0, dx_out, 0, s))) return rc;
-    if ((rc = gemm16(dz16, w16 + d * d, dx_in, T, d, d, d, d, d, 0, 1, 0, NULL, 1, s))) return rc;
+    float *dn = m->pre_norm ? dv : dx_in; /* of the norm's output (dv is dead), or of x */
+    if ((rc = gemm16(da16, w16, dn, T, d, d, d, d, d, 0, 1, 0, m->pre_norm ? NULL : dx_out, 0, s))) return rc;
+    if ((rc = gemm16(dz16, w16 + d * d, dn, T, d, d, d, d, d, 0, 1, 0, NULL, 1, s))) return rc;
+    if (m->pre_norm && (rc = norm_backward(m, l, x_in, dn, dx_out, dx_in, acc, T, s))) return rc;
     if ((rc = gemm16(da16, w->x16, gp.W_a, d, d, T, d, d, d, 1, 1, 0, NULL, acc, s))) return rc;
     return gemm16(dz16, w->x16, gp.W_z, d, d, T, d, d, d, 1, 1, 0, NULL, acc, s);
 }
@@ -378,7 +448,7 @@ static int refresh_w16(KmbNDModel *m, cudaStream_t s) {
     return kmb_nd_to_bf16(m->params + m->V * d, d, w16_head(m), d, m->V, d, s);
 }
 
-KmbNDModel *kmb_ndmodel_create(const KmbNDModelConfig *cfg) {
+static KmbNDModel *create(const KmbNDModelConfig *cfg, int pre_norm, float norm_eps) {
     if (!cfg || cfg->dim <= 0 || cfg->dim % 32 || cfg->n_layers <= 0 || cfg->vocab <= 0 ||
         cfg->vocab % 8) {
         kmb_fail(KMB_EINVAL, "ndmodel: dim must be a positive multiple of 32, n_layers > 0, "
@@ -399,12 +469,14 @@ KmbNDModel *kmb_ndmodel_create(const KmbNDModelConfig *cfg) {
         return NULL;
     }
     m->cfg = *cfg;
+    m->pre_norm = pre_norm;
+    m->norm_eps = norm_eps;
     m->P = P;
     m->d = cfg->dim;
     m->L = cfg->n_layers;
     m->V = cfg->vocab;
     m->per_layer = layer_size(m->d);
-    m->n = 2 * m->V * m->d + m->L * m->per_layer;
+    m->n = 2 * m->V * m->d + m->L * m->per_layer + norm_size(m);
     int rc = KMB_OK;
     const size_t nb = sizeof(float) * (size_t)m->n;
     m->params = dalloc(nb, &rc);
@@ -433,6 +505,16 @@ KmbNDModel *kmb_ndmodel_create(const KmbNDModelConfig *cfg) {
         return NULL;
     }
     return m;
+}
+
+KmbNDModel *kmb_ndmodel_create(const KmbNDModelConfig *cfg) { return create(cfg, 0, 0.f); }
+
+KmbNDModel *kmb_ndmodel_create_prenorm(const KmbNDModelConfig *cfg, float norm_eps) {
+    if (!(norm_eps > 0.f) || isinf(norm_eps)) {
+        kmb_fail(KMB_EINVAL, "ndmodel: norm_eps must be positive and finite");
+        return NULL;
+    }
+    return create(cfg, 1, norm_eps);
 }
 
 void kmb_ndmodel_free(KmbNDModel *m) {
@@ -483,7 +565,7 @@ static int forward_all(KmbNDModel *m, const unsigned *tokens, long batch, float 
         if ((rc = block_forward(m, l, batch, xi, xi + (size_t)T * d, s))) return rc;
     }
     const float *xL = w->x_store + (size_t)m->L * T * d;
-    if ((rc = kmb_nd_to_bf16(xL, d, w->x16, d, T, d, s))) return rc;
+    if ((rc = operand(m, m->L, xL, T, s))) return rc;
     if ((rc = gemm16(w->x16, w16_head(m), w->logits, T, m->V, d, d, d, m->V, 0, 0, 0, NULL, 0, s)))
         return rc;
     if ((rc = kmb_nd_roll_targets(w->tok, w->tgt, batch, m->P, s))) return rc;
@@ -564,9 +646,10 @@ static int pass_backward(KmbNDModel *m, const unsigned *tokens, long batch, floa
      * head's backward, whose weight gradient reads the bf16 copy of x_L. */
     if ((rc = kmb_nd_to_bf16(w->dlogits, V, w->l16, V, T, V, s))) return rc;
     if ((rc = gemm16(w->l16, w->x16, g_head, V, d, T, V, d, d, 1, 1, 0, NULL, acc, s))) return rc;
-    if ((rc = gemm16(w->l16, w16_head(m), w->x_store + (size_t)m->L * td, T, d, V, V, d, d, 0,
-                     1, 0, NULL, 0, s)))
+    float *xL = w->x_store + (size_t)m->L * td;
+    if ((rc = gemm16(w->l16, w16_head(m), m->pre_norm ? w->tmp1 : xL, T, d, V, V, d, d, 0, 1, 0, NULL, 0, s)))
         return rc;
+    if (m->pre_norm && (rc = norm_backward(m, m->L, xL, w->tmp1, NULL, xL, acc, T, s))) return rc;
     if (feed && (rc = kmb_dist_bucket_add(m->dist, g_head, (size_t)V * d, 1, sp))) return rc;
     for (long l = m->L - 1; l >= 0; --l) {
         float *slot = w->x_store + (size_t)l * td;
@@ -583,6 +666,8 @@ static int pass_backward(KmbNDModel *m, const unsigned *tokens, long batch, floa
     if ((rc = kmb_embed(NULL, w->tok, T, d, V, NULL, w->x_store, g_emb, s))) return rc;
     if (feed) {
         if ((rc = kmb_dist_bucket_add(m->dist, g_emb, (size_t)V * d, 1, sp))) return rc;
+        if (m->pre_norm && (rc = kmb_dist_bucket_add(m->dist, norm_weight(m->grads, m, 0), (size_t)norm_size(m), 1, sp)))
+            return rc;
         if ((rc = kmb_dist_bucket_flush(m->dist, sp))) return rc;
         if ((rc = kmb_dist_wait(m->dist, sp))) return rc;
     }

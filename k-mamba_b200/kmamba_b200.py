@@ -310,6 +310,7 @@ PROTOTYPES = {
                                  C.POINTER(C.c_ulonglong), C.POINTER(C.c_ulonglong)]),
     # Mamba-ND model (kmamba_ndmodel.h)
     "kmb_ndmodel_create": (C.c_void_p, [C.POINTER(KmbNDModelConfig)]),
+    "kmb_ndmodel_create_prenorm": (C.c_void_p, [C.POINTER(KmbNDModelConfig), C.c_float]),
     "kmb_ndmodel_free": (None, [C.c_void_p]),
     "kmb_ndmodel_param_count": (lg, [C.c_void_p]),
     "kmb_ndmodel_params": (C.c_void_p, [C.c_void_p]),

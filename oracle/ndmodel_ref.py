@@ -31,6 +31,10 @@ Model (dims d = dim, N = 16 states, K = 3, 3 axes, P points per volume):
   logits = bf(x_L) bf(H)^T                                [P, 256]
   loss = mean over positions of CE(logits[i], tok[(i + 1) mod P])
 
+Pre-norm models (layers and tree with "norm_weight" / "norm_bias") project
+LN(x) instead of x, and the head reads LN(x_L), LN(x) = (x - mean) /
+sqrt(var + eps) * weight + bias over the d channels.
+
 bf(.) is round-to-nearest-even to bf16 of a GEMM operand, in the forward
 and in both gradient GEMMs (the GPU's tensor-core GEMMs take bf16
 operands); every other operation is float64 here and fp32 on the GPU.
@@ -100,7 +104,14 @@ def scan_nd(c, delta, A, B, C, dims):
     return torch.stack([(h[p] * C[p][None, :]).sum(1) for p in range(P)])
 
 
-def forward_loss(params, tokens, dims, K=3):
+def norm(x, tree, eps):
+    if "norm_weight" not in tree:
+        return x
+    c = x - x.mean(-1, keepdim=True)
+    return c / torch.sqrt((c * c).mean(-1, keepdim=True) + eps) * tree["norm_weight"] + tree["norm_bias"]
+
+
+def forward_loss(params, tokens, dims, K=3, eps=1e-5):
     """params: dict of float64 tensors (requires_grad as the caller wants);
     tokens: int64 [batch, P].  Returns the mean next-token loss."""
     batch, P = tokens.shape
@@ -109,8 +120,9 @@ def forward_loss(params, tokens, dims, K=3):
     for b in range(batch):
         x = E[tokens[b]]
         for layer in params["layers"]:
-            a = Bf16Linear.apply(x, layer["W_a"])
-            z = Bf16Linear.apply(x, layer["W_z"])
+            n = norm(x, layer, eps)
+            a = Bf16Linear.apply(n, layer["W_a"])
+            z = Bf16Linear.apply(n, layer["W_z"])
             v = conv3d_causal(a, layer["conv_kernel"], layer["conv_bias"], dims, K)
             c = v * torch.sigmoid(v)
             q = Bf16Linear.apply(c, layer["W_p"])
@@ -121,7 +133,7 @@ def forward_loss(params, tokens, dims, K=3):
             y = scan_nd(c, delta, -1.0 - torch.exp(layer["A_log"]), Bm, Cm, dims)
             g = y * (z * torch.sigmoid(z))
             x = x + Bf16Linear.apply(g, layer["W_out"])
-        logits = Bf16Linear.apply(x, params["head"])
+        logits = Bf16Linear.apply(norm(x, params, eps), params["head"])
         tgt = torch.roll(tokens[b], -1)
         total = total + torch.nn.functional.cross_entropy(logits, tgt, reduction="sum")
     return total / (batch * P)
