@@ -580,13 +580,12 @@ struct Maps {
 
 /* Joins the tile with the ones before it in its chain and returns the state
  * that enters it.  agg: the warps' maps, joined from the last when REVERSE;
- * first: the state that enters the chain.  For kernels with one tile a CTA:
- * every warp looks at other tiles, then all go through what was seen. */
+ * h: the state that enters the chain (place 0).  For kernels with one tile a
+ * CTA: every warp looks at other tiles, then all go through what was seen. */
 template <bool VEC, bool MARKED, bool REVERSE, int W, int N, int V>
 __device__ __forceinline__ F<V> enter_tile(const Dev &p, const Place &at, const Lane<VEC, V> &ln,
-                                           const Maps<W, V> &agg, Maps<N, V> &seen, int warps, const float *first) {
+                                           const Maps<W, V> &agg, Maps<N, V> &seen, int warps, F<V> h) {
     const int warp = threadIdx.x / 32;
-    F<V> h = ln.at(at.pos == 0 ? first : nullptr);
     if (p.tiles == 1) return h;
     const Shown &s = p.shown;
     const long o = at.pos * s.step + at.chain * 32 + ln.lane;
@@ -680,7 +679,8 @@ struct RunOf {
     }
 
     /* The forward before the state that enters is known: decays and input
-     * terms of the rows, and the run's map. */
+     * terms of the rows (a sequence's first row: its state), and the run's
+     * map. */
     __device__ __forceinline__ Map<V> forward_map(const Rates<V> &rt, F<V> (&c)[R], F<V> (&b)[R]) const {
 #pragma unroll
         for (int j = 0; j < R; ++j) {
@@ -699,6 +699,7 @@ struct RunOf {
                 }
                 m.H = advance<WEAK>(c[j], m.H, b[j]);
                 m.A = shrink<WEAK>(c[j], m.A);
+                if (begins(j)) b[j] = m.H; /* h0 is not read again: h_last may be h0, and another warp's to write */
             }
         }
         if (fresh) m.A = all<V>(-1.f);
@@ -714,8 +715,7 @@ struct RunOf {
         for (int j = 0; j < R; ++j) {
             if (in(j)) {
                 if (j == mark) ln.put(p.ckpt_out + (at.b * p.chunks + (row0 + j) / chunk) * p.a.D, h);
-                if (begins(j)) h = of(p.a.h0, j);
-                h = advance<WEAK>(c[j], h, b[j]);
+                h = begins(j) ? b[j] : advance<WEAK>(c[j], h, b[j]);
                 io.y(j, h);
                 if (ends(j)) put(p.a.h_last, j, h);
             }
@@ -723,11 +723,12 @@ struct RunOf {
         if (!PACKED && p.a.h_last && live > 0 && row0 + live == p.a.L) ln.put(p.a.h_last + at.b * p.a.D, h);
     }
 
-    /* The backward, likewise: the terms of the rows and the run's maps, of
-     * the states and of the adjoint.  The adjoint that reaches row t - 1 from
+    /* The backward, likewise: the terms of the rows, what the states of
+     * sequences that end here are worth, and the run's maps, of the states and
+     * of the adjoint.  The adjoint that reaches row t - 1 from
      * row t is C_t = a_t (dy_t + C_{t+1}). */
-    __device__ __forceinline__ void backward_maps(const Rates<V> &rt, Terms<V> (&t)[R], Map<V> &state,
-                                                  Map<V> &adjoint) const {
+    __device__ __forceinline__ void backward_maps(const Rates<V> &rt, Terms<V> (&t)[R], F<V> (&last)[R],
+                                                  Map<V> &state, Map<V> &adjoint) const {
 #pragma unroll
         for (int j = 0; j < R; ++j) t[j] = terms<WEAK>(io.gr(j), io.gi(j), rt);
         F<V> A = all<V>(1.f), H = all<V>(0.f), K = H;
@@ -747,7 +748,7 @@ struct RunOf {
         for (int j = R - 1; j >= 0; --j) {
             if (in(j)) {
                 if (ends(j)) {
-                    K = of(p.a.dh_last, j);
+                    K = last[j] = of(p.a.dh_last, j); /* not read again: dh0 may be dh_last */
                     closed = true;
                 }
                 K = shrink<WEAK>(t[j].c, K + io.dy(j));
@@ -769,12 +770,13 @@ struct RunOf {
         }
     }
     /* C: the adjoint that reaches the run.  Returns the sum of udu. */
-    __device__ __forceinline__ F<V> backward_rows(F<V> C, const Terms<V> (&t)[R], const F<V> (&f)[R]) const {
+    __device__ __forceinline__ F<V> backward_rows(F<V> C, const Terms<V> (&t)[R], const F<V> (&last)[R],
+                                                  const F<V> (&f)[R]) const {
         F<V> sum = all<V>(0.f);
 #pragma unroll
         for (int j = R - 1; j >= 0; --j) {
             if (in(j)) {
-                if (ends(j)) C = of(p.a.dh_last, j);
+                if (ends(j)) C = last[j];
                 const F<V> G = C + io.dy(j), udu = G * f[j];
                 sum = sum + udu;
                 io.grads(j, G * t[j].si, udu * t[j].q, G * t[j].i);
@@ -854,8 +856,9 @@ __device__ __forceinline__ void any_forward(const Dev &p, const Place &at, const
     F<kV> c[kFR], b[kFR];
     const Map<kV> m = run.forward_map(rt, c, b);
     sh.agg.put(warp, ln.lane, m.A, m.H);
+    /* before the barrier: h_last may be h0, and another warp's to write */
+    const F<kV> first = ln.at(!PACKED && p.a.h0 && at.pos == 0 ? p.a.h0 + at.b * p.a.D : nullptr);
     __syncthreads();
-    const float *first = !PACKED && p.a.h0 ? p.a.h0 + at.b * p.a.D : nullptr;
     F<kV> h = enter_tile<VEC, PACKED, false>(p, at, ln, sh.agg, sh.seen, blockDim.x / 32, first);
     for (int w = 0; w < warp; ++w) h = apply<PACKED>(sh.agg.at(w, ln.lane), h);
     run.forward_rows(h, c, b);
@@ -933,18 +936,20 @@ __device__ __forceinline__ F<kV> any_backward(const Dev &p, const Place &at, con
     const RunOf<AnyBwdIo<T, VEC>, VEC, PACKED, false, WEAK, kBR<T>, PACKED ? kBT<T> : 1, kV> run = {
         p, at, ln, sh.rows, io, row0, live, warp};
     Terms<kV> t[kBR<T>];
+    F<kV> ends[kBR<T>];
     Map<kV> state, adjoint;
-    run.backward_maps(rt, t, state, adjoint);
+    run.backward_maps(rt, t, ends, state, adjoint);
     sh.states.put(warp, ln.lane, state.A, state.H);
     sh.agg.put(warp, ln.lane, adjoint.A, adjoint.H);
+    /* before the barrier: dh0 may be dh_last, and another warp's to write */
+    const F<kV> last = ln.at(!PACKED && p.a.dh_last && at.pos == 0 ? p.a.dh_last + at.b * p.a.D : nullptr);
     __syncthreads();
     F<kV> f[kBR<T>];
     for (int w = 0; w < warp; ++w) entry = apply<PACKED>(sh.states.at(w, ln.lane), entry);
     run.backward_factors(entry, rt.rate, t, f);
-    const float *last = !PACKED && p.a.dh_last ? p.a.dh_last + at.b * p.a.D : nullptr;
     F<kV> C = enter_tile<VEC, PACKED, true>(p, at, ln, sh.agg, sh.seen, warps, last);
     for (int w = warps - 1; w > warp; --w) C = apply<PACKED>(sh.agg.at(w, ln.lane), C);
-    return run.backward_rows(C, t, f);
+    return run.backward_rows(C, t, ends, f);
 }
 
 template <typename T, bool VEC, bool PACKED>
@@ -1319,10 +1324,10 @@ __device__ __forceinline__ void work(const Dev &p, char *tiles, RingShared<T, BW
             const auto run = bench.run(full, weak);
             if constexpr (BWD) {
                 Terms<V> x[R];
-                F<V> f[R];
+                F<V> f[R], ends[R];
                 {
                     Map<V> state, adjoint;
-                    run.backward_maps(bench.rates(), x, state, adjoint);
+                    run.backward_maps(bench.rates(), x, ends, state, adjoint);
                     sh.states.put(worker, lane, state.A, state.H);
                     sh.agg.put(worker, lane, adjoint.A, adjoint.H);
                 }
@@ -1334,7 +1339,7 @@ __device__ __forceinline__ void work(const Dev &p, char *tiles, RingShared<T, BW
                 if (worker != 0) Workers::enter();
                 F<V> C = from(sh.in[lane]);
                 for (int w = kW - 1; w > worker; --w) C = apply<PACKED>(sh.agg.at(w, lane), C);
-                st.sums[worker][lane] = to(run.backward_rows(C, x, f));
+                st.sums[worker][lane] = to(run.backward_rows(C, x, ends, f));
             } else {
                 F<V> c[R], b[R];
                 {

@@ -208,9 +208,42 @@ def test_resident_kernels_in_place_and_same_bits(lib, cuda, packed):
             assert torch.equal(o.t, first[k]), k
         d = mk()
         a = d.args()
-        a.y = a.x
+        a.y, a.h_last = a.x, a.h0
         kb.check(lib, lib.kmb_glr_fwd(byref(a)))
-        assert torch.equal(d.x.t, first["y"])
+        assert torch.equal(d.x.t, first["y"]) and torch.equal(d.t["h0"], first["h_last"])
+        d = mk()
+        a = d.args()
+        a.dh0 = a.dh_last
+        kb.check(lib, lib.kmb_glr_bwd(byref(a)))
+        assert torch.equal(d.t["dh_last"], first["dh0"])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [256, 70])
+def test_short_sequences_with_states_in_place(lib, cuda, D, dtype):
+    """Sequences that begin and end in one tile, in rows of different warps:
+    the last state goes where the first one came from."""
+    rng = np.random.default_rng(D)
+    off = np.concatenate([[0], np.cumsum(rng.integers(0, 40, 300))])
+    mk = lambda: Case(300, int(off[-1]), D, dtype, offsets=off, seed=7)  # noqa: E731
+    c = mk()
+    v, e = c.ref()
+    inside = c.inside
+    for _ in range(5):
+        c = mk()
+        c.inside = inside
+        a = c.args()
+        a.h_last = a.h0
+        kb.check(lib, lib.kmb_glr_fwd(byref(a)))
+        within("h_last", c.t["h0"].double().cpu().numpy(), v["h_last"], e["h_last"])
+        c.check(v, e, ("y",))
+        c = mk()
+        c.inside = inside
+        a = c.args()
+        a.dh0 = a.dh_last
+        kb.check(lib, lib.kmb_glr_bwd(byref(a)))
+        within("dh0", c.t["dh_last"].double().cpu().numpy(), v["dh0"], e["dh0"])
+        c.check(v, e, ("dx", "dgate_r", "dgate_i", "ddecay"))
 
 
 @pytest.mark.parametrize("ckpt,ws", [(False, True), (True, False), (False, False)])
@@ -365,8 +398,8 @@ def test_nan_stays_in_its_sequence(lib, cuda):
 
 def test_in_place(lib, cuda):
     """y over x; the gradients over x and the gates; h_last over h0 and dh0 over dh_last."""
-    for off in (None, [0, 150, 150, 420]):
-        c = Case(3, 420, 66, BF16, offsets=off)
+    for off in (None, [0, 150, 150, 420], [0, 3, 17, 40, 41, 41, 120, 420]):
+        c = Case(len(off) - 1 if off else 3, 420, 66, BF16, offsets=off)
         v, e = c.ref()
         a = c.args()
         a.h_last, a.y = a.h0, a.x
@@ -374,7 +407,7 @@ def test_in_place(lib, cuda):
         c.t["h_last"], c.y = c.t["h0"], c.x
         c.check(v, e, ("h_last",))
         within("y", c.y.np().reshape(-1, 66), v["y"], e["y"], BF16)
-        c = Case(3, 420, 66, BF16, offsets=off)
+        c = Case(len(off) - 1 if off else 3, 420, 66, BF16, offsets=off)
         a = c.args()
         a.dx, a.dgate_r, a.dgate_i, a.dh0 = a.x, a.gate_r, a.gate_i, a.dh_last
         kb.check(lib, lib.kmb_glr_bwd(byref(a)))
