@@ -369,7 +369,7 @@ size_t kmb_layernorm_workspace_bytes(const KmbLayerNorm *args);
  *   y_t = h_t
  * The gates are pre-activations, as the GEMM of the block's projections
  * leaves them.  x, gate_r, gate_i, y and their gradients are of one type
- * (KMB_F32 or KMB_BF16); decay, h0, h_last, ckpt, dh_last, dh0 and ddecay
+ * (KMB_F32 or KMB_BF16); decay (finite), h0, h_last, ckpt, dh_last, dh0 and ddecay
  * are fp32, and so is every state and sum.
  *
  * Sequences, without offsets: `batch` sequences of L rows.  Each tensor is
@@ -397,7 +397,8 @@ size_t kmb_layernorm_workspace_bytes(const KmbLayerNorm *args);
  * overwritten, or added to when accumulate is 1).
  *
  * An output may be the very tensor of an input of the same call (same
- * pointer and strides); any other overlap is not allowed.  batch = 0 and
+ * pointer and strides), not of another output; any other overlap is not
+ * allowed.  batch = 0 and
  * L = 0 are allowed.  Device memory of the current device only, every
  * tensor aligned to its element.
  *

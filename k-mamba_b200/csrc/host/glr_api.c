@@ -45,6 +45,21 @@ static int check_rows(const KmbGLR *a, const KmbRows *r, const char *name, int o
     return KMB_OK;
 }
 
+/* An output may be an input, the very same rows, but not another output. */
+static int check_overlap(const KmbGLR *a, const KmbRows *const *in, int ni, const KmbRows *const *out, int no) {
+    for (int i = 0; i < no; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (out[i]->data == out[j]->data) return kmb_fail(KMB_EINVAL, "glr: two outputs share their memory");
+        for (int j = 0; j < ni; ++j) {
+            if (out[i]->data != in[j]->data) continue;
+            if (out[i]->row_stride != in[j]->row_stride ||
+                (!a->offsets && a->batch > 1 && out[i]->batch_stride != in[j]->batch_stride))
+                return kmb_fail(KMB_EINVAL, "glr: an output over an input of other strides");
+        }
+    }
+    return KMB_OK;
+}
+
 static int validate(const KmbGLR *a, int bwd) {
     if (!a) return kmb_fail(KMB_EINVAL, "glr: NULL arguments");
     if (a->batch < 0 || a->L < 0 || a->D <= 0)
@@ -64,11 +79,17 @@ static int validate(const KmbGLR *a, int bwd) {
     int rc = check_rows(a, &a->x, "x", 0);
     if (!rc) rc = check_rows(a, &a->gate_r, "gate_r", 0);
     if (!rc) rc = check_rows(a, &a->gate_i, "gate_i", 0);
-    if (!bwd) return rc ? rc : check_rows(a, &a->y, "y", 1);
+    const KmbRows *in[] = {&a->x, &a->gate_r, &a->gate_i, &a->dy};
+    const KmbRows *fwd_out[] = {&a->y}, *bwd_out[] = {&a->dx, &a->dgate_r, &a->dgate_i};
+    if (!bwd) {
+        if (!rc) rc = check_rows(a, &a->y, "y", 1);
+        return rc ? rc : check_overlap(a, in, 3, fwd_out, 1);
+    }
     if (!rc) rc = check_rows(a, &a->dy, "dy", 0);
     if (!rc) rc = check_rows(a, &a->dx, "dx", 1);
     if (!rc) rc = check_rows(a, &a->dgate_r, "dgate_r", 1);
-    return rc ? rc : check_rows(a, &a->dgate_i, "dgate_i", 1);
+    if (!rc) rc = check_rows(a, &a->dgate_i, "dgate_i", 1);
+    return rc ? rc : check_overlap(a, in, 4, bwd_out, 3);
 }
 
 static int run(const KmbGLR *a, int bwd) {

@@ -44,6 +44,13 @@ static int validate(const KmbLayerNorm *a, int bwd) {
         (bwd && (misaligned(a->dy, ys) || misaligned(a->dx, xs) || misaligned(a->dres, xs) ||
                  misaligned(a->dweight, 4) || misaligned(a->dbias, 4))))
         return kmb_fail(KMB_EINVAL, "layernorm: a tensor is not aligned to its element");
+    /* an output over an input has its type and stride */
+    const int same = a->x_type == a->y_type;
+    if (a->rows && ((!bwd && a->y == a->x && !(same && a->ld_y == a->ld_x)) ||
+                    (bwd && ((a->dx == a->x && a->ld_dx != a->ld_x) ||
+                             (a->dx == a->dy && !(same && a->ld_dx == a->ld_dy)) ||
+                             (a->dx == a->dres && a->ld_dx != a->ld_dres)))))
+        return kmb_fail(KMB_EINVAL, "layernorm: an output over an input of another type or stride");
     return KMB_OK;
 }
 

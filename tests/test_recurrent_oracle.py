@@ -64,8 +64,8 @@ BAD = 0x1000  # never dereferenced: the host's checks come first
 
 def ln_args(**kw):
     a = kb.KmbLayerNorm()
-    for n in ("x", "y", "dy", "dx", "dweight"):
-        setattr(a, n, BAD)
+    for k, n in enumerate(("x", "y", "dy", "dx", "dweight")):
+        setattr(a, n, BAD + 4096 * k)
     a.rows, a.D, a.eps = 4, 8, 1e-5
     a.ld_x = a.ld_y = a.ld_dy = a.ld_dx = 8
     for k, v in kw.items():
@@ -79,7 +79,7 @@ def ln_args(**kw):
     (dict(x_type=2), b"type"), (dict(y_type=-1), b"type"), (dict(eps=-1.0), b"eps"),
     (dict(eps=float("nan")), b"eps"), (dict(eps=float("inf")), b"eps"), (dict(accumulate=2), b"accumulate"),
     (dict(x=BAD + 2), b"aligned"), (dict(y=BAD + 1, y_type=1), b"aligned"), (dict(weight=BAD + 1), b"aligned"),
-    (dict(), b"device memory")])
+    (dict(y=BAD, y_type=1), b"another type"), (dict(y=BAD, ld_y=9), b"another type"), (dict(), b"device memory")])
 def test_layernorm_fwd_refuses(lib, kw, word):
     assert lib.kmb_layernorm_fwd(C.byref(ln_args(**kw))) == kb.KMB_EINVAL
     assert word in lib.kmb_last_error(), lib.kmb_last_error()
@@ -90,7 +90,8 @@ def test_layernorm_fwd_refuses(lib, kw, word):
     (dict(rstd=BAD), b"together"), (dict(ld_dy=7), b"row stride"), (dict(ld_dx=7), b"row stride"),
     (dict(dres=BAD, ld_dres=7), b"row stride"), (dict(workspace=BAD, workspace_bytes=15), b"workspace"),
     (dict(workspace=BAD + 8, workspace_bytes=1 << 30), b"16-byte"), (dict(dbias=BAD + 2), b"aligned"),
-    (dict(), b"device memory")])
+    (dict(dx=BAD, ld_dx=9), b"another type"), (dict(dx=BAD + 4096 * 2, y_type=1), b"another type"),
+    (dict(dres=BAD + 4096 * 3, ld_dres=9), b"another type"), (dict(), b"device memory")])
 def test_layernorm_bwd_refuses(lib, kw, word):
     assert lib.kmb_layernorm_bwd(C.byref(ln_args(**kw))) == kb.KMB_EINVAL
     assert word in lib.kmb_last_error(), lib.kmb_last_error()
@@ -106,8 +107,8 @@ def test_layernorm_sizes(lib):
 def glr_args(batch=2, L=5, D=8, **kw):
     a = kb.KmbGLR()
     a.batch, a.L, a.D, a.scale = batch, L, D, 8.0
-    for n in ("x", "gate_r", "gate_i", "y", "dy", "dx", "dgate_r", "dgate_i"):
-        setattr(a, n, kb.KmbRows(BAD, D, L * D))
+    for k, n in enumerate(("x", "gate_r", "gate_i", "y", "dy", "dx", "dgate_r", "dgate_i")):
+        setattr(a, n, kb.KmbRows(BAD + 4096 * k, D, L * D))
     a.decay = BAD
     for k, v in kw.items():
         setattr(a, k, v)
@@ -126,7 +127,8 @@ FWD_BAD = [
 
 
 @pytest.mark.parametrize("kw,word", FWD_BAD + [(dict(y=R(BAD, 8, 39)), b"overlap"), (dict(y=R(BAD, 15, 8)), b"overlap"),
-                                               (dict(y=R(None, 8, 40)), b"y is required")])
+                                               (dict(y=R(None, 8, 40)), b"y is required"),
+                                               (dict(y=R(BAD, 9, 45)), b"other strides")])
 def test_glr_fwd_refuses(lib, kw, word):
     assert lib.kmb_glr_fwd(C.byref(glr_args(**kw))) == kb.KMB_EINVAL
     assert word in lib.kmb_last_error(), lib.kmb_last_error()
@@ -134,6 +136,8 @@ def test_glr_fwd_refuses(lib, kw, word):
 
 @pytest.mark.parametrize("kw,word", FWD_BAD + [(dict(dx=R(BAD, 8, 39)), b"overlap"), (dict(dy=R(None, 8, 40)), b"dy is required"),
                                                (dict(dgate_i=R(None, 8, 40)), b"dgate_i is required"),
+                                               (dict(dx=R(BAD + 7 * 4096, 8, 40)), b"two outputs"),
+                                               (dict(dgate_r=R(BAD, 8, 48)), b"other strides"),
                                                (dict(workspace=BAD, workspace_bytes=3), b"workspace"),
                                                (dict(workspace=BAD + 4, workspace_bytes=1 << 40), b"16-byte")])
 def test_glr_bwd_refuses(lib, kw, word):
@@ -151,7 +155,7 @@ def test_glr_sizes(lib):
     assert lib.kmb_glr_ckpt_elems(C.byref(glr_args(batch=3, L=0, D=7))) == 0
     assert lib.kmb_glr_ckpt_elems(C.byref(glr_args(D=-1))) == 0
     # a time-major output passes the overlap check (and then fails on the pointers)
-    lib.kmb_glr_fwd(C.byref(glr_args(y=R(BAD, 16, 8))))
+    lib.kmb_glr_fwd(C.byref(glr_args(y=R(BAD + 64, 16, 8))))
     assert b"device memory" in lib.kmb_last_error()
 
 
