@@ -27,7 +27,7 @@
  * Measured (B200, 6.56 TB/s copy): forward 8 x 4096 x 1536 fp32 137 us (5.9
  * TB/s), bf16 104 us (3.9 TB/s); 1 x 65536 x 2048 bf16 355 us (3.0 TB/s);
  * backward 8 x 4096 x 1536 bf16 166 us (4.2 TB/s); rows that are not 16-byte
- * aligned, 24001 x 771 fp32, 114 and 267 us (2.6 and 1.9 TB/s).
+ * aligned, 24001 x 771 fp32, 111 and 237 us (2.7 and 2.2 TB/s).
  */
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -952,8 +952,13 @@ __device__ __forceinline__ F<kV> any_backward(const Dev &p, const Place &at, con
     return run.backward_rows(C, t, ends, f);
 }
 
+/* CTAs of an SM: 64 registers a thread do for 4 rows, 237 against 262 us with
+ * 128 (24001 x 771 fp32); 8 rows would spill */
+template <typename T>
+constexpr int kBCtas = sizeof(T) == 2 ? 2 : 4;
+
 template <typename T, bool VEC, bool PACKED>
-__global__ void __launch_bounds__(kBW * 32, 2) k_glr_bwd(const __grid_constant__ Dev p) {
+__global__ void __launch_bounds__(kBW * 32, kBCtas<T>) k_glr_bwd(const __grid_constant__ Dev p) {
     __shared__ AnyBwdShared<kBW, kBT<T>, PACKED> sh;
     const int warp = threadIdx.x / 32, warps = blockDim.x / 32;
     const Place at(p, tile_id(p, &sh.slot));
