@@ -210,6 +210,22 @@ def test_same_bits_every_run(lib, cuda, rows, D):
         assert all(torch.equal(p, q) for p, q in zip(first, (c.dx.t, c.dw, c.db)))
 
 
+@pytest.mark.parametrize("rows,D", [(1, 1), (33, 1), (3, 1000), (255, 128), (1024, 128), (1025, 128), (256, 129), (257, 129),
+                                    (256, 511), (32, 513), (33, 513), (31, 2047), (32, 2048), (32, 2049)])
+@pytest.mark.parametrize("xt,yt", [(F32, F32), (BF16, F32), (BF16, BF16)])
+def test_few_rows(lib, cuda, rows, D, xt, yt):
+    """Around the sizes up to which one launch does rows and sums; three calls
+    that add up give three times the sums."""
+    c = Case(rows, D, xt, yt, seed=rows + D)
+    bwd(lib, c, res=True, stats=False)
+    check_bwd(c, res=True, stats=False)
+    dw, db, dx = c.dw.clone(), c.db.clone(), c.dx.t.clone()
+    for _ in range(2):
+        bwd(lib, c, res=True, stats=False, acc=1)
+        assert torch.equal(c.dx.t, dx)
+    assert torch.equal(c.dw, (dw + dw) + dw) and torch.equal(c.db, (db + db) + db)
+
+
 def test_gradient_against_differences(lib, cuda):
     """Along one direction: (f(x + t v) - f(x - t v)) / 2t of the forward, the
     sum taken in float64.  t = 2^-6: truncation ~ t^2, rounding ~ 2^-24 / t."""
