@@ -417,6 +417,35 @@ def test_in_place(lib, cuda):
             within(k, o.np().reshape(-1, 66), v[k], e[k], BF16)
 
 
+@pytest.mark.parametrize("ckpt", [False, True])
+@pytest.mark.parametrize("D,L", [(66, 420), (256, 6000)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_outputs_over_other_inputs(lib, cuda, packed, D, L, ckpt):
+    """y over a gate; each gradient over another's input, dh0 over h0."""
+    off = [0, 3, 17, 40, 41, 41, 120, L] if packed else None
+    batch = 7 if packed else 3
+    for dx, dr, di in (("dy", "x", "gate_r"), ("gate_r", "gate_i", "dy"), ("gate_i", "dy", "x")):
+        c = Case(batch, L, D, BF16, offsets=off)
+        v, e = c.ref()
+        a = c.args()
+        if ckpt:
+            states = torch.full((max(1, lib.kmb_glr_ckpt_elems(byref(a))),), SENTINEL, device="cuda")
+            a.ckpt = states.data_ptr()
+            kb.check(lib, lib.kmb_glr_fwd(byref(a)))
+        a.dx, a.dgate_r, a.dgate_i, a.dh0 = getattr(a, dx), getattr(a, dr), getattr(a, di), a.h0
+        kb.check(lib, lib.kmb_glr_bwd(byref(a)))
+        within("dh0", c.t["h0"].double().cpu().numpy(), v["dh0"], e["dh0"])
+        c.check(v, e, ("ddecay",))
+        for k, o in (("dx", dx), ("dgate_r", dr), ("dgate_i", di)):
+            within(k, getattr(c, o).np().reshape(-1, D), v[k], e[k], BF16)
+    for over in ("gate_r", "gate_i"):
+        c = Case(batch, L, D, BF16, offsets=off)
+        a = c.args()
+        a.y = getattr(a, over)
+        kb.check(lib, lib.kmb_glr_fwd(byref(a)))
+        within("y", getattr(c, over).np().reshape(-1, D), v["y"], e["y"], BF16)
+
+
 def test_same_bits_every_run(lib, cuda):
     for off in (None, [0, 1000, 1003, 3000]):
         c = Case(3, 3000, 100, offsets=off)

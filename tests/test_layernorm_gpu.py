@@ -297,6 +297,36 @@ def test_graph_capture_and_shared_workspace(lib, cuda):
         check_bwd(c, stats=False)
 
 
+def test_few_rows_captured(lib, cuda):
+    """A backward of one launch, captured and replayed on new inputs."""
+    c = Case(100, 384)
+    a = c.args()
+    a.dweight, a.dbias = c.dw.data_ptr(), c.db.data_ptr()
+    ws = torch.empty(lib.kmb_layernorm_workspace_bytes(byref(a)), dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    stream = torch.cuda.Stream()
+    try:
+        lib.kmb_set_sync(0)
+        lib.kmb_set_stream(stream.cuda_stream)
+        kb.check(lib, lib.kmb_layernorm_bwd(byref(a)))
+        stream.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            kb.check(lib, lib.kmb_layernorm_bwd(byref(a)))
+        c.xv = typed(c.xv[::-1] * 1.5 + 0.25, F32)
+        c.x.set(c.xv)
+        c.dw.fill_(SENTINEL)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            g.replay()
+            g.replay()
+        torch.cuda.synchronize()
+    finally:
+        lib.kmb_set_stream(None)
+        lib.kmb_set_sync(1)
+    check_bwd(c, stats=False)
+
+
 def test_rows_past_32_bits(lib, cuda):
     """A tensor of more than 2^32 elements between the first and last row."""
     D, rows = 256, 3
