@@ -24,10 +24,10 @@
  * to the final state of the one before it, whichever of the two was read,
  * so results do not depend on timing.
  *
- * Measured (B200, 6.56 TB/s copy): forward 8 x 4096 x 1536 fp32 137 us (5.9
- * TB/s), bf16 104 us (3.9 TB/s); 1 x 65536 x 2048 bf16 355 us (3.0 TB/s);
- * backward 8 x 4096 x 1536 bf16 166 us (4.2 TB/s); rows that are not 16-byte
- * aligned, 24001 x 771 fp32, 111 and 237 us (2.7 and 2.2 TB/s).
+ * Measured (B200, 6.56 TB/s copy): forward 8 x 4096 x 1536 fp32 135 us (6.0
+ * TB/s), bf16 103 us (3.9 TB/s); 1 x 65536 x 2048 bf16 352 us (3.0 TB/s);
+ * backward 8 x 4096 x 1536 bf16 163 us (4.3 TB/s); rows that are not 16-byte
+ * aligned, 24001 x 771 fp32, 109 and 234 us (2.7 and 2.2 TB/s).
  */
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -867,6 +867,7 @@ __device__ __forceinline__ void any_forward(const Dev &p, const Place &at, const
 template <typename T, bool VEC, bool PACKED>
 __global__ void __launch_bounds__(kFW * 32, 3) k_glr_fwd(const __grid_constant__ Dev p) {
     __shared__ AnyShared<kFW, kFT, PACKED> sh;
+    kmb_wait_before();
     const int warp = threadIdx.x / 32;
     const Place at(p, tile_id(p, &sh.slot));
     const long ch0 = (long)at.group * kC;
@@ -960,6 +961,7 @@ constexpr int kBCtas = sizeof(T) == 2 ? 2 : 4;
 template <typename T, bool VEC, bool PACKED>
 __global__ void __launch_bounds__(kBW * 32, kBCtas<T>) k_glr_bwd(const __grid_constant__ Dev p) {
     __shared__ AnyBwdShared<kBW, kBT<T>, PACKED> sh;
+    kmb_wait_before();
     const int warp = threadIdx.x / 32, warps = blockDim.x / 32;
     const Place at(p, tile_id(p, &sh.slot));
     const long ch0 = (long)at.group * kC;
@@ -1369,6 +1371,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, BWD>::kCtas)) k_glr_ring(c
     typedef Shape<T, BWD> S;
     extern __shared__ __align__(128) char tiles[];
     RingShared<T, BWD, PACKED> &sh = *reinterpret_cast<RingShared<T, BWD, PACKED> *>(tiles + S::kStages * S::kStage);
+    kmb_wait_before();
     const int warp = threadIdx.x / 32;
     if (threadIdx.x == 0) {
         for (int k = 0; k < S::kStages; ++k) {
@@ -1387,6 +1390,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, BWD>::kCtas)) k_glr_ring(c
 __global__ void __launch_bounds__(1024) k_glr_ddecay(const float *part, long rows, long ld, long D,
                                                      const float *decay, float *ddecay, int acc) {
     __shared__ float s[32][33];
+    kmb_wait_before();
     const int tx = threadIdx.x, ty = threadIdx.y;
     const long d = (long)blockIdx.x * 32 + tx;
     float v = 0.f;
@@ -1408,6 +1412,7 @@ __global__ void __launch_bounds__(1024) k_glr_ddecay(const float *part, long row
  * the ticket, and works out the channels' rates (0 beyond the last). */
 __global__ void __launch_bounds__(256) k_glr_begin(uint4 *fill, long n, float2 *rates, long channels, long D,
                                                    const float *decay, float scale) {
+    kmb_let_after();
     const long at = (long)blockIdx.x * 256 + threadIdx.x, step = (long)gridDim.x * 256;
     for (long k = at; k < n; k += step) fill[k] = make_uint4(kUnset, kUnset, kUnset, kUnset);
     for (long c = at; c < channels; c += step) {
@@ -1505,6 +1510,7 @@ __global__ void __launch_bounds__(kStepThreads) k_glr_step(const __grid_constant
 /* launches                                                             */
 /* ------------------------------------------------------------------ */
 
+int started(cudaError_t e) { return e == cudaSuccess ? KMB_OK : kmb_cuda_fail(e, "glr: launch"); }
 int done(const char *what) {
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? KMB_OK : kmb_cuda_fail(e, what);
@@ -1672,8 +1678,7 @@ int launch_ring(const Dev &d, const Plan &q, const TensorMaps &tm, cudaStream_t 
     if (e != cudaSuccess) return kmb_cuda_fail(e, "glr: shared memory");
     const long n = q.tiles * q.chains;
     const long most = (long)S::kCtas * kSMs;
-    k<<<(unsigned)(n < most ? n : most), kThreads, bytes, s>>>(d, tm);
-    return done("glr: launch");
+    return started(kmb_launch_after(d.ticket != nullptr, k, (unsigned)(n < most ? n : most), kThreads, bytes, s, d, tm));
 }
 
 template <typename T>
@@ -1701,13 +1706,12 @@ int launch(const Dev &d, const Plan &q, bool bwd, bool vec, cudaStream_t s) {
     if (bwd) {
         auto k = packed ? (vec ? k_glr_bwd<T, true, true> : k_glr_bwd<T, false, true>)
                         : (vec ? k_glr_bwd<T, true, false> : k_glr_bwd<T, false, false>);
-        k<<<n, threads, 0, s>>>(d);
+        return started(kmb_launch_after(d.ticket != nullptr, k, n, threads, 0, s, d));
     } else {
         auto k = packed ? (vec ? k_glr_fwd<T, true, true> : k_glr_fwd<T, false, true>)
                         : (vec ? k_glr_fwd<T, true, false> : k_glr_fwd<T, false, false>);
-        k<<<n, threads, 0, s>>>(d);
+        return started(kmb_launch_after(d.ticket != nullptr, k, n, threads, 0, s, d));
     }
-    return done("glr: launch");
 }
 int launch(const Dev &d, const Plan &q, bool bwd, bool vec, cudaStream_t s) {
     return d.a.type == KMB_BF16 ? launch<__nv_bfloat16>(d, q, bwd, vec, s) : launch<float>(d, q, bwd, vec, s);
@@ -1792,9 +1796,9 @@ extern "C" int kmb_launch_glr_bwd(const KmbGLR *a, cudaStream_t s) {
     const KmbRows *rows[] = {&d.a.x, &d.a.gate_r, &d.a.gate_i, &d.a.dy, &d.a.dx, &d.a.dgate_r, &d.a.dgate_i};
     rc = launch(d, q, true, vectors(&d.a, rows, 7), s);
     if (rc || !a->ddecay) return rc;
-    k_glr_ddecay<<<(unsigned)((a->D + 31) / 32), dim3(32, 32), 0, s>>>(
-        d.part, q.tiles * q.batch, q.groups * q.channels, a->D, a->decay, a->ddecay, a->accumulate);
-    return done("glr: backward launch");
+    return started(kmb_launch_after(true, k_glr_ddecay, (unsigned)((a->D + 31) / 32), dim3(32, 32), 0, s,
+                                    (const float *)d.part, q.tiles * q.batch, q.groups * q.channels, a->D, a->decay,
+                                    a->ddecay, a->accumulate));
 }
 
 template <typename T>

@@ -52,6 +52,31 @@ __device__ __forceinline__ bool kmb_mbar_wait(uint64_t *bar, uint32_t parity, in
     return true;
 }
 
+/* Kernels that follow one another in a call: the second is launched with
+ * kmb_launch_after and begins with kmb_wait_before, which returns when the
+ * first has ended and what it wrote is visible; the launch itself is then no
+ * longer in between: 2 to 3 us a pair (layer norm backward 4096 x 1024 bf16
+ * 18.1 -> 15.6 us).  kmb_let_after in the first: the second's CTAs may come
+ * to wait on the SM as soon as every CTA of the first has been there. */
+__device__ __forceinline__ void kmb_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void kmb_let_after() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... P>
+cudaError_t kmb_launch_after(bool after, void (*k)(P...), dim3 grid, dim3 block, size_t shared, cudaStream_t s,
+                             P... args) {
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = s;
+    cfg.attrs = &at;
+    cfg.numAttrs = after ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
 /* `bytes` (a multiple of 16, both addresses 16-byte aligned) from global to
  * this CTA's shared memory, counted on bar. */
 __device__ __forceinline__ void kmb_bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {

@@ -12,17 +12,18 @@
  * are two passes over registers.  CTAs are resident for the whole call and
  * walk the rows.  In the backward every thread keeps the column sums of its
  * own columns, written once at the end as one row of partial sums a CTA,
- * which a second kernel adds in a fixed order; a small call is one cluster,
- * whose CTAs add them through one another's shared memory.
+ * which a second kernel adds in a fixed order (it is launched before the
+ * first one ends; one launch of a cluster that adds its sums in shared memory
+ * was no faster, 128 x 384 fp32 7.2 against 6.6 us, and slower with more rows).
  *
  * Measured (B200, 6.56 TB/s copy): forward 262144 x 1024 fp32 -> bf16 246 us
  * (6.56 TB/s), 8192 x 8192 bf16 53 us (5.0 TB/s); backward with the residual
  * gradient, 262144 x 1024 fp32, 620 us (6.9 TB/s); backward 2048 x 8192 bf16
- * 37 us (2.7 TB/s: 14 rows a CTA, then a second launch), 128 x 384 fp32 6.5
- * us (the launch); rows of odd width, 16411 x 1537 bf16, 39 us (2.6 TB/s),
- * where every value is a 2-byte access to shared memory.
+ * 37 us (2.7 TB/s: 14 rows a CTA, then the sums), 4096 x 1024 bf16 15.6 us;
+ * 128 x 384 fp32 6.6 us (the launches); rows of odd width,
+ * 16411 x 1537 bf16, 39 us (2.6 TB/s), where every value is a 2-byte access
+ * to shared memory.
  */
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include "kmb_common.cuh"
@@ -533,9 +534,6 @@ __global__ void __launch_bounds__(kLoop) k_ln_fwd_loop(const __grid_constant__ K
 /* backward                                                             */
 /* ------------------------------------------------------------------ */
 
-/* sums: 0 none; kParts to the workspace, for k_ln_sums; kCluster all here */
-enum { kParts = 1, kCluster };
-
 template <typename TX, typename TY, int V, int EPT, int L, int MODE>
 __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayerNorm a, int wpr, int sums,
                                                 int stages) {
@@ -651,41 +649,25 @@ __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayer
         if (live) c.store(po, d);
     }
     if (!sums) return;
-    /* the CTA's sums to its row of the workspace, or (a cluster is the whole
-     * grid) behind `fold` in its shared memory */
-    float *fold = reinterpret_cast<float *>(smem + (RING ? ring_head(blockDim.x / 32) : 0));
-    const bool cluster = sums == kCluster;
-    float *part = cluster ? fold + (wpr > 1 ? 0 : walk.groups * (L * EPT))
-                          : (float *)a.workspace + (long)blockIdx.x * 2 * a.D;
+    float *part = (float *)a.workspace + (long)blockIdx.x * 2 * a.D;
     if (wpr > 1) {
         c.columns(part, pw);
         c.columns(part + a.D, pb);
-    } else {
-        /* one row a group: added through shared memory, the ring's stages when there is one */
+        return;
+    }
+    /* one row a group: added through shared memory, the ring's stages when there is one */
+    float *fold = reinterpret_cast<float *>(smem + (RING ? ring_head(blockDim.x / 32) : 0));
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            __syncthreads();
-            c.columns(fold + walk.group * (L * EPT), which ? pb : pw);
-            __syncthreads();
-            for (int j = threadIdx.x; j < a.D; j += blockDim.x) {
-                float v = 0.f;
-                for (int g = 0; g < walk.groups; ++g) v += fold[g * (L * EPT) + j];
-                part[which * a.D + j] = v;
-            }
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+        c.columns(fold + walk.group * (L * EPT), which ? pb : pw);
+        __syncthreads();
+        for (int j = threadIdx.x; j < a.D; j += blockDim.x) {
+            float v = 0.f;
+            for (int g = 0; g < walk.groups; ++g) v += fold[g * (L * EPT) + j];
+            part[which * a.D + j] = v;
         }
     }
-    if (!cluster) return;
-    const auto all = cooperative_groups::this_cluster();
-    all.sync();
-    for (unsigned j = blockIdx.x * blockDim.x + threadIdx.x; j < 2 * a.D; j += gridDim.x * blockDim.x) {
-        float v = 0.f;
-        for (unsigned r = 0; r < gridDim.x; ++r) v += *all.map_shared_rank(part + j, r);
-        float *to = j < a.D ? a.dweight : a.dbias;
-        if (!to) continue;
-        to += j < a.D ? j : j - a.D;
-        *to = a.accumulate ? *to + v : v;
-    }
-    all.sync(); /* no CTA leaves while its sums are read */
 }
 
 /* Wider rows: a kernel for the columns' sums (first, since dx may be x or
@@ -823,6 +805,7 @@ __global__ void __launch_bounds__(kColThreads) k_ln_cols(const __grid_constant__
 __global__ void __launch_bounds__(1024) k_ln_sums(const float *part, long parts, long D, float *dw, float *db,
                                                   int acc) {
     __shared__ float s[32][33];
+    kmb_wait_before();
     const int tx = threadIdx.x, ty = threadIdx.y, rows = blockDim.y;
     const long j = (long)blockIdx.x * 32 + tx;
     float v = 0.f;
@@ -856,16 +839,14 @@ int fwd_ept(long D) { return D <= 128 ? 16 : D <= 256 ? 8 : D <= 512 ? 16 : 32; 
 int bwd_ept(long D) { return D <= 128 ? 16 : D <= 256 ? 8 : 16; }
 constexpr long kNarrow = 128, kFwdKeep = 512 * 32, kFwdWide = 1024 * 32, kBwdMax = 512 * 16;
 
-/* Rows that a CTA has under way at once. */
-long rows_at_once(long D, int wpr) { return wpr > 1 ? 1 : D <= kNarrow ? kWarps * 4 : kWarps; }
-
 int warps_of(long D, int ept) { return D <= kNarrow ? 1 : (int)((D + 32 * ept - 1) / (32 * ept)); }
 int threads_of(int wpr) { return 32 * (wpr == 1 ? kWarps : wpr); }
 
 /* CTAs of a resident kernel of 512 threads an SM (128 registers each), no
  * more than there are rows (or groups of rows) */
 long ctas(long rows, long D, int wpr) {
-    const long per = rows_at_once(D, wpr), need = (rows + per - 1) / per;
+    const int per = wpr > 1 ? 1 : D <= kNarrow ? 4 * kWarps : kWarps;
+    const long need = (rows + per - 1) / per;
     const int fit = 512 / threads_of(wpr);
     const long most = (long)kSMs * (fit > 0 ? fit : 1);
     return need < most ? (need > 0 ? need : 1) : most;
@@ -919,7 +900,7 @@ int run_fwd(const KmbLayerNorm *a, cudaStream_t s) {
      * 262144 rows of 1024 fp32 take 249 us from global memory and 275 us
      * through a ring; of 512, 345 and 253 us. */
     const int stages = V > 1 && wpr == 1 && row >= 4096 ? 0 : ring_stages(a->D, wpr, row);
-    const long per = rows_at_once(a->D, wpr);
+    const long per = wpr > 1 ? 1 : kWarps * (32 / L);
     if (L == 32 && stages && a->rows > n * per) { /* more than a row a group */
         const size_t bytes = ring_size(wpr, row, stages);
         constexpr int E = L == 32 && V > 1 ? kWhole : kNone, P = L == 32 ? kPieces : kNone;
@@ -954,37 +935,9 @@ int fwd(const KmbLayerNorm *a, cudaStream_t s) {
     return vec ? fwd_v<TX, TY, V>(a, s) : fwd_v<TX, TY, 1>(a, s);
 }
 
-/* A small backward is one cluster of eight CTAs, which add their column sums
- * through one another's shared memory, without a second launch.  One against
- * two launches at 2, 4 and 8 rows after one another: 384 columns, 6.7 / 8.2,
- * 8.2 / 8.7 and 12.3 / 9.2 us; 96 columns, 6.2 (one row), 9.8 / 10.2 (4 rows)
- * and 21 / 10 us (16); 1024 columns, 6.2 / 8.2 us (2) and 10.3 / 8.2 us (8);
- * 4096 columns, equal with 2 rows (fp32). */
-bool one_cluster(const KmbLayerNorm *a) {
-    return a->rows && a->D <= 2048 && a->rows <= 8 * 4 * rows_at_once(a->D, warps_of(a->D, bwd_ept(a->D)));
-}
-
 template <typename TX, typename TY, int V, int EPT, int L>
 int run_bwd(const KmbLayerNorm *a, int sums, cudaStream_t s) {
     const int wpr = warps_of(a->D, EPT), t = threads_of(wpr);
-    if (sums && one_cluster(a)) {
-        const long per = rows_at_once(a->D, wpr), need = (a->rows + per - 1) / per;
-        unsigned n = 1;
-        while (n < 8 && n < need) n *= 2;
-        cudaLaunchConfig_t cfg = {};
-        cudaLaunchAttribute at[1];
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = n;
-        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-        cfg.gridDim = dim3(n);
-        cfg.blockDim = dim3((unsigned)t);
-        cfg.dynamicSmemBytes = 8 * (size_t)a->D + (wpr == 1 ? (size_t)kWarps * 32 * EPT * 4 : 0);
-        cfg.stream = s;
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, k_ln_bwd<TX, TY, V, EPT, L, kNone>, *a, wpr, (int)kCluster, 0);
-        return e == cudaSuccess ? KMB_OK : kmb_cuda_fail(e, "layernorm: launch");
-    }
     const unsigned n = (unsigned)ctas(a->rows, a->D, wpr);
     const size_t fold = sums && wpr == 1 ? (size_t)kWarps * 32 * EPT * 4 : 0;
     const bool exact = V > 1 && whole(a->x, a->ld_x, a->D, sizeof(TX)) &&
@@ -992,7 +945,7 @@ int run_bwd(const KmbLayerNorm *a, int sums, cudaStream_t s) {
     const int mode = exact ? kWhole : kPieces;
     const long row = ring_slot(a->D * sizeof(TX), mode) * (a->dres ? 2 : 1) + ring_slot(a->D * sizeof(TY), mode);
     const int stages = ring_stages(a->D, wpr, row);
-    const long per = rows_at_once(a->D, wpr);
+    const long per = wpr > 1 ? 1 : kWarps * (32 / L);
     if (L == 32 && stages && a->rows > n * per) {
         size_t bytes = ring_size(wpr, row, stages);
         if (fold && bytes < ring_head(kWarps) + fold) bytes = ring_head(kWarps) + fold;
@@ -1057,10 +1010,11 @@ int bwd(const KmbLayerNorm *a, cudaStream_t s) {
         rc = vec ? bwd_v<TX, TY, V>(a, sums, s) : bwd_v<TX, TY, 1>(a, sums, s);
     else if (a->rows)
         rc = vec ? bwd_wide<TX, TY, V>(a, sums, s) : bwd_wide<TX, TY, 1>(a, sums, s);
-    if (rc || !sums || one_cluster(a)) return rc;
-    k_ln_sums<<<(unsigned)((2 * a->D + 31) / 32), dim3(32, parts > 256 || a->D <= 2048 ? 32 : 8), 0, s>>>(
-        (const float *)a->workspace, a->rows ? parts : 0, a->D, a->dweight, a->dbias, a->accumulate);
-    return done();
+    if (rc || !sums) return rc;
+    const cudaError_t e = kmb_launch_after(
+        true, k_ln_sums, (unsigned)((2 * a->D + 31) / 32), dim3(32, parts > 256 || a->D <= 2048 ? 32 : 8), 0, s,
+        (const float *)a->workspace, a->rows ? parts : 0L, a->D, a->dweight, a->dbias, a->accumulate);
+    return e == cudaSuccess ? KMB_OK : kmb_cuda_fail(e, "layernorm: launch");
 }
 
 } // namespace

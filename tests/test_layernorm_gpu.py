@@ -214,8 +214,8 @@ def test_same_bits_every_run(lib, cuda, rows, D):
                                     (256, 511), (32, 513), (33, 513), (31, 2047), (32, 2048), (32, 2049)])
 @pytest.mark.parametrize("xt,yt", [(F32, F32), (BF16, F32), (BF16, BF16)])
 def test_few_rows(lib, cuda, rows, D, xt, yt):
-    """Around the sizes up to which one launch does rows and sums; three calls
-    that add up give three times the sums."""
+    """Fewer rows than CTAs, the rows' kernel and the sums' close together;
+    three calls that add up give three times the sums."""
     c = Case(rows, D, xt, yt, seed=rows + D)
     bwd(lib, c, res=True, stats=False)
     check_bwd(c, res=True, stats=False)
@@ -298,7 +298,7 @@ def test_graph_capture_and_shared_workspace(lib, cuda):
 
 
 def test_few_rows_captured(lib, cuda):
-    """A backward of one launch, captured and replayed on new inputs."""
+    """A short backward, captured and replayed on new inputs."""
     c = Case(100, 384)
     a = c.args()
     a.dweight, a.dbias = c.dw.data_ptr(), c.db.data_ptr()
