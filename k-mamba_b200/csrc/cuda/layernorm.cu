@@ -608,7 +608,10 @@ __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayer
                 c.template fetch<false>(pd + d_src.step, rd);
             } else { /* a lane without a row adds nothing to the columns' sums */
 #pragma unroll
-                for (int k = 0; k < C::NV; ++k) rd[k] = Vec<TY, V>{};
+                for (int k = 0; k < C::NV; ++k) {
+                    rx[k] = Vec<TX, V>{};
+                    rd[k] = Vec<TY, V>{};
+                }
             }
         } else if (here) {
             c.template load<true>((const TX *)(ring.at(ring.stage) + x_src.lead(px)), h);
@@ -617,7 +620,10 @@ __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayer
             c.template load<false>(px, h);
             c.template load<false>(pd, d);
         }
-        if (!a.mean) row_stats(red, [&](auto f) { return red.one(c.sum(h, f)); }, inv, a.eps, m, s);
+        if (!a.mean) {
+            row_stats(red, [&](auto f) { return red.one(c.sum(h, f)); }, inv, a.eps, m, s);
+            if (!live) m = s = 0.f; /* of zeros and eps = 0, rstd is infinite, and 0 times it no 0 */
+        }
         float2 t1 = kmb_f2s(0.f), t2 = t1;
         const float2 m2 = kmb_f2s(-m), sd = kmb_f2s(s);
 #pragma unroll

@@ -343,3 +343,31 @@ def test_rows_past_32_bits(lib, cuda):
     kb.check(lib, lib.kmb_layernorm_fwd(byref(a)))
     (y, _, _), (ey, _, _) = ref.ln_fwd(xv, c.w, c.b, EPS)
     within("y", c.y.np(), y, ey)
+
+
+@pytest.mark.parametrize("D", [24, 96, 128])
+@pytest.mark.parametrize("rows", [1, 5, 130, 9473])
+@pytest.mark.parametrize("stats", [False, True])
+def test_eps_zero(lib, cuda, rows, D, stats):
+    """eps = 0 divides by the rows' own spread alone.  Lanes that share a warp
+    with rows and have none (four rows a warp, up to 128 columns) add nothing
+    to the sums, although zeros have no spread."""
+    c = Case(rows, D, seed=rows + D)
+    a = c.args()
+    a.eps = 0.0
+    if stats:
+        (_, m, r), _ = ref.ln_fwd(c.xv, None, None, 0.0)
+        c.mean, c.rstd = f32(m), f32(r)
+        a.mean, a.rstd = c.mean.data_ptr(), c.rstd.data_ptr()
+    a.dweight, a.dbias = c.dw.data_ptr(), c.db.data_ptr()
+    kb.check(lib, lib.kmb_layernorm_bwd(byref(a)))
+    m, r = (c.mean.double().cpu().numpy(), c.rstd.double().cpu().numpy()) if stats else (None, None)
+    (dx, dw, db), (ex, ew, eb) = ref.ln_bwd(c.xv, c.w, c.dyv, 0.0, None, m, r)
+    within("dx", c.dx.np(), dx, ex)
+    within("dweight", c.dw.double().cpu().numpy(), dw, ew)
+    within("dbias", c.db.double().cpu().numpy(), db, eb)
+    a = c.args()
+    a.eps = 0.0
+    kb.check(lib, lib.kmb_layernorm_fwd(byref(a)))
+    (y, _, _), (ey, _, _) = ref.ln_fwd(c.xv, c.w, c.b, 0.0)
+    within("y", c.y.np(), y, ey)
