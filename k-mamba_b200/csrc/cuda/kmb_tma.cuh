@@ -37,8 +37,10 @@ __device__ __forceinline__ bool kmb_mbar_done(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 /* Waits for the phase with `parity`, at most about 2^31 cycles; then *error
- * is set, and later waits of the launch give up at once.  False when it gave
- * up. */
+ * is set.  False when it gave up.  While *error is set every wait that is not
+ * over after 16 looks gives up, of later launches too, until the host clears
+ * the word: a caller that gave up lets its copies land before it ends
+ * (kmb_mbar_done). */
 __device__ __forceinline__ bool kmb_mbar_wait(uint64_t *bar, uint32_t parity, int *error) {
     long long t0 = 0;
     for (int n = 1; !kmb_mbar_done(bar, parity); ++n) {

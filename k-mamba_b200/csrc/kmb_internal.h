@@ -105,6 +105,8 @@ int kmb_launch_gemm_bf16(const KmbGemm *g, cudaStream_t s);
 int kmb_launch_layernorm_fwd(const KmbLayerNorm *a, cudaStream_t s);
 int kmb_launch_layernorm_bwd(const KmbLayerNorm *a, cudaStream_t s);
 size_t kmb_layernorm_scratch_bytes(long rows, long D);
+/* Sets the error word as an expired wait does (tests of what comes after one). */
+int kmb_layernorm_expire(void);
 
 /* Gated linear recurrence (csrc/cuda/glr.cu); arguments already validated,
  * the workspace in place. */

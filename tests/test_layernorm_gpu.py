@@ -371,3 +371,19 @@ def test_eps_zero(lib, cuda, rows, D, stats):
     kb.check(lib, lib.kmb_layernorm_fwd(byref(a)))
     (y, _, _), (ey, _, _) = ref.ln_fwd(c.xv, c.w, c.b, 0.0)
     within("y", c.y.np(), y, ey)
+
+
+@pytest.mark.parametrize("rows,D,xt", [(4097, 300, F32), (3001, 1537, BF16), (2500, 2048, F32), (1200, 5000, BF16)])
+def test_expired_wait_is_reported(lib, cuda, rows, D, xt):
+    """The error word set on the host, as by a wait that expired: the calls
+    that find it return KMB_ETIMEOUT once, and end in order (rows through the
+    ring: copies under way, no refill); the next ones are whole again."""
+    c = Case(rows, D, xt, xt)
+    for call, check in ((fwd, check_fwd), (bwd, check_bwd)):
+        assert lib.kmb_layernorm_expire() == kb.KMB_OK
+        with pytest.raises(RuntimeError, match="a wait for a row expired"):
+            call(lib, c)
+        torch.cuda.synchronize()
+        assert lib.kmb_layernorm_check_error() == kb.KMB_OK
+        call(lib, c)
+        check(c)
