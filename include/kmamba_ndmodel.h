@@ -87,7 +87,10 @@ int kmb_ndmodel_sync_weights(KmbNDModel *m);
 int kmb_ndmodel_set_dist(KmbNDModel *m, KMambaDistributedContext *ctx);
 
 /* tokens: uint32 [batch, points], device or host memory.  loss (host) is
- * the mean cross entropy of this rank's batch. */
+ * the mean cross entropy of this rank's batch.  The calls below return
+ * KMB_ETIMEOUT when a bounded wait of the GEMMs or the layer norms gave up;
+ * after kmb_set_sync(0) the caller asks (kmb_gemm_check_error,
+ * kmb_layernorm_check_error). */
 int kmb_ndmodel_forward(KmbNDModel *m, const unsigned *tokens, long batch, float *loss);
 /* forward + backward: the gradients land in kmb_ndmodel_grads (averaged
  * over ranks when a context is attached). */

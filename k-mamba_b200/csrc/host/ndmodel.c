@@ -531,16 +531,19 @@ long kmb_ndmodel_param_count(const KmbNDModel *m) { return m ? m->n : 0; }
 float *kmb_ndmodel_params(KmbNDModel *m) { return m ? m->params : NULL; }
 float *kmb_ndmodel_grads(KmbNDModel *m) { return m ? m->grads : NULL; }
 
-static int finish(int rc) {
+/* Both words are asked, so that neither is left for a later call. */
+static int finish(const KmbNDModel *m, int rc) {
     if (rc || !kmb_sync_enabled()) return rc;
     const cudaError_t e = cudaStreamSynchronize(kmb_stream());
     if (e != cudaSuccess) return kmb_cuda_fail(e, "ndmodel: synchronize");
-    return kmb_gemm_check_error();
+    const int norm = m->pre_norm ? kmb_layernorm_check_error() : KMB_OK;
+    rc = kmb_gemm_check_error();
+    return rc ? rc : norm;
 }
 
 int kmb_ndmodel_sync_weights(KmbNDModel *m) {
     if (!m) return kmb_fail(KMB_EINVAL, "ndmodel: NULL model");
-    return finish(refresh_w16(m, kmb_stream()));
+    return finish(m, refresh_w16(m, kmb_stream()));
 }
 
 int kmb_ndmodel_set_dist(KmbNDModel *m, KMambaDistributedContext *ctx) {
@@ -623,7 +626,7 @@ int kmb_ndmodel_forward(KmbNDModel *m, const unsigned *tokens, long batch, float
         total += (double)li * (double)bi;
     }
     if (!rc && loss) *loss = (float)(total / (double)batch);
-    return finish(rc);
+    return finish(m, rc);
 }
 
 /* One pass of forward + backward over `batch` volumes; gradients are
@@ -689,7 +692,7 @@ int kmb_ndmodel_backward(KmbNDModel *m, const unsigned *tokens, long batch, floa
         total += (double)li * (double)bi;
     }
     if (!rc && loss) *loss = (float)(total / (double)batch);
-    return finish(rc);
+    return finish(m, rc);
 }
 
 int kmb_ndmodel_step(KmbNDModel *m, float lr, float weight_decay) {
@@ -701,7 +704,7 @@ int kmb_ndmodel_step(KmbNDModel *m, float lr, float weight_decay) {
     int rc = kmb_adamw(m->params, m->grads, m->m, m->v, m->n, lr, b1, b2, 1e-8f, weight_decay,
                        bc1, bc2, s);
     if (!rc) rc = refresh_w16(m, s);
-    return finish(rc);
+    return finish(m, rc);
 }
 
 int kmb_ndmodel_train_step(KmbNDModel *m, const unsigned *tokens, long batch, float lr,

@@ -107,3 +107,30 @@ def test_refusals(lib):
         assert b"norm_eps" in lib.kmb_last_error()
     assert not lib.kmb_ndmodel_create_prenorm(C.byref(config([4, 4, 4], 48, 1)), 1e-5)
     assert b"multiple of 32" in lib.kmb_last_error()
+
+
+def test_expired_wait_is_reported(lib, cuda):
+    """A layer norm whose wait gave up: the model's call that finds the word
+    returns KMB_ETIMEOUT, and the next is as it was."""
+    import torch
+    m = lib.kmb_ndmodel_create_prenorm(C.byref(config([6, 6, 6], 256, 1)), EPS)
+    plain = lib.kmb_ndmodel_create(C.byref(config([6, 6, 6], 256, 1)))
+    assert m and plain, kb.last_error(lib)
+    try:
+        tok = torch.randint(0, 256, (2, 216), dtype=torch.int32, device="cuda")
+        want, got = C.c_float(), C.c_float()
+        kb.check(lib, lib.kmb_ndmodel_forward(m, tok.data_ptr(), 2, C.byref(want)))
+        for call in (lambda: lib.kmb_ndmodel_forward(m, tok.data_ptr(), 2, C.byref(got)),
+                     lambda: lib.kmb_ndmodel_backward(m, tok.data_ptr(), 2, C.byref(got))):
+            assert lib.kmb_layernorm_expire() == kb.KMB_OK
+            assert call() == kb.KMB_ETIMEOUT
+            assert b"a wait for a row expired" in lib.kmb_last_error()
+            kb.check(lib, call())
+            assert got.value == want.value
+        # a model without norms does not ask for the word
+        assert lib.kmb_layernorm_expire() == kb.KMB_OK
+        kb.check(lib, lib.kmb_ndmodel_forward(plain, tok.data_ptr(), 2, C.byref(got)))
+    finally:
+        lib.kmb_layernorm_check_error()
+        lib.kmb_ndmodel_free(m)
+        lib.kmb_ndmodel_free(plain)
