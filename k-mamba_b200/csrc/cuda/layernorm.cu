@@ -693,12 +693,14 @@ __global__ void __launch_bounds__(512) k_ln_bwd(const __grid_constant__ KmbLayer
 
 /* Wider rows: a kernel for the columns' sums (first, since dx may be x or
  * dy), before it one for the statistics when the caller has none, and one
- * for dx, which reads the row a second time, from L2. */
+ * for dx, which reads the row a second time, from L2.  Columns are unsigned:
+ * a step behind a row of almost 2^31 passes the signed ones. */
 template <typename TX>
 __global__ void __launch_bounds__(kLoop) k_ln_stats_loop(const __grid_constant__ KmbLayerNorm a, float *mean,
                                                          float *rstd) {
     __shared__ float2 slot[2][32];
     Reducer<32> red(slot, kLoop / 32);
+    const unsigned D = (unsigned)a.D;
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const TX *x = (const TX *)a.x + r * a.ld_x;
         float m, s;
@@ -706,7 +708,7 @@ __global__ void __launch_bounds__(kLoop) k_ln_stats_loop(const __grid_constant__
             red,
             [&](auto f) {
                 float t = 0.f;
-                for (int j = threadIdx.x; j < (int)a.D; j += kLoop) t += f(kmb_f2s(ld(x + j))).x;
+                for (unsigned j = threadIdx.x; j < D; j += kLoop) t += f(kmb_f2s(ld(x + j))).x;
                 return red.one(t);
             },
             1.f / (float)a.D, a.eps, m, s);
@@ -722,7 +724,7 @@ __global__ void __launch_bounds__(kLoop) k_ln_dx_loop(const __grid_constant__ Km
     __shared__ float2 slot[2][32];
     Reducer<32> red(slot, kLoop / 32);
     const float inv = 1.f / (float)a.D;
-    const int D = (int)a.D;
+    const unsigned D = (unsigned)a.D;
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const TX *x = (const TX *)a.x + r * a.ld_x;
         const TY *dy = (const TY *)a.dy + r * a.ld_dy;
@@ -737,7 +739,7 @@ __global__ void __launch_bounds__(kLoop) k_ln_dx_loop(const __grid_constant__ Km
                 red,
                 [&](auto f) {
                     float s = 0.f;
-                    for (int j = threadIdx.x; j < D; j += kLoop) s += f(kmb_f2s(ld(x + j))).x;
+                    for (unsigned j = threadIdx.x; j < D; j += kLoop) s += f(kmb_f2s(ld(x + j))).x;
                     return red.one(s);
                 },
                 inv, a.eps, mean, rstd);
@@ -746,7 +748,7 @@ __global__ void __launch_bounds__(kLoop) k_ln_dx_loop(const __grid_constant__ Km
         /* f(column, x, g) over the thread's values, four vectors under way */
         const auto each = [&](auto f) {
 #pragma unroll 4
-            for (int j = threadIdx.x * V; j < D; j += kLoop * V) {
+            for (unsigned j = threadIdx.x * V; j < D; j += kLoop * V) {
                 Vec<TX, V> vx;
                 Vec<TY, V> vd;
                 vx.take(x + j);
@@ -762,7 +764,7 @@ __global__ void __launch_bounds__(kLoop) k_ln_dx_loop(const __grid_constant__ Km
                 f(j, h, d);
             }
         };
-        each([&](int, const float *h, const float *g) {
+        each([&](unsigned, const float *h, const float *g) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 s1 += g[e];
@@ -772,7 +774,7 @@ __global__ void __launch_bounds__(kLoop) k_ln_dx_loop(const __grid_constant__ Km
         const float2 t = red.two(s1, s2);
         s1 = t.x * inv;
         s2 = t.y * inv;
-        each([&](int j, const float *h, const float *g) {
+        each([&](unsigned j, const float *h, const float *g) {
             float o[V], q[V];
             if (res) {
                 Vec<TX, V> v;

@@ -387,3 +387,57 @@ def test_expired_wait_is_reported(lib, cuda, rows, D, xt):
         assert lib.kmb_layernorm_check_error() == kb.KMB_OK
         call(lib, c)
         check(c)
+
+
+@pytest.mark.parametrize("D", [(1 << 31) - 8, (1 << 31) - 3])
+def test_one_row_of_almost_2_31_columns(lib, cuda, D):
+    """x = 1, -1, 1, ..  dy has a few entries, at both ends; elsewhere dx is
+    what the averages leave.
+
+    Errors.  A thread's sum of x is a whole number of at most 2^22: exact.
+    Across 32 lanes and 16 warps it passes 2^24: 5 + 16 additions of values
+    whose absolute sum is D, so the mean is off by at most 21 U.  The centred
+    squares are then within 42 U of 1.  A thread adds them to a sum below
+    2^23, of which 1 is a whole number of steps: an addition is off by no more
+    than the square's distance from 1, 42 U, and the sum of all by 42 + 42 +
+    21 U; rstd by half of that and its own steps, 57 U; xhat by 21 + 57 + 2 U."""
+    x = torch.ones(D, dtype=BF16, device="cuda")
+    x[1::2] = -1
+    y, mean, rstd = torch.empty_like(x), torch.zeros(1, device="cuda"), torch.zeros(1, device="cuda")
+    a = kb.KmbLayerNorm()
+    a.x, a.y, a.mean, a.rstd = x.data_ptr(), y.data_ptr(), mean.data_ptr(), rstd.data_ptr()
+    a.rows, a.D, a.eps, a.x_type, a.y_type = 1, D, EPS, kb.KMB_BF16, kb.KMB_BF16
+    a.ld_x = a.ld_y = a.ld_dy = a.ld_dx = D
+    kb.check(lib, lib.kmb_layernorm_fwd(byref(a)))
+    m = (D % 2) / D
+    r = (1 - m * m + EPS) ** -0.5
+    assert abs(mean.item() - m) <= 21 * ref.U and abs(rstd.item() - r) <= 57 * ref.U
+    assert torch.equal(y, x)  # (1 + 1e-5)^-1/2 rounds to 1
+    del y
+    at = torch.tensor([0, 3, D - 5000, D - 2, D - 1], device="cuda")
+    v = torch.tensor([1.0, -2.0, 0.5, 4.0, -8.0], device="cuda")
+    dy = torch.zeros_like(x)
+    dy[at] = v.to(BF16)
+    rest = 2 * 15.5 / D  # |rstd (avg g + xhat avg(g xhat))| <= 2 sum |g| / D
+    for saved in (False, True):
+        for sums in (False, True):
+            dx = torch.full_like(x, SENTINEL)
+            b = kb.KmbLayerNorm.from_buffer_copy(a)
+            b.dy, b.dx = dy.data_ptr(), dx.data_ptr()
+            if not saved:
+                b.mean = b.rstd = None
+            if sums:
+                dw, db = (torch.full((D,), SENTINEL, device="cuda") for _ in range(2))
+                ws = torch.empty(lib.kmb_layernorm_workspace_bytes(byref(b)), dtype=torch.uint8, device="cuda")
+                b.dweight, b.dbias, b.workspace, b.workspace_bytes = dw.data_ptr(), db.data_ptr(), ws.data_ptr(), ws.numel()
+            kb.check(lib, lib.kmb_layernorm_bwd(byref(b)))
+            if sums:
+                assert bool(((dw[at] - v * x[at] * r).abs() <= 82 * ref.U * v.abs()).all())
+                assert torch.equal(db[at], v)
+                dw[at] = db[at] = 0
+                assert not bool(dw.any()) and not bool(db.any())
+                del dw, db, ws
+            assert bool(((dx[at].float() - v * r).abs() <= 2.0 ** -8 * v.abs()).all())
+            dx[at] = 0
+            assert dx.max().item() <= rest and dx.min().item() >= -rest
+            del dx
