@@ -441,3 +441,57 @@ def test_one_row_of_almost_2_31_columns(lib, cuda, D):
             dx[at] = 0
             assert dx.max().item() <= rest and dx.min().item() >= -rest
             del dx
+
+
+# Enough rows for the ring of copies in both directions (more than a row for
+# each warp, or CTA, of the resident grid).  Up to 1024 columns (backward 512)
+# a warp has a row, above that several.  Whole pieces, vectors: rows that
+# begin and end on 16 bytes.  Shared pieces, vectors: bf16 rows of a multiple
+# of four columns beside fp32 ones.  Shared pieces, single values: the rest.
+RING = [(2500, 512, 0, 0), (2500, 1024, 8, 8), (1300, 2048, 0, 0), (500, 8192, 0, 0), (400, 20000, 0, 0),
+        (2500, 300, 0, 4), (2500, 388, 0, 0), (1300, 2052, 4, 4), (500, 5004, 0, 4),
+        (2500, 257, 0, 0), (2500, 257, 3, 1), (2500, 771, 0, 1), (2500, 771, 5, 0), (2500, 1025, 0, 0),
+        (2500, 1537, 5, 0), (2500, 1537, 5, 1), (2500, 1537, 0, 1), (1300, 2049, 0, 3), (1300, 2049, 7, 0),
+        (500, 5001, 0, 0), (500, 5001, 3, 1), (500, 8191, 1, 1)]
+
+
+@pytest.mark.parametrize("xt,yt", [(F32, F32), (F32, BF16), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("rows,D,gap,shift", RING)
+def test_ring(lib, cuda, rows, D, gap, shift, xt, yt):
+    c = Case(rows, D, xt, yt, gap, shift, seed=rows + D)
+    fwd(lib, c)
+    check_fwd(c)
+    for res, stats in ((False, True), (True, False)):
+        bwd(lib, c, res=res, stats=stats)
+        check_bwd(c, res=res, stats=stats)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("rows,D,gap,shift", [(2500, 512, 0, 0), (2500, 300, 0, 1), (2500, 771, 0, 1), (2500, 1537, 5, 1),
+                                              (1300, 2048, 0, 0), (1300, 2049, 0, 3), (500, 5001, 0, 1)])
+def test_ring_in_place(lib, cuda, rows, D, gap, shift, t):
+    """Outputs over inputs whose later rows, and whose neighbours' bytes, are
+    being copied meanwhile."""
+    mk = lambda: Case(rows, D, t, t, gap, shift, seed=rows + D)  # noqa: E731
+    c = mk()
+    a = c.args()
+    a.y = a.x
+    kb.check(lib, lib.kmb_layernorm_fwd(byref(a)))
+    (y, _, _), (ey, _, _) = ref.ln_fwd(c.xv, c.w, c.b, EPS)
+    within("y", c.x.np(), y, ey, t)
+    (dx, dw, db), (ex, ew, eb) = ref.ln_bwd(c.xv, c.w, c.dyv, EPS, c.resv)
+    for target in ("x", "dy", "res"):
+        c = mk()
+        a = c.args()
+        a.dres, a.ld_dres = c.res.t.data_ptr(), c.res.ld
+        a.dweight, a.dbias = c.dw.data_ptr(), c.db.data_ptr()
+        o = getattr(c, target)
+        a.dx, a.ld_dx = o.t.data_ptr(), o.ld
+        kb.check(lib, lib.kmb_layernorm_bwd(byref(a)))
+        within("dx", o.np(), dx, ex, t)
+        within("dweight", c.dw.double().cpu().numpy(), dw, ew)
+        within("dbias", c.db.double().cpu().numpy(), db, eb)
+        # what lies around the rows is as it was (NaN)
+        f = o.flat.clone()
+        f.as_strided(o.t.shape, o.t.stride(), o.t.storage_offset()).fill_(float("nan"))
+        assert bool(f.isnan().all())
