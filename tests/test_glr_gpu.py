@@ -655,3 +655,42 @@ def test_rows_past_32_bits(lib, cuda):
     c.x.t.copy_(torch.from_numpy(c.v["x"]).to(BF16))
     run(lib, c)
     c.check(*c.ref(), ALL)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("batch,L,D,spare", [(3, 1200, 520, 0), (3, 1121, 520, 40), (1, 5600, 264, 8), (2, 1300, 1032, 3)])
+def test_resident_kernels_on_slices(lib, cuda, batch, L, D, spare, packed, dtype):
+    """More tiles than SMs on the three parts of one projection, whose width is
+    no multiple of a tile's 64 channels: a tile's last columns reach into the
+    part beside it, which it neither takes nor writes.  `spare` rows of another
+    kind lie behind every sequence (batch strides above L rows)."""
+    total = batch * L
+    off = [0, 0, 300, 301, total - 7, total] if packed else None
+    c = Case(5 if packed else batch, total if packed else L, D, dtype, offsets=off, seed=D + L)
+    lead = (1, total) if packed else (batch, L)
+    parts = {}
+    for names in (("x", "gate_r", "gate_i"), ("dx", "dgate_r", "dgate_i"), ("y", "dy")):
+        p = torch.full((lead[0], lead[1] + spare, len(names) * D + 16), SENTINEL, dtype=dtype, device="cuda")
+        for k, n in enumerate(names):
+            part = p[:, :lead[1], 8 + k * D:8 + (k + 1) * D]
+            if n in c.v:
+                part.copy_(torch.from_numpy(c.v[n]).to(dtype).view(part.shape))
+            getattr(c, n).t = part[0] if packed else part
+        parts[names] = p
+    before = {k: p.clone() for k, p in parts.items()}
+    for ckpt in (True, False):
+        for k, p in parts.items():
+            p.copy_(before[k])
+        run(lib, c, ckpt=ckpt)
+        v, e = c.ref()
+        c.check(v, e, ("h_last", "dh0", "ddecay"))
+        for k in OUT:
+            within(k, getattr(c, k).np().reshape(-1, D), v[k], e[k], dtype)
+        for names, p in parts.items():
+            after, was = p.clone(), before[names]
+            for n in names:
+                if n in OUT:
+                    k = names.index(n)
+                    after[:, :lead[1], 8 + k * D:8 + (k + 1) * D] = SENTINEL
+            assert torch.equal(after, was), names
