@@ -134,3 +134,38 @@ def test_expired_wait_is_reported(lib, cuda):
         lib.kmb_layernorm_check_error()
         lib.kmb_ndmodel_free(m)
         lib.kmb_ndmodel_free(plain)
+
+
+def test_gradients_through_a_communicator(lib, cuda):
+    """With a communicator of one rank, whose mean is the gradient itself:
+    every gradient goes through the buckets once, the norms' among them, and
+    is the same but for the order of the weight gradients' atomic sums."""
+    import torch
+    cfg = config([6, 6, 6], 64, 2)
+    uid = C.create_string_buffer(128)
+    assert lib.kmb_dist_get_unique_id(uid) == kb.KMB_OK
+    ctx = lib.kmb_dist_init_with_id(1, 0, torch.cuda.current_device(), uid)
+    assert ctx, kb.last_error(lib)
+    m = lib.kmb_ndmodel_create_prenorm(C.byref(cfg), EPS)
+    assert m, kb.last_error(lib)
+    try:
+        n = lib.kmb_ndmodel_param_count(m)
+        tok = torch.randint(0, 256, (2, 216), dtype=torch.int32, device="cuda")
+        loss = C.c_float()
+        kb.check(lib, lib.kmb_ndmodel_backward(m, tok.data_ptr(), 2, C.byref(loss)))
+        want = device_array(lib.kmb_ndmodel_grads(m), n)
+        kb.check(lib, lib.kmb_ndmodel_set_dist(m, ctx))
+        first, last = C.c_ulonglong(), C.c_ulonglong()
+        lib.kmb_dist_stats(ctx, None, C.byref(first))
+        kb.check(lib, lib.kmb_ndmodel_backward(m, tok.data_ptr(), 2, C.byref(loss)))
+        torch.cuda.synchronize()
+        lib.kmb_dist_stats(ctx, None, C.byref(last))
+        assert last.value - first.value == 4 * n
+        got = device_array(lib.kmb_ndmodel_grads(m), n)
+        norms = 2 * 3 * 64
+        assert np.abs(want[-norms:]).max() > 0
+        assert norm_err(got[-norms:], want[-norms:]) <= 1e-5 and norm_err(got, want) <= 1e-5
+        kb.check(lib, lib.kmb_ndmodel_set_dist(m, None))
+    finally:
+        lib.kmb_ndmodel_free(m)
+        lib.kmamba_distributed_fini_nccl(ctx)
