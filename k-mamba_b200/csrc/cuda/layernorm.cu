@@ -919,10 +919,13 @@ int run_fwd(const KmbLayerNorm *a, cudaStream_t s) {
     const unsigned n = (unsigned)ctas(a->rows, a->D, wpr);
     const bool exact = V > 1 && whole(a->x, a->ld_x, a->D, sizeof(TX));
     const long row = ring_slot(a->D * sizeof(TX), exact ? kWhole : kPieces);
-    /* Rows of 4 KB, one a warp, keep 64 KB of an SM under way by themselves:
-     * 262144 rows of 1024 fp32 take 249 us from global memory and 275 us
-     * through a ring; of 512, 345 and 253 us. */
-    const int stages = V > 1 && wpr == 1 && row >= 4096 ? 0 : ring_stages(a->D, wpr, row);
+    /* Long rows, one a warp (fp32, up to 1024 columns), keep 64 KB of an SM
+     * under way by themselves.  From global memory and through the ring, 100M
+     * values: fp32 -> fp32 1024 columns 132 and 139 us, 1000 130 and 141, 896
+     * 128 and 142, 768 131 and 145, 640 145 and 151, 520 162 and 142; fp32 ->
+     * bf16 1024 94 and 102, 1000 100 and 109, 896 104 and 111, 768 111 and
+     * 106, 640 123 and 103, 520 142 and 126.  Both gain from 896 columns on. */
+    const int stages = V > 1 && wpr == 1 && row >= 3584 ? 0 : ring_stages(a->D, wpr, row);
     const long per = wpr > 1 ? 1 : kWarps * (32 / L);
     if (L == 32 && stages && a->rows > n * per) { /* more than a row a group */
         const size_t bytes = ring_size(wpr, row, stages);
