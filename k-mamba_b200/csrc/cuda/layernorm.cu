@@ -1037,8 +1037,12 @@ int bwd(const KmbLayerNorm *a, cudaStream_t s) {
     else if (a->rows)
         rc = vec ? bwd_wide<TX, TY, V>(a, sums, s) : bwd_wide<TX, TY, 1>(a, sums, s);
     if (rc || !sums) return rc;
+    /* Rows of threads of the sums' kernel: many where its CTAs are few.  Of a
+     * call with 8 and 32, fp32: 2048 x 1024 16.4 and 14.4 us, 4096 x 1024 20.5
+     * and 18.5, 4096 x 2048 24.8 and 24.6; 4096 x 2560 28.7 and 30.8, 4096 x
+     * 4096 39.0 and 41.2, 2048 x 8192 41.0 and 46.0, 64 x 8192 8.3 and 14.4. */
     const cudaError_t e = kmb_launch_after(
-        true, k_ln_sums, (unsigned)((2 * a->D + 31) / 32), dim3(32, parts > 256 || a->D <= 2048 ? 32 : 8), 0, s,
+        true, k_ln_sums, (unsigned)((2 * a->D + 31) / 32), dim3(32, a->D <= 2048 ? 32 : 8), 0, s,
         (const float *)a->workspace, a->rows ? parts : 0L, a->D, a->dweight, a->dbias, a->accumulate);
     return e == cudaSuccess ? KMB_OK : kmb_cuda_fail(e, "layernorm: launch");
 }
