@@ -296,7 +296,8 @@ int kmb_gemm_check_error(void);
  * types x_type and y_type (an fp32 residual stream normalised into bf16
  * GEMM operands is x_type KMB_F32, y_type KMB_BF16).  weight and bias are
  * fp32 [D]; NULL stands for ones / zeros.  mean and rstd are optional fp32
- * [rows] outputs.
+ * [rows] outputs.  eps may be 0 (a row of one value is then not finite).
+ * x - mean has to be finite in fp32.
  *
  * Backward: reads x, weight, dy (y_type, ld_dy) and either the forward's
  * mean and rstd or, when both are NULL, computes them again from x and
@@ -306,8 +307,8 @@ int kmb_gemm_check_error(void);
  * dx is of x_type (ld_dx).  dres (optional, x_type, ld_dres) is the
  * gradient that reaches x by another way, the residual path of a pre-norm
  * block.  dweight / dbias are optional fp32 [D], overwritten, or added to
- * when accumulate is 1; their sums run in a fixed order (the same bits
- * every run).
+ * when accumulate is 1; their sums are held in fp32 and run in a fixed order
+ * (the same bits every run).
  *
  * y may be the very tensor x, and dx the very tensor x, dy or dres (same
  * pointer, type and row stride); any other overlap of an output with
@@ -372,6 +373,14 @@ size_t kmb_layernorm_workspace_bytes(const KmbLayerNorm *args);
  * (KMB_F32 or KMB_BF16); decay (finite), h0, h_last, ckpt, dh_last, dh0 and ddecay
  * are fp32, and so is every state and sum.
  *
+ * Precision.  With rates scale softplus(decay) of at most 1/4 the recurrence
+ * runs on a - 1, else on a, which next to 1 holds 1 - a to 2^-25 / (1 - a).
+ * Which of them is decided for 64 channels together (those from a multiple of
+ * 64 on), in kmb_glr_step for each channel alone: beside a channel that forgets
+ * fast, one with a long memory has the second form's error, and a prefill and
+ * the steps after it may differ by as much.  A state that is infinite may
+ * become NaN at the next row.
+ *
  * Sequences, without offsets: `batch` sequences of L rows.  Each tensor is
  * a KmbRows: row t of sequence b begins at data + b batch_stride + t
  * row_stride (elements; channels are contiguous, both strides >= D, so
@@ -380,7 +389,8 @@ size_t kmb_layernorm_workspace_bytes(const KmbLayerNorm *args);
  * With offsets (device int64 [batch + 1], not decreasing, 0 <= offset <=
  * L): sequence b has the packed rows offsets[b] .. offsets[b + 1] - 1 of
  * tensors with L rows; batch_stride is not read.  Sequences may be empty.
- * Rows outside every sequence are neither read nor written.
+ * Rows outside every sequence are not written and nothing in them is used;
+ * they may be read (aligned tensors are loaded a tile of rows at a time).
  *
  * h0 (may be NULL: zeros), h_last, dh_last (may be NULL: zeros) and dh0
  * are [batch, D]; the outputs among them are optional.  h_last of an empty
@@ -458,7 +468,9 @@ int kmb_glr_check_error(void);
  * slots NULL: state k), which is advanced by one step in place and written
  * to y.  A row whose slot is negative or >= n_states (padding) is left out:
  * nothing of it is read or written.  Of several rows that name one slot
- * the first is taken, and nothing of the others is written.
+ * the first is taken, and nothing of the others is written; they are found by
+ * comparing each row's slot with those before it, rows^2 / 2 comparisons for
+ * every 128 to 512 channels (none when slots is NULL).
  */
 typedef struct {
     KmbRows x;

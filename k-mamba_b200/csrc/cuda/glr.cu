@@ -12,8 +12,9 @@
  * (dL/du goes through a and through the root; u times the root's share is
  * kappa b, so nothing divides by a vanishing root: kappa -> 1/2 at u = 0.)
  *
- * Both directions are one pass over the data.  A CTA takes a tile of rows x
- * channels: a warp owns a run of consecutive rows, a lane 2 or 4 channels.
+ * Both directions are one pass over the data (a single-pass scan with
+ * decoupled look-back).  A CTA takes a tile of rows x
+ * channels: a warp owns a run of consecutive rows, a lane two channels.
  * A run is first reduced to its affine map h -> A h + H, the maps of a
  * tile's warps are joined through shared memory, and the maps of the tiles
  * of one channel group through global memory: a tile publishes its map,
@@ -187,9 +188,9 @@ __device__ __forceinline__ float sqrt_mufu(float v) {
  * Polynomials of the exponent u on [0, kWeak], fitted for minimax relative
  * error with the constant term held (iteratively reweighted least squares
  * on Chebyshev nodes); in fp32 Horner form each is within 7e-8:
- *   (e^-u - 1) / u                    2.9e-9 in real arithmetic
- *   sqrt((1 - e^-2u) / (2 u))         4.8e-9
- *   kappa = u / (e^2u - 1)            3.4e-9
+ *   (e^-u - 1) / u                    3.0e-9 in real arithmetic, as stored
+ *   sqrt((1 - e^-2u) / (2 u))         5.1e-9
+ *   kappa = u / (e^2u - 1)            6.6e-9
  * A channel whose rate is at most kWeak needs no exponential of u, no
  * square root and no cancelling 1 - a^2, and its recurrence runs on a - 1
  * as h + (b + (a - 1) h): a memory of 1 / (1 - a) steps multiplies the error
@@ -953,8 +954,9 @@ __device__ __forceinline__ F<kV> any_backward(const Dev &p, const Place &at, con
     return run.backward_rows(C, t, ends, f);
 }
 
-/* CTAs of an SM: 64 registers a thread do for 4 rows, 237 against 262 us with
- * 128 (24001 x 771 fp32); 8 rows would spill */
+/* CTAs of an SM.  Four of 4 rows (72 registers a thread, 112 to 212 bytes of
+ * it spilled) take 237 us, three 262 and two (128 registers) 260 (24001 x 771
+ * fp32).  8 rows spill 56 to 248 bytes with two CTAs already. */
 template <typename T>
 constexpr int kBCtas = sizeof(T) == 2 ? 2 : 4;
 
@@ -1565,8 +1567,14 @@ bool tensor_ok(const KmbGLR *a, const KmbRows &r) {
 
 /*
  * The plan of a direction: the resident kernel where the tensors allow it
- * and there are more tiles than half of its CTAs, else the kernel for any
- * alignment, one CTA a tile.
+ * and there is a tile for each SM, else the kernel for any alignment, one CTA
+ * a tile.  Below that the two are close, above it the resident one gains.
+ * Forward + backward, by threads and resident, us (tiles of the forward):
+ *   1 x 1024 x 128 (38)     fp32  9.1 + 14.4, 10.3 + 13.3   bf16  8.8 + 12.4, 10.3 + 12.4
+ *   1 x 1024 x 512 (152)    fp32 10.3 + 16.5, 10.3 + 14.6   bf16 10.2 + 14.4, 10.3 + 14.0
+ *   4 x 1024 x 256 (304)    fp32 10.6 + 20.4, 12.3 + 18.5   bf16 10.3 + 16.5, 12.0 + 16.2
+ *   1 x 16384 x 128 (586)   fp32 39.0 + 91.4, 26.7 + 52.9   bf16 37.4 + 48.9, 25.4 + 31.9
+ *   8 x 1024 x 512 (1216)   fp32 22.6 + 43.0, 22.6 + 38.5   bf16 20.5 + 41.0, 18.6 + 28.5
  */
 template <typename T>
 Plan plan_of(const KmbGLR *a, bool bwd) {
@@ -1807,7 +1815,10 @@ static int launch_step(const KmbGLRStep *a, cudaStream_t s) {
     bool vec = a->D % 4 == 0 && (size_t)a->state % 16 == 0 && a->ld_state % 4 == 0;
     for (const KmbRows *r : {&a->x, &a->gate_r, &a->gate_i, &a->y})
         vec = vec && (size_t)r->data % (4 * es) == 0 && r->row_stride % 4 == 0;
-    /* a few rows are a matter of latency: one channel a thread */
+    /* A few rows are a matter of latency: one channel a thread.  Scalars and
+     * vectors, us: 64 x 1536 4.2 both, 128 x 1536 fp32 4.2 and 5.1, 64 x 4096
+     * 6.2 and 5.2, 256 x 1536 6.2 both, 512 x 1024 8.2 and 6.2; of narrow rows
+     * vectors leave most of a CTA without work: 2000 x 128 6.2 and 8.2. */
     if (a->rows * a->D < 4L * kSMs * kStepThreads) vec = false;
     const long per = kStepThreads * (vec ? 4 : 1), tiles = (a->D + per - 1) / per;
     if (a->rows >= (1L << 31) / tiles) return kmb_fail(KMB_EUNSUPPORTED, "glr: too many rows");

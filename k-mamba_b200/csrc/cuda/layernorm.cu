@@ -12,9 +12,10 @@
  * are two passes over registers.  CTAs are resident for the whole call and
  * walk the rows.  In the backward every thread keeps the column sums of its
  * own columns, written once at the end as one row of partial sums a CTA,
- * which a second kernel adds in a fixed order (it is launched before the
- * first one ends; one launch of a cluster that adds its sums in shared memory
- * was no faster, 128 x 384 fp32 7.2 against 6.6 us, and slower with more rows).
+ * which a second kernel adds in a fixed order (its launch is under way when
+ * the first one's CTAs end; one launch of a cluster that adds its sums in
+ * shared memory was no faster, 128 x 384 fp32 7.2 against 6.6 us, and slower
+ * with more rows).
  *
  * Measured (B200, 6.56 TB/s copy): forward 262144 x 1024 fp32 -> bf16 246 us
  * (6.56 TB/s), 8192 x 8192 bf16 53 us (5.0 TB/s); backward with the residual
