@@ -374,7 +374,8 @@ size_t kmb_layernorm_workspace_bytes(const KmbLayerNorm *args);
  * are fp32, and so is every state and sum.
  *
  * Precision.  With rates scale softplus(decay) of at most 1/4 the recurrence
- * runs on a - 1, else on a, which next to 1 holds 1 - a to 2^-25 / (1 - a).
+ * runs on a - 1, else on a, which next to 1 holds 1 - a to a relative
+ * 2^-25 / (1 - a).
  * Which of them is decided for 64 channels together (those from a multiple of
  * 64 on), in kmb_glr_step for each channel alone: beside a channel that forgets
  * fast, one with a long memory has the second form's error, and a prefill and

@@ -191,9 +191,9 @@ __device__ __forceinline__ float sqrt_mufu(float v) {
  *   (e^-u - 1) / u                    3.0e-9 in real arithmetic, as stored
  *   sqrt((1 - e^-2u) / (2 u))         5.1e-9
  *   kappa = u / (e^2u - 1)            6.6e-9
- * A channel whose rate is at most kWeak needs no exponential of u, no
- * square root and no cancelling 1 - a^2, and its recurrence runs on a - 1
- * as h + (b + (a - 1) h): a memory of 1 / (1 - a) steps multiplies the error
+ * A tile's channels whose rates are all at most kWeak need no exponential of
+ * u, no square root and no cancelling 1 - a^2, and their recurrence runs on
+ * a - 1 as h + (b + (a - 1) h): a memory of 1 / (1 - a) steps multiplies the error
  * of the decay, and a itself, next to 1, cannot hold it to more than
  * 2^-25 / (1 - a).
  */
